@@ -10,6 +10,9 @@
  * File:line citations name the reference interface (paths inside the Kitty
  * project, src/kitty/...) that the entry point replaces.
  *
+ * The entry points at the end (rotary positions, prompt attention, the 8-bit cache)
+ * have no counterpart in the reference.
+ *
  * Geometry is fixed to what the reference hard-codes (kvcache/kitty.py:43-47):
  * page = 128 tokens, head_dim = 128, 32 boosted channels, sink = 32 tokens.
  * Anything else is rejected with KITTY_E_BADSHAPE.
@@ -336,6 +339,105 @@ int64_t kitty_lse_exchange_bytes(int64_t rows, int32_t world, int64_t *flag_offs
 int kitty_lse_exchange_merge(const float *local_partial, int64_t rows, void *const *peer_buffers, int32_t rank,
                              int32_t world, int32_t seq, void *out, int out_dtype, int32_t *status, int64_t wait_ns,
                              void *stream);
+
+/* ---- Rotary positions of prompts and tokens ------------------------------------------------
+ * (No counterpart in the reference, whose models call the element-wise sequence of
+ * models/qwen3/modeling_qwen3.py:222-232.)  Pair p of a head is turned by angle position * w_p and multiplied by
+ * `factor`; channels from rotary_dim on keep their value.  Angles are formed in 64 bits, the rotation in 32 bits with
+ * one rounding to the data type at the end (kitty_rope_qk rounds every product, as its models do). */
+typedef enum {
+  KITTY_ROPE_HALF = 0,       /* pair p = channels p and p + rotary_dim/2 */
+  KITTY_ROPE_INTERLEAVED = 1 /* pair p = channels 2p and 2p + 1          */
+} kitty_rope_layout;
+
+typedef struct {
+  const double *turns;   /* DEVICE array [rotary_dim / 2]: w_p / (2 pi), the turns per position of each pair */
+  float factor;          /* on cosine and sine (1 unless the scaling asks for more)                        */
+  int32_t rotary_dim;    /* even, 2 .. 128                                                                  */
+  int32_t layout;        /* kitty_rope_layout                                                               */
+  int32_t reserved;
+} kitty_rotary_plan;
+
+/* q [B, h_q, T, 128] and k [B, h_kv, T, 128] of `dtype` (any of the three) turned into q_out / k_out.  positions:
+ * device int64, row b at positions + b*pos_stride_b (0: one row for all), T values each.  strides: HOST array of
+ * twelve element strides, (batch, head, token) of q, k, q_out and k_out; channels are consecutive and every row starts
+ * on a 16-byte boundary.  An output may be its own input (in place); any other overlap is the caller's error.
+ * h_q or h_kv may be 0. */
+int kitty_rotary(const kitty_rotary_plan *plan, const void *q, const void *k, const int64_t *positions,
+                 int64_t pos_stride_b, void *q_out, void *k_out, int dtype, int32_t B, int32_t T, int32_t h_q,
+                 int32_t h_kv, const int64_t *strides, void *stream);
+
+/* ---- Attention over a whole prompt ---------------------------------------------------------
+ * (No counterpart in the reference, which hands the prompt to the model's library attention,
+ * models/qwen3/modeling_qwen3.py:228-242.)  Causal (or full) attention of query rows over keys and values in hand,
+ * grouped heads, head_dim 128, fp16 or bf16, on the tcgen05 tensor cores.
+ *
+ * Dense form (cu_q null): q [B, h_q, Lq, 128], k / v [B, h_kv, Lk, 128].  q_lens / k_lens: device int32 [B] or null
+ * (every row Lq / Lk); rows of a right-padded batch from q_lens[b] on are written as zeros.
+ * Packed form (cu_q not null): B = number of sequences, q [Lq, h_q, 128] and k / v [Lk, h_kv, 128] hold all of them one
+ * after the other, sequence s at rows cu_q[s] .. cu_q[s+1] (device int32 [B+1]; cu_k null: the same for the keys).
+ * Rows behind the last sequence are left as they are, or written as zeros when zero_rest is non-zero.
+ * causal: the last query of a sequence sees its last key, query i sees keys 0 .. i + (keys - queries).  A row that
+ * sees no key is zero.  Keys and values that a row does not see never reach its result, whatever they hold.
+ * strides: HOST array of nine element strides, (batch, head, token) of q, k and v (batch ignored when packed).
+ * out: contiguous [B, Lq, h_q, 128] or [Lq, h_q, 128] of the same type.  scaling: positive and finite.
+ * status: device int32 or null, set to 1 when a bounded device-side wait ran out. */
+int kitty_prompt_attn(const void *q, const void *k, const void *v, int dtype, const int64_t *strides, int32_t B,
+                      int64_t Lq, int64_t Lk, int32_t h_q, int32_t h_kv, float scaling, int causal,
+                      const int32_t *q_lens, const int32_t *k_lens, const int32_t *cu_q, const int32_t *cu_k,
+                      void *out, int zero_rest, int32_t *status, void *stream);
+
+/* ---- The 8-bit cache --------------------------------------------------------------------------
+ * (No counterpart in the reference; for layers or models that two bits per value hurt.)  Pages of 128 tokens behind a
+ * page table, as in the 2-bit cache; a page holds four blocks of 32 tokens of every head, and a block holds its keys
+ * and its values as whole numbers -127..127 with one fp32 scale each: scale = max|x| / 127 (1 if all are zero), code =
+ * 127 x / max|x| rounded to the nearest, halves away from zero.  A block with an infinity or NaN gets scale NaN.  The
+ * tokens of a row's open block (length % 32 of them) stay in 16 bits.  What is stored does not depend on how the
+ * tokens were cut into calls.  The caller keeps the lengths; every call takes them as a device array, so the calls can
+ * be captured in a CUDA graph and replayed.
+ *
+ * Block record (8208 bytes, byte = code + 128): 4096 B keys | 4096 B values | key scale, value scale (fp32) | 8 B.
+ * Keys: 16-byte piece (i, half, lane = 4g + t) = channels 64*half + 16t ... + 15 of token 8*(g/2) + 2i + g%2.
+ * Values: piece (x, lane) = channel 16x + g, tokens 8t ... 8t+7, then channel 16x + 8 + g, the same tokens: the order
+ * in which the attention kernel's lanes hold them as matrix operands. */
+#define KITTY_KV8_BLOCK 32
+#define KITTY_KV8_RECORD 8208
+
+typedef struct {
+  int32_t max_bs, max_page, num_pages, h_kv, head_dim, dtype; /* dtype: F16 or BF16, of tails, inputs and outputs */
+  uint8_t *pages;             /* u8 [num_pages, h_kv, 4, 8208]                         */
+  void *tail_k, *tail_v;      /* dtype [max_bs, h_kv, 32, 128]                         */
+  const int64_t *page_table;  /* i64 [max_bs, max_page], entries 0 .. num_pages - 1     */
+  int32_t *status;            /* device int32: bits below are set, never cleared        */
+} kitty_kv8_layer;
+
+#define KITTY_KV8_BAD_PAGE 1   /* a page-table entry out of range: its block was skipped             */
+#define KITTY_KV8_BAD_LENGTH 2 /* a length or start outside 0 .. 128*max_page: it was clamped        */
+#define KITTY_KV8_TIMEOUT 4    /* a bounded device-side wait ran out                                 */
+
+/* Tokens key / value [B, h_kv, T, 128] (element strides (batch, head, token) in the HOST array strides: key, value,
+ * query) become tokens start[b], start[b] + 1, ... of row b; counts[b] of them (null: all T).  With a rotary plan the
+ * keys are turned on the way by their position in the row, and rounded to the data type before they are stored; the
+ * query rows [B, h_q, T, 128] (or null, h_q = 0) are turned by the same positions into q_out [B, h_q, T, 128]
+ * (contiguous), all T of them.  Tokens that end up in an open block go to the tails, others into their pages: a
+ * token-by-token caller and one that gives the whole prompt leave the same bytes. */
+int kitty_kv8_append(const kitty_kv8_layer *layer, const void *key, const void *value, const int64_t *strides,
+                     const int32_t *start, const int32_t *counts, int32_t B, int32_t T,
+                     const kitty_rotary_plan *rotary, const void *query, void *q_out, int32_t h_q, void *stream);
+
+/* Tokens start[b] .. start[b] + n - 1 of every row (start null: from 0) as values of the layer's type, k_out / v_out
+ * [B, h_kv, n, 128] contiguous.  lengths: device int32 [B], what the rows hold; tokens behind it are zeros. */
+int kitty_kv8_expand(const kitty_kv8_layer *layer, const int32_t *lengths, const int32_t *start, void *k_out,
+                     void *v_out, int32_t B, int32_t n, void *stream);
+
+/* One query token per row over the tokens the row holds (lengths: device int32 [B]; 0 gives zeros).  query
+ * [B, h_q, 1, 128] and out [B, 1, h_q, 128], contiguous, of the layer's type; up to 16 query heads per key head,
+ * B <= KITTY_KV8_MAX_BATCH.  workspace: kitty_kv8_workspace_bytes, 16-byte aligned, no initial contents; calls that
+ * share one must not overlap. */
+#define KITTY_KV8_MAX_BATCH 2048
+int64_t kitty_kv8_workspace_bytes(int32_t B, int32_t h_kv, int32_t h_q);
+int kitty_kv8_attn(const kitty_kv8_layer *layer, const int32_t *lengths, const void *query, int32_t B, int32_t h_q,
+                   float scaling, void *out, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -17,6 +17,9 @@ STATIC_SCRATCH_BYTES = 8 << 20
 KITTY_F16, KITTY_BF16, KITTY_F32 = 0, 1, 2
 SELECT_FUSED, SELECT_SUPPLIED = 0, 1
 DIV_IEEE, DIV_FULL = 0, 1
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+KV8_BLOCK, KV8_RECORD, KV8_MAX_BATCH = 32, 8208, 2048
+KV8_BAD_PAGE, KV8_BAD_LENGTH, KV8_TIMEOUT = 1, 2, 4
 
 EXPORTS = [
     "kitty_version", "kitty_strerror", "kitty_quant_pack_k", "kitty_quant_pack_v", "kitty_quant_pack_kv",
@@ -25,7 +28,8 @@ EXPORTS = [
     "kitty_lse_merge", "kitty_decode_attn_static", "kitty_plan_step", "kitty_decode_step",
     "kitty_lse_exchange_bytes", "kitty_lse_exchange_merge", "kitty_decode_attn_exchange", "kitty_rope_qk",
     "kitty_plan_step_split", "kitty_decode_step_exchange", "kitty_append_rows", "kitty_flush_rows",
-    "kitty_decode_attn_rows",
+    "kitty_decode_attn_rows", "kitty_rotary", "kitty_prompt_attn", "kitty_kv8_append", "kitty_kv8_expand",
+    "kitty_kv8_workspace_bytes", "kitty_kv8_attn",
 ]
 
 
@@ -51,6 +55,23 @@ class KittyStepState(C.Structure):
                [(n, C.c_int32) for n in ("pb", "pe", "ch", "nchunk", "has_sink", "has_tail", "n_slots", "n_tiles",
                                          "chunk_slot0", "edge_slot", "n_items", "n_edge", "flush_k", "flush_v",
                                          "edge_parts", "edge_part_tok", "xchg_seq", "reserved")]
+
+
+class KittyRotaryPlan(C.Structure):
+    """struct kitty_rotary_plan"""
+    _fields_ = [("turns", C.c_void_p), ("factor", C.c_float), ("rotary_dim", C.c_int32), ("layout", C.c_int32),
+                ("reserved", C.c_int32)]
+
+
+class KittyKV8Layer(C.Structure):
+    """struct kitty_kv8_layer"""
+    _fields_ = [(n, C.c_int32) for n in ("max_bs", "max_page", "num_pages", "h_kv", "head_dim", "dtype")] + \
+               [(n, C.c_void_p) for n in ("pages", "tail_k", "tail_v", "page_table", "status")]
+
+
+def i64_array(values):
+    """HOST array of int64 for the entry points that take strides that way."""
+    return (C.c_int64 * len(values))(*values)
 
 
 class KittyError(RuntimeError):
@@ -137,6 +158,20 @@ def lib() -> C.CDLL:
     L.kitty_lse_exchange_merge.argtypes = [vp, i64, vp, i32, i32, i32, vp, C.c_int, vp, i64, vp]
     L.kitty_lse_merge.restype = C.c_int
     L.kitty_lse_merge.argtypes = [vp, i32, i64, vp, C.c_int, vp]
+    rot, kv8, strides = C.POINTER(KittyRotaryPlan), C.POINTER(KittyKV8Layer), C.POINTER(i64)
+    L.kitty_rotary.restype = C.c_int
+    L.kitty_rotary.argtypes = [rot, vp, vp, vp, i64, vp, vp, C.c_int, i32, i32, i32, i32, strides, vp]
+    L.kitty_prompt_attn.restype = C.c_int
+    L.kitty_prompt_attn.argtypes = [vp, vp, vp, C.c_int, strides, i32, i64, i64, i32, i32, C.c_float, C.c_int, vp, vp,
+                                    vp, vp, vp, C.c_int, vp, vp]
+    L.kitty_kv8_append.restype = C.c_int
+    L.kitty_kv8_append.argtypes = [kv8, vp, vp, strides, vp, vp, i32, i32, rot, vp, vp, i32, vp]
+    L.kitty_kv8_expand.restype = C.c_int
+    L.kitty_kv8_expand.argtypes = [kv8, vp, vp, vp, vp, i32, i32, vp]
+    L.kitty_kv8_workspace_bytes.restype = i64
+    L.kitty_kv8_workspace_bytes.argtypes = [i32, i32, i32]
+    L.kitty_kv8_attn.restype = C.c_int
+    L.kitty_kv8_attn.argtypes = [kv8, vp, vp, i32, i32, C.c_float, vp, vp, i64, vp]
     _lib = L
     return L
 

@@ -1,0 +1,137 @@
+// Rotary positions of whole prompts and of single tokens: query and key heads in one launch.
+//
+// Bound by memory: every element is read once and written once (4 bytes of traffic per 16-bit element).  A block takes
+// a few tokens of one sequence and many heads, computes the tokens' angle table once (the 64-bit products and the sine
+// and cosine are shared by all heads) and streams the head rows through registers.
+#include "rotary.cuh"
+
+#include "decode.cuh"
+
+namespace kitty {
+
+struct RotArgs {
+  kitty_rotary_plan pl;
+  const void *in[2];
+  void *out[2];
+  int64_t is[2][3], os[2][3];      // element strides (batch, head, token) of query / key and of their outputs
+  const int64_t *pos;
+  int64_t pos_b;
+  int32_t T, h_q, h_all, tt, hc, tiles;
+};
+
+constexpr int ROT_TOK = 8;         // tokens of a block's table
+
+// LPR threads per head row; each thread keeps ROWS rows in flight.
+template <typename T, int MODE, int LPR, int ROWS>
+__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotArgs a) {
+  using U = RotUnits<T, MODE>;
+  __shared__ __align__(16) float2 tab[ROT_TOK][HD / 2];
+  const int r = a.pl.rotary_dim, np = r / 2;
+  const int b = blockIdx.x / a.tiles, t0 = (blockIdx.x % a.tiles) * a.tt;
+  const int ntok = min(a.tt, a.T - t0);
+  const int h0 = blockIdx.y * a.hc, nh = min(a.hc, a.h_all - h0);
+  const int rows = ntok * nh;
+  const int nt = U::turned(r), nu = nt + U::copied(r);
+  const int lane = threadIdx.x % LPR, row0 = threadIdx.x / LPR;
+  constexpr int STEP = 256 / LPR;
+
+  auto locate = [&](int row, const T *&src, T *&dst, int &tok) {
+    tok = row / nh;
+    int h = h0 + row - tok * nh;
+    const int s = h >= a.h_q;
+    if (s) h -= a.h_q;
+    const int64_t t = t0 + tok;
+    src = static_cast<const T *>(a.in[s]) + b * a.is[s][0] + h * a.is[s][1] + t * a.is[s][2];
+    dst = static_cast<T *>(a.out[s]) + b * a.os[s][0] + h * a.os[s][1] + t * a.os[s][2];
+  };
+  for (int i = threadIdx.x; i < ntok * np; i += 256) {
+    const int tok = i / np, p = i - tok * np;
+    tab[tok][U::slot(p, r)] = rot_angle(a.pl, a.pos[b * a.pos_b + t0 + tok], p);
+  }
+  __syncthreads();
+  for (int base = row0; base < rows; base += STEP * ROWS) {
+    for (int u = lane; u < nu; u += LPR) {
+      RotUnit<T, MODE> x[ROWS];
+      const T *src;
+      T *dst[ROWS];
+      int tok[ROWS];
+#pragma unroll
+      for (int j = 0; j < ROWS; ++j)
+        if (base + j * STEP < rows) {
+          locate(base + j * STEP, src, dst[j], tok[j]);
+          x[j].load(src, u, r);
+        }
+#pragma unroll
+      for (int j = 0; j < ROWS; ++j)
+        if (base + j * STEP < rows) x[j].store(dst[j], u, r, tab[tok[j]]);
+    }
+  }
+}
+
+template <typename T>
+int launch_rotary(const RotArgs &a, dim3 grid, cudaStream_t s) {
+  switch (rot_mode(a.pl, sizeof(T))) {
+    case ROT_HALF: {
+      // units of a full-width head: 8 (16 bit) or 16 (32 bit); a partly rotated head has up to twice as many
+      if (sizeof(T) == 2 && a.pl.rotary_dim == HD) rotary_kernel<T, ROT_HALF, 8, 4><<<grid, 256, 0, s>>>(a);
+      else rotary_kernel<T, ROT_HALF, 16, 4><<<grid, 256, 0, s>>>(a);
+      break;
+    }
+    case ROT_INTER: rotary_kernel<T, ROT_INTER, 16, 4><<<grid, 256, 0, s>>>(a); break;
+    case ROT_HALF_SCALAR: rotary_kernel<T, ROT_HALF_SCALAR, 32, 4><<<grid, 256, 0, s>>>(a); break;
+    default: rotary_kernel<T, ROT_INTER_SCALAR, 32, 4><<<grid, 256, 0, s>>>(a); break;
+  }
+  return cudaGetLastError() == cudaSuccess ? KITTY_OK : KITTY_E_CUDA;
+}
+
+}  // namespace kitty
+
+using namespace kitty;
+
+extern "C" int kitty_rotary(const kitty_rotary_plan *plan, const void *q, const void *k, const int64_t *positions,
+                            int64_t pos_stride_b, void *q_out, void *k_out, int dtype, int32_t B, int32_t T,
+                            int32_t h_q, int32_t h_kv, const int64_t *strides, void *stream) {
+  const int rc = check_rotary_plan(plan);
+  if (rc != KITTY_OK) return rc;
+  if (!strides || B < 0 || T < 0 || h_q < 0 || h_kv < 0 || pos_stride_b < 0) return KITTY_E_BADARG;
+  if (dtype < KITTY_F16 || dtype > KITTY_F32) return KITTY_E_BADARG;
+  if (B == 0 || T == 0 || h_q + h_kv == 0) return KITTY_OK;
+  if (!positions || (h_q && (!q || !q_out)) || (h_kv && (!k || !k_out))) return KITTY_E_BADARG;
+  const int esize = dtype == KITTY_F32 ? 4 : 2;
+  RotArgs a{};
+  a.pl = *plan;
+  const void *in[2] = {q, k};
+  void *out[2] = {q_out, k_out};
+  for (int s = 0; s < 2; ++s) {
+    a.in[s] = in[s];
+    a.out[s] = out[s];
+    if ((reinterpret_cast<uintptr_t>(in[s]) | reinterpret_cast<uintptr_t>(out[s])) & 15) return KITTY_E_BADARG;
+    for (int i = 0; i < 3; ++i) {
+      a.is[s][i] = strides[s * 3 + i];
+      a.os[s][i] = strides[6 + s * 3 + i];
+      if ((s ? h_kv : h_q) != 0 && ((a.is[s][i] * esize) % 16 != 0 || (a.os[s][i] * esize) % 16 != 0)) return KITTY_E_BADARG;
+    }
+  }
+  a.pos = positions;
+  a.pos_b = pos_stride_b;
+  a.T = T;
+  a.h_q = h_q;
+  a.h_all = h_q + h_kv;
+  a.tt = T < ROT_TOK ? T : ROT_TOK;
+  a.tiles = (T + a.tt - 1) / a.tt;
+  const int64_t blocks = static_cast<int64_t>(B) * a.tiles;
+  if (blocks > 0x7fffffff) return KITTY_E_BADSHAPE;
+  // Few tokens: spread the heads over blocks too, at least four heads each.
+  int split = 1;
+  const int want = 2 * sm_count();
+  if (blocks < want) split = static_cast<int>((want + blocks - 1) / blocks);
+  const int most = (a.h_all + 3) / 4;
+  if (split > most) split = most;
+  a.hc = (a.h_all + split - 1) / split;
+  split = (a.h_all + a.hc - 1) / a.hc;
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(split));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == KITTY_F16) return launch_rotary<__half>(a, grid, s);
+  if (dtype == KITTY_BF16) return launch_rotary<__nv_bfloat16>(a, grid, s);
+  return launch_rotary<float>(a, grid, s);
+}

@@ -1,0 +1,156 @@
+// Rotary positions: the angle table of a few tokens and the rotation of one head row.
+//
+// Pair p of a head (p < rotary_dim / 2) is turned by angle = position * w_p:
+//   (x1, x2) -> factor * (x1 cos - x2 sin, x2 cos + x1 sin)
+// with channels (p, p + rotary_dim/2) ("half") or (2p, 2p + 1) ("interleaved"); channels from rotary_dim on keep
+// their value.  The plan holds w_p in TURNS per position (w_p / 2 pi, 64 bits): position * turns loses its whole part
+// exactly in 64 bits, and the remaining fraction of a turn goes through sincospif, so an angle at position 2^31 is as
+// good as one at position 1 (a 32-bit product is off by 0.004 rad at position 100000).  The rotation itself is two
+// fused multiply-adds in 32 bits, rounded once to the data type.
+#pragma once
+
+#include "common.cuh"
+
+namespace kitty {
+
+enum RotMode { ROT_HALF = 0, ROT_INTER = 1, ROT_HALF_SCALAR = 2, ROT_INTER_SCALAR = 3, ROT_NONE = 4 };
+
+// How a head row is cut into units: a unit of the vector modes is one 16-byte piece (interleaved) or the two pieces
+// that hold both halves of its pairs (half); scalar modes take one pair per unit (rotary_dim that does not split into
+// whole pieces).  Channels from rotary_dim on are copied, in pieces (vector) or one by one (scalar).
+template <typename T, int MODE>
+struct RotUnits {
+  static constexpr int V = 16 / sizeof(T);                       // channels of a piece
+  static constexpr int PV = MODE == ROT_HALF ? V : MODE == ROT_INTER ? V / 2 : 1;   // pairs of a unit
+  static constexpr bool VEC = MODE == ROT_HALF || MODE == ROT_INTER;
+  static __device__ __forceinline__ int turned(int r) { return r / 2 / PV; }        // units that turn pairs
+  static __device__ __forceinline__ int copied(int r) { return VEC ? (HD - r) / V : HD - r; }
+  // Where pair p sits in a token's table row (float2, at most 64 of them): the pairs of all units are interleaved two
+  // by two, so that a row of threads reads consecutive 16-byte words.
+  static __device__ __forceinline__ int slot(int p, int r) {
+    if (PV == 1) return p;
+    const int u = p / PV, e = p % PV;
+    return ((e >> 1) * turned(r) + u) * 2 + (e & 1);
+  }
+};
+
+__device__ __forceinline__ float2 rot_angle(const kitty_rotary_plan &pl, int64_t pos, int p) {
+  double t = static_cast<double>(pos) * pl.turns[p];
+  t -= rint(t);
+  float s, c;
+  sincospif(static_cast<float>(t + t), &s, &c);
+  return make_float2(c * pl.factor, s * pl.factor);
+}
+
+template <typename T>
+struct Piece {          // 16 bytes as 32-bit floats
+  static constexpr int V = 16 / sizeof(T);
+  float f[V];
+  __device__ __forceinline__ void unpack(uint4 w) {
+    if constexpr (sizeof(T) == 4) {
+      f[0] = __uint_as_float(w.x); f[1] = __uint_as_float(w.y); f[2] = __uint_as_float(w.z); f[3] = __uint_as_float(w.w);
+    } else {
+      Vec8<T>::unpack(w, f);
+    }
+  }
+  __device__ __forceinline__ uint4 pack() const {
+    uint4 w;
+    T *t = reinterpret_cast<T *>(&w);
+#pragma unroll
+    for (int i = 0; i < V; ++i) t[i] = from_f32<T>(f[i]);
+    return w;
+  }
+};
+
+// One unit of a head row in flight: load() requests its channels, store() turns them by the token's table row and
+// writes them.  `row` / `out` may be the same memory: a unit reads all it needs before it writes, and units are
+// disjoint.
+template <typename T, int MODE>
+struct RotUnit {
+  using U = RotUnits<T, MODE>;
+  uint4 a, b;
+  T s0, s1;
+
+  __device__ __forceinline__ void load(const T *row, int u, int r) {
+    const int nt = U::turned(r);
+    if constexpr (U::VEC) {
+      if (u < nt) {
+        const T *p = row + (MODE == ROT_HALF ? u * U::V : 2 * u * U::PV);
+        a = *reinterpret_cast<const uint4 *>(p);
+        if constexpr (MODE == ROT_HALF) b = *reinterpret_cast<const uint4 *>(p + r / 2);
+      } else {
+        a = *reinterpret_cast<const uint4 *>(row + r + (u - nt) * U::V);
+      }
+    } else {
+      if (u < nt) {
+        s0 = row[MODE == ROT_HALF_SCALAR ? u : 2 * u];
+        s1 = row[MODE == ROT_HALF_SCALAR ? u + r / 2 : 2 * u + 1];
+      } else {
+        s0 = row[r + (u - nt)];
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T *out, int u, int r, const float2 *tab) const {
+    const int nt = U::turned(r);
+    if constexpr (MODE == ROT_HALF) {
+      if (u < nt) {
+        Piece<T> x, y;
+        x.unpack(a);
+        y.unpack(b);
+#pragma unroll
+        for (int e = 0; e < U::V; e += 2) {
+          const float4 cs = *reinterpret_cast<const float4 *>(tab + ((e >> 1) * nt + u) * 2);
+          const float x0 = x.f[e], y0 = y.f[e], x1 = x.f[e + 1], y1 = y.f[e + 1];
+          x.f[e] = fmaf(x0, cs.x, -y0 * cs.y);
+          y.f[e] = fmaf(y0, cs.x, x0 * cs.y);
+          x.f[e + 1] = fmaf(x1, cs.z, -y1 * cs.w);
+          y.f[e + 1] = fmaf(y1, cs.z, x1 * cs.w);
+        }
+        *reinterpret_cast<uint4 *>(out + u * U::V) = x.pack();
+        *reinterpret_cast<uint4 *>(out + u * U::V + r / 2) = y.pack();
+      } else {
+        *reinterpret_cast<uint4 *>(out + r + (u - nt) * U::V) = a;
+      }
+    } else if constexpr (MODE == ROT_INTER) {
+      if (u < nt) {
+        Piece<T> x;
+        x.unpack(a);
+#pragma unroll
+        for (int e = 0; e < U::PV; ++e) {
+          const float2 cs = tab[((e >> 1) * nt + u) * 2 + (e & 1)];
+          const float x0 = x.f[2 * e], x1 = x.f[2 * e + 1];
+          x.f[2 * e] = fmaf(x0, cs.x, -x1 * cs.y);
+          x.f[2 * e + 1] = fmaf(x1, cs.x, x0 * cs.y);
+        }
+        *reinterpret_cast<uint4 *>(out + u * U::V) = x.pack();
+      } else {
+        *reinterpret_cast<uint4 *>(out + r + (u - nt) * U::V) = a;
+      }
+    } else {
+      if (u < nt) {
+        const float2 cs = tab[u];
+        const float x0 = to_f32<T>(s0), x1 = to_f32<T>(s1);
+        out[MODE == ROT_HALF_SCALAR ? u : 2 * u] = from_f32<T>(fmaf(x0, cs.x, -x1 * cs.y));
+        out[MODE == ROT_HALF_SCALAR ? u + r / 2 : 2 * u + 1] = from_f32<T>(fmaf(x1, cs.x, x0 * cs.y));
+      } else {
+        out[r + (u - nt)] = s0;
+      }
+    }
+  }
+};
+
+// Mode of a plan for elements of `esize` bytes.
+inline int rot_mode(const kitty_rotary_plan &p, int esize) {
+  const int v = 16 / esize;
+  if (p.layout == KITTY_ROPE_HALF) return p.rotary_dim % (2 * v) == 0 ? ROT_HALF : ROT_HALF_SCALAR;
+  return p.rotary_dim % v == 0 ? ROT_INTER : ROT_INTER_SCALAR;
+}
+
+inline int check_rotary_plan(const kitty_rotary_plan *p) {
+  if (p == nullptr || p->turns == nullptr) return KITTY_E_BADARG;
+  if (p->rotary_dim < 2 || p->rotary_dim > HD || p->rotary_dim % 2 != 0) return KITTY_E_BADSHAPE;
+  if (p->layout != KITTY_ROPE_HALF && p->layout != KITTY_ROPE_INTERLEAVED) return KITTY_E_BADARG;
+  return KITTY_OK;
+}
+
+}  // namespace kitty

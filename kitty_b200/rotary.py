@@ -1,0 +1,182 @@
+"""Rotary positions of prompts and tokens.
+
+`RotaryEmbedding` holds what a model's configuration says about its angles (base, how much of the head turns, pair
+layout, scaling for long contexts); `apply_rotary` turns the query and key heads of any number of tokens in one launch.
+The reference leaves this to its models' element-wise sequence (models/qwen3/modeling_qwen3.py:222-232), whose roundings
+`hf_adapter.rope_decode_token` reproduces for a decode token; here angles are formed in 64 bits and every output is
+rounded once.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+HEAD_DIM = 128
+ROPE_LAYOUTS = {"half": _lib.ROPE_HALF, "interleaved": _lib.ROPE_INTERLEAVED}
+
+
+def _scaled_frequencies(rotary_dim: int, base: float, scaling: Optional[dict]):
+    """Radians per position of every pair (Python floats) and the factor on cosine and sine, from the fields of a
+    transformers configuration's rope parameters."""
+    n = rotary_dim // 2
+    inv = [base ** (-2.0 * i / rotary_dim) for i in range(n)]
+    if scaling is None:
+        return inv, 1.0
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if kind == "default":
+        return inv, 1.0
+    known = ("linear", "llama3", "yarn")
+    if kind not in known:
+        raise ValueError(f"rope scaling {kind!r} is not supported (default, {', '.join(known)})")
+    factor = float(scaling["factor"])
+    if not (factor > 0 and math.isfinite(factor)):
+        raise ValueError(f"rope scaling factor must be positive, got {factor}")
+    if kind == "linear":
+        return [w / factor for w in inv], 1.0
+    original = float(scaling["original_max_position_embeddings"])
+    if not (original > 0 and math.isfinite(original)):
+        raise ValueError(f"original_max_position_embeddings must be positive, got {original}")
+    if kind == "llama3":
+        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        if not high > low:
+            raise ValueError(f"high_freq_factor must be above low_freq_factor, got {high} and {low}")
+        out = []
+        for w in inv:       # few turns over the original context: stretched; many: kept; in between: blended
+            mix = min(max((original * w / (2 * math.pi) - low) / (high - low), 0.0), 1.0)
+            out.append(w / factor * (1.0 - mix) + w * mix)
+        return out, 1.0
+    # yarn: pairs that make beta_fast turns or more over the original context keep their angle, those with beta_slow or
+    # fewer are stretched, a ramp over the pair index in between; all sines and cosines are scaled
+    unknown = set(scaling) - {"rope_type", "type", "factor", "original_max_position_embeddings", "beta_fast", "beta_slow",
+                              "attention_factor", "truncate", "rope_theta", "partial_rotary_factor"}
+    if unknown:
+        raise ValueError(f"yarn fields {sorted(unknown)} are not supported")
+    if base == 1.0:
+        raise ValueError("yarn scaling needs a base other than 1")
+
+    def index(turns):
+        return rotary_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+    # a field that is there but None means its default, as in the configurations
+    def given(name, default):
+        value = scaling.get(name)
+        return default if value is None else float(value)
+
+    first, last = index(given("beta_fast", 32.0)), index(given("beta_slow", 1.0))
+    if scaling.get("truncate", True):
+        first, last = math.floor(first), math.ceil(last)
+    first, last = max(first, 0), min(last, rotary_dim - 1)
+    span = last - first if last != first else 0.001
+    out = []
+    for i, w in enumerate(inv):
+        ramp = min(max((i - first) / span, 0.0), 1.0)
+        out.append(w / factor * ramp + w * (1.0 - ramp))
+    return out, given("attention_factor", 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
+
+
+class RotaryEmbedding:
+    """Angles of a model's rotary positions, kept on a CUDA device.
+
+    head_dim: 128.  rotary_dim: channels that turn (even, default all; the rest keep their value).  layout: 'half' (pair
+    p = channels p and p + rotary_dim/2) or 'interleaved' (channels 2p and 2p + 1).  scaling: None or the rope parameters
+    of a transformers configuration, with `rope_type` 'default', 'linear', 'llama3' or 'yarn'."""
+
+    def __init__(self, head_dim: int = HEAD_DIM, base: float = 10000.0, rotary_dim: Optional[int] = None,
+                 layout: str = "half", scaling: Optional[dict] = None, device="cuda"):
+        rotary_dim = head_dim if rotary_dim is None else int(rotary_dim)
+        if head_dim != HEAD_DIM:
+            raise ValueError(f"kitty_b200 kernels are built for head_dim=128, got {head_dim}")
+        if rotary_dim < 2 or rotary_dim > head_dim or rotary_dim % 2:
+            raise ValueError(f"rotary_dim must be even and in 2 .. {head_dim}, got {rotary_dim}")
+        if layout not in ROPE_LAYOUTS:
+            raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
+        if not (base > 0 and math.isfinite(base)):
+            raise ValueError(f"base must be positive, got {base}")
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise ValueError("kitty_b200 has no CPU path: the angles live on a CUDA device")
+        inv, self.factor = _scaled_frequencies(rotary_dim, float(base), scaling)
+        self.head_dim, self.rotary_dim, self.layout, self.base = head_dim, rotary_dim, layout, float(base)
+        self.scaling = dict(scaling) if scaling is not None else None
+        self.inv_freq = torch.tensor(inv, dtype=torch.float64)                  # radians per position, on the host
+        self._turns = torch.tensor([w / (2 * math.pi) for w in inv], dtype=torch.float64, device=dev)
+        self.device = self._turns.device
+        self._c_plan = _lib.KittyRotaryPlan(self._turns.data_ptr(), self.factor, rotary_dim, ROPE_LAYOUTS[layout], 0)
+
+    def c_plan(self) -> "_lib.KittyRotaryPlan":
+        return self._c_plan
+
+
+def _head_strides(x: torch.Tensor):
+    """(batch, head, token) strides; a dimension of size one has none (views may carry any number there)."""
+    return [x.stride(i) if x.shape[i] > 1 else 0 for i in range(3)]
+
+
+def _rotary_input(x: torch.Tensor, what: str) -> torch.Tensor:
+    if x.dim() != 4 or x.shape[3] != HEAD_DIM:
+        raise ValueError(f"expected {what} [B, H, T, 128], got {tuple(x.shape)}")
+    if not x.is_cuda:
+        raise ValueError(f"kitty_b200 has no CPU path: the {what} must be on a CUDA device")
+    return x if x.stride(3) == 1 else x.contiguous()
+
+
+def _rotary_output(out: Optional[torch.Tensor], x: torch.Tensor, what: str) -> torch.Tensor:
+    """A new tensor in the input's own memory order, or the given one after its checks."""
+    if out is None:
+        return torch.empty_like(x)
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(3) != 1:
+        raise ValueError(f"{what}_out must have the {what}'s shape, type and device, with consecutive channels")
+    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+        raise ValueError(f"{what}_out is an expanded view: several heads would be written to one place")
+    same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
+    if not same and _spans_overlap(out, x):
+        raise ValueError(f"{what}_out overlaps the {what} without being the same view")
+    return out
+
+
+def _span(x: torch.Tensor):
+    last = sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+    return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size()
+
+
+def _spans_overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
+    if x.numel() == 0 or y.numel() == 0:
+        return False
+    (a, b), (c, d) = _span(x), _span(y)
+    return a < d and c < b
+
+
+def apply_rotary(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, rotary: RotaryEmbedding, *,
+                 query_out: Optional[torch.Tensor] = None, key_out: Optional[torch.Tensor] = None):
+    """Turn query [B, H_Q, T, 128] and key [B, H, T, 128] (any strides with consecutive channels, fp16 / bf16 / fp32) by
+    `positions` (int64 [T], [1, T] or [B, T]).  Returns (query, key) turned, in new tensors of the same memory order,
+    or in query_out / key_out, which may be query and key themselves (in place); other overlaps of outputs and inputs
+    are the caller's error and refused where the views' spans show them."""
+    q, k = _rotary_input(query, "query"), _rotary_input(key, "key")
+    B, _, T, _ = q.shape
+    if k.shape[0] != B or k.shape[2] != T or k.dtype != q.dtype or k.device != q.device:
+        raise ValueError("query and key must agree in batch, tokens, type and device")
+    if rotary.device != q.device:
+        raise ValueError(f"the angles are on {rotary.device}, the query on {q.device}")
+    if positions.dim() == 1:
+        positions = positions.unsqueeze(0)
+    if positions.dim() != 2 or positions.shape[1] != T or positions.shape[0] not in (1, B):
+        raise ValueError(f"expected positions [T], [1, T] or [B, T] for B={B}, T={T}, got {tuple(positions.shape)}")
+    if positions.dtype != torch.int64 or positions.device != q.device:
+        raise ValueError("positions must be int64 on the query's device")
+    if T > 1 and positions.stride(1) != 1:
+        positions = positions.contiguous()
+    qo, ko = _rotary_output(query_out, q, "query"), _rotary_output(key_out, k, "key")
+    code = _lib.dtype_code(q.dtype)
+    strides = _lib.i64_array(_head_strides(q) + _head_strides(k) + _head_strides(qo) + _head_strides(ko))
+    with torch.cuda.device(q.device):
+        rc = _lib.lib().kitty_rotary(rotary.c_plan(), q.data_ptr(), k.data_ptr(), positions.data_ptr(),
+                                     positions.stride(0) if positions.shape[0] > 1 else 0, qo.data_ptr(),
+                                     ko.data_ptr(), code, B, T, q.shape[1], k.shape[1], strides,
+                                     _lib.stream_ptr(q.device))
+    _lib.check(rc, "kitty_rotary")
+    return qo, ko

@@ -1,0 +1,198 @@
+"""Prompt attention against the formula in 64 bits."""
+import pytest
+import torch
+
+from tests.ops_ref import HALF, attend, attend_fast, attention_bound, logit_error
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+SC = 128 ** -0.5
+
+
+@pytest.fixture(scope="module")
+def kb():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    import kitty_b200
+
+    return kitty_b200
+
+
+def _inputs(shape_q, shape_k, dtype, seed, qscale=0.7):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    q = (qscale * torch.randn(shape_q, generator=g, device=DEV)).to(dtype)
+    k = torch.randn(shape_k, generator=g, device=DEV)
+    k[..., :4] *= 8.0
+    v = torch.randn(shape_k, generator=g, device=DEV)
+    return q, k.to(dtype), v.to(dtype)
+
+
+def _limits(n, m, causal):
+    i = torch.arange(n, device=DEV)
+    return (i + 1 + m - n).clamp(0, m) if causal else torch.full((n,), m, device=DEV)
+
+
+def _check_rows(got, q, k, v, scaling, causal, what=""):
+    """got [n, H_Q, D], q [n, H_Q, D], k / v [m, H, D] of one sequence."""
+    n, hq, _ = q.shape
+    m, h, _ = k.shape
+    lim = _limits(n, m, causal)
+    for x in range(hq):
+        qx, kx, vx = q[:, x].double(), k[:, x // (hq // h)].double(), v[:, x // (hq // h)].double()
+        want, mag = attend_fast(qx, kx, vx, scaling, lim)
+        bound = attention_bound(want, mag, q.dtype, HALF[q.dtype], logit_error(qx, kx, scaling))
+        off = (got[:, x].double() - want).abs()
+        assert (off <= bound).all(), (what, x, off.max().item(), (off - bound).max().item())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,hq,h,Lq,Lk", [
+    (1, 1, 1, 1, 1), (1, 4, 1, 128, 128), (2, 8, 2, 127, 127), (1, 7, 1, 129, 129), (1, 28, 4, 300, 300),
+    (2, 4, 4, 257, 257), (1, 8, 1, 640, 640), (1, 3, 1, 1, 777), (2, 4, 2, 100, 900), (1, 2, 2, 5, 133),
+    (1, 32, 1, 70, 70), (1, 2, 1, 200, 90), (1, 1, 1, 1300, 1300)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_dense(kb, dtype, B, hq, h, Lq, Lk, causal):
+    q, k, v = _inputs((B, hq, Lq, 128), (B, h, Lk, 128), dtype, Lq + Lk)
+    got = kb.prompt_attention(q, k, v, SC, causal=causal)
+    assert got.shape == (B, Lq, hq, 128) and got.dtype == dtype
+    for b in range(B):
+        _check_rows(got[b], *(x[b].transpose(0, 1) for x in (q, k, v)), SC, causal)
+    # projection layout, read in place
+    qt, kt, vt = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v))
+    assert torch.equal(kb.prompt_attention(qt, kt, vt, SC, causal=causal), got)
+    assert kb.prompt_attention_status(DEV) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,h", [(28, 4), (4, 4), (3, 1)])
+@pytest.mark.parametrize("lens", [[1, 37, 128, 129, 300], [0, 5, 0, 0, 513, 1, 256], [700], [0], [1] * 70])
+def test_packed(kb, dtype, hq, h, lens):
+    T = sum(lens)
+    extra = 3
+    q, k, v = _inputs((T + extra, hq, 128), (T + extra, h, 128), dtype, T)
+    cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=DEV)
+    k[T:], v[T:] = float("nan"), float("inf")                         # rows of no sequence
+    out = torch.full((T + extra, hq, 128), 9.0, dtype=dtype, device=DEV)
+    got = kb.prompt_attention(q, k, v, SC, cu_seqlens=cu, out=out)
+    assert got is out and (out[T:] == 9.0).all()                      # rows behind the last sequence stay
+    fresh = kb.prompt_attention(q, k, v, SC, cu_seqlens=cu)
+    assert torch.equal(fresh[:T], out[:T]) and (fresh[T:] == 0).all()
+    at = 0
+    for n in lens:
+        if n:
+            _check_rows(got[at:at + n], q[at:at + n], k[at:at + n], v[at:at + n], SC, True, (lens, n))
+        at += n
+
+
+def test_packed_pieces(kb):
+    """Further pieces: each sequence has more keys than queries (or fewer: its first rows see nothing)."""
+    nq, nk = [3, 200, 130, 10], [500, 333, 130, 4]
+    q, _, _ = _inputs((sum(nq), 8, 128), (1, 2, 128), torch.bfloat16, 1)
+    _, k, v = _inputs((1, 8, 128), (sum(nk), 2, 128), torch.bfloat16, 2)
+    cq = torch.tensor([0, 3, 203, 333, 343], dtype=torch.int32, device=DEV)
+    ck = torch.tensor([0, 500, 833, 963, 967], dtype=torch.int32, device=DEV)
+    got = kb.prompt_attention(q, k, v, SC, cu_seqlens=cq, cu_seqlens_k=ck)
+    a = b = 0
+    for n, m in zip(nq, nk):
+        _check_rows(got[a:a + n], q[a:a + n], k[b:b + m], v[b:b + m], SC, True, (n, m))
+        a, b = a + n, b + m
+    assert (got[333:339] == 0).all()                                  # 10 queries over 4 keys: six see none
+
+
+def test_padded_batch(kb):
+    q, k, v = _inputs((4, 6, 260, 128), (4, 2, 300, 128), torch.float16, 3)
+    ql = torch.tensor([260, 0, 129, 17], dtype=torch.int32, device=DEV)
+    kl = torch.tensor([300, 40, 129, 0], dtype=torch.int32, device=DEV)
+    for b in range(4):                                                # padding holds garbage
+        k[b, :, int(kl[b]):], v[b, :, int(kl[b]):] = float("inf"), float("nan")
+    got = kb.prompt_attention(q, k, v, SC, query_lengths=ql, key_lengths=kl)
+    for b in range(4):
+        n, m = int(ql[b]), int(kl[b])
+        assert (got[b, n:] == 0).all()
+        if n and m:
+            _check_rows(got[b, :n], *(x[b].transpose(0, 1)[:w] for x, w in ((q, n), (k, m), (v, m))), SC, True)
+        elif n:
+            assert (got[b, :n] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_what_a_row_does_not_see(kb, dtype):
+    """Infinities and NaN among later keys and values reach no earlier row, and reach every row that sees them."""
+    L = 400
+    q, k, v = _inputs((1, 2, L, 128), (1, 1, L, 128), dtype, 4)
+    clean = kb.prompt_attention(q, k, v, SC)
+    k2, v2 = k.clone(), v.clone()
+    v2[0, 0, 150, 5] = float("nan")
+    v2[0, 0, 350, 7] = float("inf")
+    k2[0, 0, 390] = float("nan")
+    got = kb.prompt_attention(q, k2, v2, SC)
+    for x in range(2):
+        want, mag = attend(q[0, x].double(), k[0, 0].double(), v[0, 0].double(), SC, _limits(L, L, True))
+        bound = attention_bound(want, mag, dtype, HALF[dtype], logit_error(q[0, x].double(), k[0, 0].double(), SC))
+        off = (got[0, :, x].double() - want).abs()
+        assert (off[:150] <= bound[:150]).all()
+        others = [c for c in range(128) if c != 5]
+        assert (off[150:350][:, others] <= bound[150:350][:, others]).all()
+    assert torch.isnan(got[0, 150:390, :, 5]).all()
+    assert torch.isinf(got[0, 350:390, :, 7]).all()
+    assert torch.isnan(got[0, 390:]).all()
+    assert torch.isfinite(clean).all()
+
+
+def test_extreme_logits(kb):
+    """Maxima that rise and fall by far more than the lag, and rows whose weight sits on one key."""
+    L = 520
+    q, k, v = _inputs((1, 2, L, 128), (1, 1, L, 128), torch.bfloat16, 5, qscale=6.0)
+    ramp = torch.linspace(0.05, 4.0, L, device=DEV)[None, None, :, None]
+    for kk in ((k.float() * ramp).bfloat16(), (k.float() * ramp.flip(2)).bfloat16()):
+        got = kb.prompt_attention(q, kk, v, SC)
+        _check_rows(got[0], q[0].transpose(0, 1), kk[0].transpose(0, 1), v[0].transpose(0, 1), SC, True)
+    zero = torch.zeros_like(q)
+    got = kb.prompt_attention(zero, k, v, SC)                          # all weights equal: running means
+    _check_rows(got[0], zero[0].transpose(0, 1), k[0].transpose(0, 1), v[0].transpose(0, 1), SC, True)
+
+
+def test_streams_graphs_and_empty(kb):
+    q, k, v = _inputs((1, 4, 200, 128), (1, 2, 200, 128), torch.float16, 6)
+    want = kb.prompt_attention(q, k, v, SC)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for s in streams:                                                  # two calls at once
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append([kb.prompt_attention(q, k, v, SC) for _ in range(3)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for per in outs for o in per)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cap = kb.prompt_attention(q, k, v, SC)
+    q.copy_(q.flip(2))
+    graph.replay()
+    assert torch.equal(cap, kb.prompt_attention(q, k, v, SC))
+    assert kb.prompt_attention(q[:, :, :0], k, v, SC).shape == (1, 0, 4, 128)
+    assert kb.prompt_attention(q[:0], k[:0], v[:0], SC).shape == (0, 200, 4, 128)
+    none = kb.prompt_attention(q, k[:, :, :0], v[:, :, :0], SC, causal=False)
+    assert (none == 0).all()
+    one = kb.prompt_attention(q, k[:, :1].expand(1, 4, 200, 128), v[:, :1].expand(1, 4, 200, 128), SC)
+    assert torch.equal(one, kb.prompt_attention(q, k[:, :1], v[:, :1], SC))
+
+
+def test_agrees_with_decode_attention(kb):
+    """The row of a prompt's last token equals decode attention over a cache that still holds everything in fp16."""
+    import types
+
+    cfg = types.SimpleNamespace(num_hidden_layers=1, head_dim=128, num_key_value_heads=2, num_attention_heads=8, hidden_size=1024)
+    q, k, v = _inputs((2, 8, 150, 128), (2, 2, 150, 128), torch.float16, 8)
+    cache = kb.KittyCache(cfg, 2, 256, device=DEV)
+    cache.update(k, v, 0)
+    cache.quantize_prefill(0)
+    assert cache.kv_cache[0].PageCount_K == 0                           # 150 tokens: sink and Q-buffer only
+    dec = kb.decode_attention(q[:, :, -1:].contiguous(), cache.kv_cache[0], 2, SC)
+    got = kb.prompt_attention(q, k, v, SC)[:, -1:]
+    for b in range(2):
+        for x in range(8):
+            qx, kx, vx = q[b, x, -1:].double(), k[b, x // 4].double(), v[b, x // 4].double()
+            want, mag = attend_fast(qx, kx, vx, SC, torch.tensor([150], device=DEV))
+            bound = attention_bound(want, mag, torch.float16, HALF[torch.float16], logit_error(qx, kx, SC))
+            assert ((got[b, :, x].double() - want).abs() <= bound).all()
+    assert (dec.float() - got.float()).abs().max() <= 1e-2 * got.float().abs().max()

@@ -1,0 +1,149 @@
+"""What the prompt-side operators and the 8-bit cache refuse (no GPU needed: every check comes before the first launch)."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+P = 4096            # stands for an aligned pointer: refused calls never follow it
+
+
+@pytest.fixture(scope="module")
+def L():
+    from kitty_b200 import _lib
+
+    return _lib
+
+
+def _plan(L, r=128, layout=0, turns=P):
+    return L.KittyRotaryPlan(turns, 1.0, r, layout, 0)
+
+
+def _layer(L, **over):
+    f = dict(max_bs=4, max_page=8, num_pages=32, h_kv=2, head_dim=128, dtype=L.KITTY_BF16, pages=P, tail_k=P, tail_v=P,
+             page_table=P, status=P)
+    f.update(over)
+    return L.KittyKV8Layer(*f.values())
+
+
+def _rotary(L, plan, q=P, k=P, pos=P, pos_b=0, qo=P, ko=P, dtype=0, B=1, T=1, hq=1, h=1, st=(0,) * 12):
+    return L.lib().kitty_rotary(plan, q, k, pos, pos_b, qo, ko, dtype, B, T, hq, h, L.i64_array(list(st)), None)
+
+
+def test_rotary_entry_point(L):
+    assert _rotary(L, None) == L.KITTY_E_BADARG
+    assert _rotary(L, _plan(L, turns=None)) == L.KITTY_E_BADARG
+    for r in (0, 3, 130, -2):
+        assert _rotary(L, _plan(L, r)) == L.KITTY_E_BADSHAPE
+    assert _rotary(L, _plan(L, layout=2)) == L.KITTY_E_BADARG
+    good = _plan(L)
+    for kw in (dict(q=None), dict(k=None), dict(pos=None), dict(qo=None), dict(dtype=3), dict(B=-1), dict(T=-1), dict(q=P + 2),
+               dict(ko=P + 8), dict(hq=-1), dict(pos_b=-1), dict(st=(4,) + (0,) * 11), dict(dtype=2, st=(2,) + (0,) * 11)):
+        assert _rotary(L, good, **kw) == L.KITTY_E_BADARG, kw
+    assert _rotary(L, good, B=0) == L.KITTY_OK and _rotary(L, good, T=0, q=None, k=None) == L.KITTY_OK
+
+
+def _prompt(L, q=P, k=P, v=P, dtype=0, st=(0,) * 9, B=1, Lq=1, Lk=1, hq=1, h=1, sc=1.0, ql=None, kl=None, cu=None, cuk=None,
+            out=P):
+    return L.lib().kitty_prompt_attn(q, k, v, dtype, L.i64_array(list(st)), B, Lq, Lk, hq, h, sc, 1, ql, kl, cu, cuk, out, 0,
+                                     None, None)
+
+
+def test_prompt_entry_point(L):
+    for kw in (dict(q=None), dict(k=None), dict(out=None), dict(dtype=2), dict(dtype=7), dict(hq=3, h=2), dict(h=0), dict(hq=0),
+               dict(B=-1), dict(Lq=-1), dict(sc=0.0), dict(sc=-1.0), dict(sc=math.inf), dict(sc=math.nan), dict(q=P + 8),
+               dict(out=P + 4), dict(Lq=2), dict(Lq=2, st=(0, 0, 4) + (0,) * 6), dict(Lk=2, st=(0,) * 5 + (-128,) + (0,) * 3)):
+        assert _prompt(L, **kw) == L.KITTY_E_BADARG, kw
+    assert _prompt(L, Lq=(1 << 30) + 1) == L.KITTY_E_BADSHAPE
+    assert _prompt(L, B=0) == L.KITTY_OK and _prompt(L, Lq=0) == L.KITTY_OK
+
+
+def test_kv8_entry_points(L):
+    lib = L.lib()
+    z9 = L.i64_array([0] * 9)
+
+    def append(layer, k=P, v=P, st=z9, start=P, B=1, T=1, plan=None, q=None, qo=None, hq=0):
+        return lib.kitty_kv8_append(layer, k, v, st, start, None, B, T, plan, q, qo, hq, None)
+
+    def expand(layer, n=4, lens=P, k=P, v=P, B=1):
+        return lib.kitty_kv8_expand(layer, lens, None, k, v, B, n, None)
+
+    def attn(layer, lens=P, q=P, B=1, hq=2, out=P, ws=P, nbytes=1 << 40):
+        return lib.kitty_kv8_attn(layer, lens, q, B, hq, 1.0, out, ws, nbytes, None)
+
+    for over in (dict(pages=None), dict(tail_k=None), dict(page_table=None), dict(status=None), dict(dtype=2), dict(max_bs=0),
+                 dict(num_pages=0), dict(h_kv=0), dict(max_page=-1), dict(pages=P + 8)):
+        bad = _layer(L, **over)
+        assert append(bad) == expand(bad) == attn(bad) == L.KITTY_E_BADARG, over
+    for over in (dict(head_dim=64), dict(max_page=(1 << 23) + 1)):
+        bad = _layer(L, **over)
+        assert append(bad) == expand(bad) == attn(bad) == L.KITTY_E_BADSHAPE, over
+    good = _layer(L)
+    for kw in (dict(k=None), dict(v=P + 2), dict(start=None), dict(B=5), dict(B=-1), dict(T=-1), dict(hq=2, q=P, qo=P),
+               dict(hq=2, plan=_plan(L), q=None, qo=P), dict(hq=2, plan=_plan(L), q=P, qo=None), dict(plan=_plan(L, layout=5)),
+               dict(st=L.i64_array([4] + [0] * 8)), dict(hq=1, plan=_plan(L), q=P, qo=P, st=L.i64_array([0] * 8 + [2]))):
+        assert append(good, **kw) == L.KITTY_E_BADARG, kw
+    assert append(good, T=0) == append(good, B=0) == L.KITTY_OK
+    for kw in (dict(lens=None), dict(k=None), dict(v=P + 8), dict(B=5), dict(n=-1)):
+        assert expand(good, **kw) == L.KITTY_E_BADARG, kw
+    assert expand(good, n=0) == L.KITTY_OK
+    for kw in (dict(lens=None), dict(q=None), dict(q=P + 4), dict(out=None), dict(ws=None), dict(B=5), dict(hq=3), dict(hq=0)):
+        assert attn(good, **kw) == L.KITTY_E_BADARG, kw
+    assert attn(good, hq=34) == L.KITTY_E_BADSHAPE
+    assert attn(good, nbytes=100) == L.KITTY_E_WORKSPACE
+    assert attn(good, B=0) == L.KITTY_OK
+    assert lib.kitty_kv8_workspace_bytes(1, 2, 3) == L.KITTY_E_BADARG
+    assert lib.kitty_kv8_workspace_bytes(L.KV8_MAX_BATCH + 1, 2, 4) == L.KITTY_E_BADSHAPE
+    assert lib.kitty_kv8_workspace_bytes(128, 8, 32) > lib.kitty_kv8_workspace_bytes(1, 8, 32) > 0
+
+
+def test_struct_sizes(L):
+    assert C.sizeof(L.KittyRotaryPlan) == 24 and C.sizeof(L.KittyKV8Layer) == 6 * 4 + 5 * 8
+
+
+def test_python_refusals_without_a_gpu():
+    import kitty_b200 as kb
+    from kitty_b200.rotary import _scaled_frequencies
+
+    x = torch.zeros(1, 2, 4, 128, dtype=torch.float16)
+    for bad in (dict(head_dim=64), dict(rotary_dim=3), dict(rotary_dim=130), dict(layout="pairs"), dict(base=0.0),
+                dict(base=math.inf), dict(device="cpu"), dict(scaling={"rope_type": "dynamic", "factor": 2.0}),
+                dict(scaling={"rope_type": "linear", "factor": -1.0}),
+                dict(scaling={"rope_type": "yarn", "factor": 2.0, "original_max_position_embeddings": 0}),
+                dict(scaling={"rope_type": "yarn", "factor": 2.0, "original_max_position_embeddings": 4096, "mscale": 1.0}),
+                dict(scaling={"rope_type": "llama3", "factor": 2.0, "original_max_position_embeddings": 4096,
+                              "low_freq_factor": 4.0, "high_freq_factor": 4.0})):
+        with pytest.raises(ValueError):
+            kb.RotaryEmbedding(**{"device": "cpu", **bad})
+    with pytest.raises(ValueError, match="CUDA"):
+        kb.apply_rotary(x, x, torch.arange(4), None)
+    with pytest.raises(ValueError, match="CUDA"):
+        kb.prompt_attention(x, x, x, 1.0)
+    with pytest.raises(ValueError, match="expected query"):
+        kb.prompt_attention(x[0], x, x, 1.0)
+    for bad in (dict(MAX_BS=0), dict(MAX_LEN=0), dict(H_KV=0), dict(D=64), dict(MAX_LEN=(1 << 30) + 1), dict(device="cpu")):
+        with pytest.raises(ValueError):
+            kb.KV8Layer(**{**dict(MAX_BS=1, MAX_LEN=128, H_KV=1, device="cpu"), **bad})
+    with pytest.raises(TypeError):
+        kb.KV8Layer(1, 128, 1, dtype=torch.float32, device="cpu")
+    assert _scaled_frequencies(4, 10000.0, {"rope_type": "default"}) == ([1.0, 0.01], 1.0)
+
+
+def test_scaled_frequencies_match_transformers():
+    """The angles of the scalings are those of transformers' own configurations (which it keeps in 32 bits)."""
+    from transformers import LlamaConfig
+    from transformers.modeling_rope_utils import ROPE_INIT_FUNCTIONS
+
+    from kitty_b200.rotary import _scaled_frequencies
+
+    for scaling in ({"rope_type": "linear", "factor": 4.0},
+                    {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+                     "original_max_position_embeddings": 8192},
+                    {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768}):
+        for base in (10000.0, 500000.0):
+            cfg = LlamaConfig(hidden_size=512, num_attention_heads=4, max_position_embeddings=131072,
+                              rope_parameters={**scaling, "rope_theta": base})
+            want, factor = ROPE_INIT_FUNCTIONS[scaling["rope_type"]](cfg, torch.device("cpu"))
+            inv, f = _scaled_frequencies(128, base, scaling)
+            got = torch.tensor(inv, dtype=torch.float64)
+            assert ((got - want.double()).abs() <= 2.0 ** -20 * got).all() and abs(f - factor) < 1e-12
