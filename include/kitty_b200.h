@@ -381,11 +381,17 @@ int kitty_rotary(const kitty_rotary_plan *plan, const void *q, const void *k, co
  * sees no key is zero.  Keys and values that a row does not see never reach its result, whatever they hold.
  * strides: HOST array of nine element strides, (batch, head, token) of q, k and v (batch ignored when packed).
  * out: contiguous [B, Lq, h_q, 128] or [Lq, h_q, 128] of the same type.  scaling: positive and finite.
- * status: device int32 or null, set to 1 when a bounded device-side wait ran out. */
+ * status: device int32 or null, set to 1 when a bounded device-side wait ran out.
+ * workspace: null, or kitty_prompt_workspace_bytes of scratch (0 for most calls; 16-byte aligned, no initial contents,
+ * not shared by calls that overlap).  With it, calls with few query rows cut the keys in parts that run side by side
+ * and are joined by a second kernel. */
+int64_t kitty_prompt_workspace_bytes(int32_t B, int64_t Lq, int64_t Lk, int32_t h_q, int32_t h_kv, int causal,
+                                     int packed);
 int kitty_prompt_attn(const void *q, const void *k, const void *v, int dtype, const int64_t *strides, int32_t B,
                       int64_t Lq, int64_t Lk, int32_t h_q, int32_t h_kv, float scaling, int causal,
                       const int32_t *q_lens, const int32_t *k_lens, const int32_t *cu_q, const int32_t *cu_k,
-                      void *out, int zero_rest, int32_t *status, void *stream);
+                      void *out, int zero_rest, int32_t *status, void *workspace, int64_t workspace_bytes,
+                      void *stream);
 
 /* ---- The 8-bit cache --------------------------------------------------------------------------
  * (No counterpart in the reference; for layers or models that two bits per value hurt.)  Pages of 128 tokens behind a

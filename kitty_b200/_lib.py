@@ -28,7 +28,7 @@ EXPORTS = [
     "kitty_lse_merge", "kitty_decode_attn_static", "kitty_plan_step", "kitty_decode_step",
     "kitty_lse_exchange_bytes", "kitty_lse_exchange_merge", "kitty_decode_attn_exchange", "kitty_rope_qk",
     "kitty_plan_step_split", "kitty_decode_step_exchange", "kitty_append_rows", "kitty_flush_rows",
-    "kitty_decode_attn_rows", "kitty_rotary", "kitty_prompt_attn", "kitty_kv8_append", "kitty_kv8_expand",
+    "kitty_decode_attn_rows", "kitty_rotary", "kitty_prompt_workspace_bytes", "kitty_prompt_attn", "kitty_kv8_append", "kitty_kv8_expand",
     "kitty_kv8_workspace_bytes", "kitty_kv8_attn",
 ]
 
@@ -69,9 +69,13 @@ class KittyKV8Layer(C.Structure):
                [(n, C.c_void_p) for n in ("pages", "tail_k", "tail_v", "page_table", "status")]
 
 
+_I64 = {n: C.c_int64 * n for n in (9, 12)}
+
+
 def i64_array(values):
     """HOST array of int64 for the entry points that take strides that way."""
-    return (C.c_int64 * len(values))(*values)
+    n = len(values)
+    return (_I64.get(n) or C.c_int64 * n)(*values)
 
 
 class KittyError(RuntimeError):
@@ -163,7 +167,9 @@ def lib() -> C.CDLL:
     L.kitty_rotary.argtypes = [rot, vp, vp, vp, i64, vp, vp, C.c_int, i32, i32, i32, i32, strides, vp]
     L.kitty_prompt_attn.restype = C.c_int
     L.kitty_prompt_attn.argtypes = [vp, vp, vp, C.c_int, strides, i32, i64, i64, i32, i32, C.c_float, C.c_int, vp, vp,
-                                    vp, vp, vp, C.c_int, vp, vp]
+                                    vp, vp, vp, C.c_int, vp, vp, i64, vp]
+    L.kitty_prompt_workspace_bytes.restype = i64
+    L.kitty_prompt_workspace_bytes.argtypes = [i32, i64, i64, i32, i32, C.c_int, C.c_int]
     L.kitty_kv8_append.restype = C.c_int
     L.kitty_kv8_append.argtypes = [kv8, vp, vp, strides, vp, vp, i32, i32, rot, vp, vp, i32, vp]
     L.kitty_kv8_expand.restype = C.c_int
@@ -192,6 +198,23 @@ def dtype_code(dtype) -> int:
         return {torch.float16: KITTY_F16, torch.bfloat16: KITTY_BF16, torch.float32: KITTY_F32}[dtype]
     except KeyError:
         raise TypeError(f"kitty_b200 supports float16, bfloat16 and float32 tensors, got {dtype}") from None
+
+
+def call_on(device, fn, where: str, *args) -> None:
+    """Call an entry point with the current stream of `device` (a CUDA device with an index) as its last argument and
+    that device current, and raise if it refuses.  A small call costs more on the host than on the device, so the device
+    is switched only where it has to be."""
+    import torch
+
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc != KITTY_OK:
+        raise KittyError(int(rc), where)
 
 
 def stream_ptr(device) -> int:

@@ -43,9 +43,95 @@ struct PromptArgs {
   int64_t qs[3], ks[3], vs[3];                 // element strides (batch, head, token)
   const int32_t *q_lens, *k_lens, *cu_q, *cu_k;
   int32_t *status;
-  int32_t B, Lq, Lk, G, h_kv, pairs, causal, zero_rest;
+  float *part;                                 // splits > 1: [splits][rows][h_q][128] accumulators,
+  float2 *part_ml;                             // [splits][rows][h_q] (maximum in base 2, sum; sum -1: sees nothing)
+  int64_t rows;                                // output rows of one head
+  int32_t B, Lq, Lk, G, h_kv, pairs, causal, zero_rest, splits;
   float c;                                     // scaling * log2 e
 };
+
+// ---- two 32-bit floats at a time
+__device__ __forceinline__ uint64_t pk2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 un2(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// Largest of three; NaN if one of them is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x of two numbers (finite, below 2^7) on the multiply-add pipe: x = whole + f with |f| <= 1/2, 2^f by a polynomial of
+// degree four fitted for the least largest relative error (2.6e-6 = 2^-18.6), the whole part added to the exponent.
+// Below 2^-126 the result stays there: a weight of 1e-38.
+__device__ __forceinline__ uint64_t ex2_poly2(uint64_t x2) {
+  float2 x = un2(x2);
+  x2 = pk2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));
+  const uint64_t magic = pk2(12582912.0f, 12582912.0f), unmagic = pk2(-12582912.0f, -12582912.0f);
+  const uint64_t t = add2(x2, magic);                       // whole part in the low bits
+  const uint64_t f = fma2(add2(t, unmagic), pk2(-1.0f, -1.0f), x2);
+  uint64_t p = fma2(f, pk2(0.00957009f, 0.00957009f), pk2(0.0559179f, 0.0559179f));
+  p = fma2(p, f, pk2(0.24024745f, 0.24024745f));
+  p = fma2(p, f, pk2(0.69312181f, 0.69312181f));
+  p = fma2(p, f, pk2(0.99999926f, 0.99999926f));
+  const float2 pf = un2(p), tf = un2(t);
+  return pk2(__uint_as_float(__float_as_uint(pf.x) + (__float_as_uint(tf.x) << 23)),
+             __uint_as_float(__float_as_uint(pf.y) + (__float_as_uint(tf.y) << 23)));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(uint64_t p) {
+  const float2 f = un2(p);
+  if constexpr (__is_same(T, __nv_bfloat16)) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t *>(&x);
+  } else {
+    return pack_h2(f.x, f.y);
+  }
+}
+
+// Weights of 64 logits: 2^(v c - mc), their sum, and the 16-bit pairs in tensor memory.  POLY: every fourth pair goes
+// through the polynomial, which takes a quarter of the load off the 16-a-clock exponential unit.
+template <typename T, bool POLY>
+__device__ __forceinline__ uint64_t weights64(const float *v, uint64_t c2, uint64_t nmc2, uint32_t dst) {
+  uint64_t sum[2] = {0, 0};
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint64_t x = fma2(pk2(v[32 * q + 2 * i], v[32 * q + 2 * i + 1]), c2, nmc2);
+      uint64_t p;
+      if (POLY && (i & 3) == 3) {
+        p = ex2_poly2(x);
+      } else {
+        const float2 f = un2(x);
+        p = pk2(ex2(f.x), ex2(f.y));
+      }
+      sum[i & 1] = add2(sum[i & 1], p);
+      w[i] = pack2<T>(p);
+    }
+    tmem_st16(dst + 16 * q, w);
+  }
+  return add2(sum[0], sum[1]);
+}
 
 struct Seq {
   int b;              // batch coordinate
@@ -62,9 +148,10 @@ __device__ __forceinline__ int key_limit(const Seq &s, int i, int causal) {
   return causal ? clampi(i + 1 + s.nk - s.nq, 0, s.nk) : s.nk;
 }
 
-// One row again, by one warp, without the matrix units: only keys that the row sees are touched.
+// One row again, by one warp, without the matrix units: only keys that the row sees are touched.  Keys lo .. hi - 1 were
+// multiplied; the row sees those below limit.
 template <typename T>
-__device__ __noinline__ void repair_row(const PromptArgs &a, const Seq &s, int row, int head, int limit, int touched) {
+__device__ __noinline__ void repair_row(const PromptArgs &a, const Seq &s, int row, int head, int limit, int lo, int hi, int z) {
   const int lane = threadIdx.x & 31;
   const int hk = head / a.G;
   const T *k = static_cast<const T *>(a.k) + s.b * a.ks[0] + hk * a.ks[1] + s.k0 * a.ks[2] + 4 * lane;
@@ -77,7 +164,7 @@ __device__ __noinline__ void repair_row(const PromptArgs &a, const Seq &s, int r
   };
   bool cause = false;
   float x[4];
-  for (int j = limit; j < touched; ++j) {
+  for (int j = max(limit, lo); j < hi; ++j) {
     load4(v + j * a.vs[2], x);
 #pragma unroll
     for (int e = 0; e < 4; ++e) cause |= !(fabsf(x[e]) < INFINITY);
@@ -85,7 +172,7 @@ __device__ __noinline__ void repair_row(const PromptArgs &a, const Seq &s, int r
   if (!__any_sync(0xffffffffu, cause)) return;
   float q[4], acc[4] = {}, m = -INFINITY, l = 0.0f;
   load4(static_cast<const T *>(a.q) + s.b * a.qs[0] + head * a.qs[1] + (static_cast<int64_t>(s.q0) + row) * a.qs[2] + 4 * lane, q);
-  for (int j = 0; j < limit; ++j) {
+  for (int j = lo; j < min(limit, hi); ++j) {
     load4(k + j * a.ks[2], x);
     float d = q[0] * x[0] + q[1] * x[1] + q[2] * x[2] + q[3] * x[3];
 #pragma unroll
@@ -99,11 +186,17 @@ __device__ __noinline__ void repair_row(const PromptArgs &a, const Seq &s, int r
     for (int e = 0; e < 4; ++e) acc[e] = acc[e] * f + p * x[e];
     m = mn;
   }
+  const int64_t at = (s.out0 + row) * static_cast<int64_t>(a.G) * a.h_kv + head;
+  if (a.splits > 1) {
+    const int64_t pa = z * a.rows * a.G * a.h_kv + at;
+    *reinterpret_cast<float4 *>(a.part + pa * HD + 4 * lane) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    if (lane == 0) a.part_ml[pa] = make_float2(m, l);
+    return;
+  }
   T o[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(acc[e] / l);
-  T *dst = static_cast<T *>(a.out) + ((s.out0 + row) * static_cast<int64_t>(a.G) * a.h_kv + head) * HD + 4 * lane;
-  *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(o);
+  *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + at * HD + 4 * lane) = *reinterpret_cast<const uint2 *>(o);
 }
 
 template <typename T>
@@ -112,7 +205,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
                        const __grid_constant__ CUtensorMap mv, const __grid_constant__ PromptArgs a) {
   constexpr bool BF16 = __is_same(T, __nv_bfloat16);
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_q, bar_full[KV_STAGES], bar_empty[KV_STAGES], bar_s[2], bar_p[2], bar_o[2], bar_end;
+  __shared__ __align__(8) uint64_t bar_q, bar_full[KV_STAGES], bar_empty[KV_STAGES], bar_s[2], bar_p[2][2], bar_o[2], bar_end;
   __shared__ uint32_t tmem_base;
   __shared__ int item_seq, item_pair;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -121,9 +214,10 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
   // ---- which sequence, key head and pair of tiles
   Seq s;
   int h, pair;
+  const int z = blockIdx.x % a.splits, item = blockIdx.x / a.splits;      // neighbours share query tiles
   if (a.cu_q == nullptr) {
-    const int sh = blockIdx.x % (a.B * a.h_kv);
-    pair = a.pairs - 1 - blockIdx.x / (a.B * a.h_kv);      // the longest rows first
+    const int sh = item % (a.B * a.h_kv);
+    pair = a.pairs - 1 - item / (a.B * a.h_kv);      // the longest rows first
     s.b = sh / a.h_kv;
     h = sh % a.h_kv;
     s.q0 = s.k0 = 0;
@@ -132,8 +226,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     s.rows = a.Lq;
     s.out0 = static_cast<int64_t>(s.b) * a.Lq;
   } else {
-    h = blockIdx.x % a.h_kv;
-    const int want = blockIdx.x / a.h_kv;
+    h = item % a.h_kv;
+    const int want = item / a.h_kv;
     if (warp == 0) {
       const int nseq = a.B + (a.zero_rest ? 1 : 0);
       int base = 0, found = -1, fp = 0;
@@ -189,14 +283,24 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     const int last = min(row0[x] + PT, s.nq) - 1;
     nblk[x] = live[x] && last >= row0[x] ? (key_limit(s, last, a.causal) + PT - 1) / PT : 0;
   }
-  const int n = max(nblk[0], nblk[1]);
+  // this block's key tiles: all of them, or the z-th part
+  const int most = max(nblk[0], nblk[1]);
+  const int j0 = static_cast<int>(static_cast<int64_t>(most) * z / a.splits);
+  const int n = static_cast<int>(static_cast<int64_t>(most) * (z + 1) / a.splits) - j0;
+#pragma unroll
+  for (int x = 0; x < 2; ++x) nblk[x] = min(max(nblk[x] - j0, 0), n);
 
   if (n > 0) {
     if (warp == 9) tmem_alloc(smem_u32(&tmem_base), 512);
     if (threadIdx.x == 0) {
       mbar_init(smem_u32(&bar_q), 1);
       for (int i = 0; i < KV_STAGES; ++i) mbar_init(smem_u32(&bar_full[i]), 1), mbar_init(smem_u32(&bar_empty[i]), 1);
-      for (int x = 0; x < 2; ++x) mbar_init(smem_u32(&bar_s[x]), 1), mbar_init(smem_u32(&bar_p[x]), PT), mbar_init(smem_u32(&bar_o[x]), 1);
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(smem_u32(&bar_s[x]), 1);
+        mbar_init(smem_u32(&bar_p[x][0]), PT);
+        mbar_init(smem_u32(&bar_p[x][1]), PT);
+        mbar_init(smem_u32(&bar_o[x]), 1);
+      }
       mbar_init(smem_u32(&bar_end), 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -234,7 +338,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           mbar_expect_tx(bf, TILE_BYTES);
           const CUtensorMap *m = (i & 1) ? &mv : &mk;
           for (int c = 0; c < 2; ++c)
-            tma_load_4d(kv_addr + st * TILE_BYTES + c * (TILE_BYTES / 2), m, bf, 64 * c, s.k0 + (i >> 1) * PT, h, s.b);
+            tma_load_4d(kv_addr + st * TILE_BYTES + c * (TILE_BYTES / 2), m, bf, 64 * c, s.k0 + (j0 + (i >> 1)) * PT, h, s.b);
         }
         if (!ok)                                              // leave no copy in flight behind
           for (int j = max(0, i - KV_STAGES); j < i; ++j) mbar_wait(smem_u32(&bar_full[j % KV_STAGES]), (j / KV_STAGES) & 1);
@@ -266,8 +370,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         auto values = [&](int x, int j) {
           const uint32_t va = umma_lo(kv_addr + ((2 * j + 1) % KV_STAGES) * TILE_BYTES, TILE_BYTES / 2);
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            umma_ts(tmem + 2 * PT + x * HD, tmem + x * PT + kk * 8, va + (kk * 2048 >> 4), umma_hi(1024), ID_O, j > 0 || kk > 0);
+          for (int half = 0; half < 2; ++half) {
+            if (!wait(bar_p[x][half], j)) return;
+#pragma unroll
+            for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+              umma_ts(tmem + 2 * PT + x * HD, tmem + x * PT + kk * 8, va + (kk * 2048 >> 4), umma_hi(1024), ID_O, j > 0 || kk > 0);
+          }
           if (j + 1 == (x ? nblk[1] : nblk[0])) umma_commit(smem_u32(&bar_o[x]));
         };
         wait(bar_q, 0);
@@ -284,8 +392,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           for (int x = 0; x < 2 && ok; ++x) {
             const int nb = x ? nblk[1] : nblk[0];
             if (j < nb) {
-              if (!wait(bar_p[x], j)) break;
               values(x, j);
+              if (!ok) break;
             }
             if (x == 1) umma_commit(smem_u32(&bar_empty[sv]));
             if (j + 1 < n) {
@@ -312,28 +420,34 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     bool ok = true;
     // keys that every row of the tile sees need no comparison
     const int all = key_limit(s, min(row0[x], s.nq - 1), a.causal);
+    const uint64_t c2 = pk2(a.c, a.c);
     for (int j = 0; j < nb; ++j) {
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_s[x]), j & 1));
       if (!ok) break;
       tc_fence_after();
       float v[PT];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tmem_ld32(ts + 32 * i, v + 32 * i);
+      tmem_ld32(ts, v);
+      tmem_ld32(ts + 32, v + 32);
       tmem_wait_ld();
-      if ((j + 1) * PT > all) {
-        const int seen = limit - j * PT;
+      tmem_ld32(ts + 64, v + 64);
+      tmem_ld32(ts + 96, v + 96);
+      const bool masked = (j0 + j + 1) * PT > all;
+      const int seen = limit - (j0 + j) * PT;
+      float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < PT; ++i) v[i] = i < seen ? v[i] : -INFINITY;
-      }
-      float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
+      for (int half = 0; half < 2; ++half) {
+        if (half == 1) tmem_wait_ld();
+        if (masked) {
 #pragma unroll
-      for (int i = 0; i < PT; i += 8) {
-        t0 = fmaxf(t0, fmaxf(v[i], v[i + 1]));
-        t1 = fmaxf(t1, fmaxf(v[i + 2], v[i + 3]));
-        t2 = fmaxf(t2, fmaxf(v[i + 4], v[i + 5]));
-        t3 = fmaxf(t3, fmaxf(v[i + 6], v[i + 7]));
+          for (int i = 64 * half; i < 64 * half + 64; ++i) v[i] = i < seen ? v[i] : -INFINITY;
+        }
+#pragma unroll
+        for (int i = 64 * half; i < 64 * half + 64; i += 8) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t[e] = max3(t[e], v[i + 2 * e], v[i + 2 * e + 1]);
+        }
       }
-      const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+      const float top = max3(max3(t[0], t[1], t[2]), t[3], t[3]);
       const bool grow = (top - m) * a.c > LAG || m == -INFINITY;
       if (j == 0) {
         m = top;
@@ -353,69 +467,81 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         }
       }
       const float mc = m == -INFINITY ? 0.0f : m * a.c;
-      float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t w[32];
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const int e = 64 * half + 2 * i;
-          const float p0 = ex2(fmaf(v[e], a.c, -mc)), p1 = ex2(fmaf(v[e + 1], a.c, -mc));
-          const float p2 = ex2(fmaf(v[e + 2], a.c, -mc)), p3 = ex2(fmaf(v[e + 3], a.c, -mc));
-          s0 += p0;
-          s1 += p1;
-          s2 += p2;
-          s3 += p3;
-          if constexpr (BF16) {
-            __nv_bfloat162 x0 = __floats2bfloat162_rn(p0, p1), x1 = __floats2bfloat162_rn(p2, p3);
-            w[i] = *reinterpret_cast<uint32_t *>(&x0);
-            w[i + 1] = *reinterpret_cast<uint32_t *>(&x1);
-          } else {
-            w[i] = pack_h2(p0, p1);
-            w[i + 1] = pack_h2(p2, p3);
-          }
-        }
-        tmem_st32(ts + 32 * half, w);
-      }
-      l += (s0 + s1) + (s2 + s3);
+      const uint64_t nmc2 = pk2(-mc, -mc);
+      // the polynomial is for finite logits: a tile with masked ones, or a row that met an infinity or NaN, goes through
+      // the exponential unit alone
+      uint64_t sum;
+      const bool plain = masked || __any_sync(0xffffffffu, !(fabsf(top) < INFINITY));
+      if (plain) sum = weights64<T, false>(v, c2, nmc2, ts);
+      else sum = weights64<T, true>(v, c2, nmc2, ts);
       tmem_wait_st();
       tc_fence_before();
-      mbar_arrive(smem_u32(&bar_p[x]));
+      mbar_arrive(smem_u32(&bar_p[x][0]));
+      if (plain) sum = add2(sum, weights64<T, false>(v + 64, c2, nmc2, ts + 32));
+      else sum = add2(sum, weights64<T, true>(v + 64, c2, nmc2, ts + 32));
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(smem_u32(&bar_p[x][1]));
+      const float2 sf = un2(sum);
+      l += sf.x + sf.y;
     }
     if (nb > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_o[x]), 0));
     if (!ok) give_up();
     if (live[x] && ok) {
       tc_fence_after();
       const bool mine = row < s.rows;
-      const float inv = limit > 0 ? 1.0f / l : 0.0f;
-      T *dst = static_cast<T *>(a.out) + ((s.out0 + row) * static_cast<int64_t>(a.G) * a.h_kv + head[x]) * HD;
+      const int64_t at_out = (s.out0 + row) * static_cast<int64_t>(a.G) * a.h_kv + head[x];
       bool odd = false;
+      if (a.splits == 1) {
+        const float inv = limit > 0 ? 1.0f / l : 0.0f;
+        T *dst = static_cast<T *>(a.out) + at_out * HD;
 #pragma unroll 1
-      for (int i = 0; i < 4; ++i) {
-        float o[32];
-        if (nb > 0) {
+        for (int i = 0; i < 4; ++i) {
+          float o[32];
+          if (nb > 0) {
+            tmem_ld32(to + 32 * i, o);
+            tmem_wait_ld();
+          }
+          uint4 w[4];
+          T *t = reinterpret_cast<T *>(w);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float y = limit > 0 ? o[e] * inv : 0.0f;
+            odd |= !(fabsf(y) < INFINITY);
+            t[e] = from_f32<T>(y);
+          }
+          if (mine) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) reinterpret_cast<uint4 *>(dst + 32 * i)[e] = w[e];
+          }
+        }
+      } else if (mine) {
+        // a part of the keys: the accumulator as it is, the maximum and the sum; no accumulator without a sum
+        const int64_t pa = z * a.rows * a.G * a.h_kv + at_out;
+        const bool some = limit > j0 * PT && nb > 0;
+        a.part_ml[pa] = limit == 0 ? make_float2(-INFINITY, -1.0f) : some ? make_float2(m == -INFINITY ? m : m * a.c, l) : make_float2(-INFINITY, 0.0f);
+      }
+      if (a.splits > 1 && nb > 0) {
+        float *dst = a.part + (z * a.rows * a.G * a.h_kv + at_out) * HD;
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          float o[32];
           tmem_ld32(to + 32 * i, o);
           tmem_wait_ld();
-        }
-        uint4 w[4];
-        T *t = reinterpret_cast<T *>(w);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float y = limit > 0 ? o[e] * inv : 0.0f;
-          odd |= !(fabsf(y) < INFINITY);
-          t[e] = from_f32<T>(y);
-        }
-        if (mine) {
+          for (int e = 0; e < 32; ++e) odd |= limit > 0 && !(fabsf(o[e]) < INFINITY);
+          if (mine && limit > j0 * PT) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) reinterpret_cast<uint4 *>(dst + 32 * i)[e] = w[e];
+            for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(dst + 32 * i + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
         }
       }
       unsigned again = __ballot_sync(0xffffffffu, odd && mine);
       while (again) {
         const int r = __ffs(again) - 1;
         again &= again - 1;
-        const int touched = min(nb * PT, a.Lk - s.k0);
-        repair_row<T>(a, s, __shfl_sync(0xffffffffu, row, r), head[x], __shfl_sync(0xffffffffu, limit, r), touched);
+        const int hi = min((j0 + nb) * PT, a.Lk - s.k0);
+        repair_row<T>(a, s, __shfl_sync(0xffffffffu, row, r), head[x], __shfl_sync(0xffffffffu, limit, r), j0 * PT, hi, z);
       }
     }
     tc_fence_before();
@@ -426,6 +552,54 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     tc_fence_after();
     if (warp == 9) tmem_free(tmem, 512);
   }
+}
+
+// Joins the parts of split keys: one warp per (row, query head), four channels a lane.
+template <typename T>
+__global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant__ PromptArgs a) {
+  const int64_t n = a.rows * a.G * a.h_kv;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  dep_wait();
+  if (at >= n) return;
+  if (a.cu_q != nullptr && !a.zero_rest) {       // rows of no sequence are left as they are
+    const int64_t row = at / (a.G * a.h_kv);
+    if (row >= a.cu_q[a.B] || row < a.cu_q[0]) return;
+  }
+  // the parts' maxima and sums, a part per lane
+  float m = -INFINITY, l = 0.0f, acc[4] = {};
+  for (int z0 = 0; z0 < a.splits; z0 += 32) {
+    const float2 ml = z0 + lane < a.splits ? a.part_ml[(z0 + lane) * n + at] : make_float2(-INFINITY, 0.0f);
+    float top = ml.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.0f : mn;
+    const float f = ex2(m - ref);
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= f;
+    m = mn;
+    const float w = ml.y == 0.0f ? 0.0f : ex2(ml.x - ref);
+    for (int i = 0; i < min(32, a.splits - z0); ++i) {
+      const float li = __shfl_sync(0xffffffffu, ml.y, i), wi = __shfl_sync(0xffffffffu, w, i);
+      if (li < 0.0f) {                            // a row that sees nothing says so in every part
+        l = -1.0f;
+        break;
+      }
+      if (li == 0.0f) continue;
+      const float4 x = *reinterpret_cast<const float4 *>(a.part + ((z0 + i) * n + at) * HD + 4 * lane);
+      l = fmaf(li, wi, l);
+      acc[0] = fmaf(x.x, wi, acc[0]);
+      acc[1] = fmaf(x.y, wi, acc[1]);
+      acc[2] = fmaf(x.z, wi, acc[2]);
+      acc[3] = fmaf(x.w, wi, acc[3]);
+    }
+    if (l < 0.0f) break;
+  }
+  T o[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(l < 0.0f ? 0.0f : acc[e] / l);
+  *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + at * HD + 4 * lane) = *reinterpret_cast<const uint2 *>(o);
 }
 
 // Token rows of one head as boxes of 128 rows x 64 channels in the 128-byte swizzle; what lies outside reads as zero.
@@ -460,6 +634,40 @@ bool make_map(CUtensorMap *m, const void *base, bool bf16, int64_t T, int64_t H,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Pairs of tiles of a call (packed: the most that its sequences can need).
+int64_t prompt_pairs(bool packed, int64_t B, int64_t Lq, int64_t G, bool rest) {
+  if (!packed) return ((Lq + PT - 1) / PT * G + 1) / 2 * B;
+  const int64_t nseq = B + rest;
+  return ((Lq / PT + nseq) * G + 1) / 2 + nseq;
+}
+
+// In how many parts the keys are cut.  Unit: the time of one key tile against a pair of query tiles; a block of threads
+// costs FIXED of them besides its tiles, and joining parts costs a launch and the parts' way through memory.
+int prompt_splits(bool packed, int64_t B, int64_t Lq, int64_t Lk, int64_t h_kv, int64_t G, bool causal) {
+  constexpr double FIXED = 2.5, JOIN = 3.0;
+  if (Lq == 0 || Lk == 0 || B == 0) return 1;
+  const int64_t sms = sm_count();
+  const int64_t nseq = packed ? B : 1;
+  const double nq = static_cast<double>(Lq) / nseq, nk = static_cast<double>(Lk) / nseq;     // of one sequence
+  const double longest = ceil(nk / PT);
+  const double mean = causal ? fmax(1.0, (nk - fmin(nq, nk) / 2) / PT) : longest;
+  const double items = ceil(ceil(nq / PT) * G / 2) * h_kv * B;
+  const double traffic = static_cast<double>(packed ? Lq : B * Lq) * h_kv * G * (HD + 2) * 8 / 6.5e12 / 1.3e-6;   // tiles' time, per part
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= 64 && s <= longest; ++s) {
+    const double work = items * s * (mean / s + FIXED);
+    // equal blocks run in whole waves; unequal ones (longest first) fill in, but the longest is the least there is
+    double t = mean > 0.8 * longest ? ceil(items * s / sms) * (mean / s + FIXED) : fmax(work / sms, longest / s + FIXED);
+    if (s > 1) t += JOIN + traffic * s;
+    if (s == 1 || t < 0.95 * least) {
+      best = s;
+      least = t;
+    }
+  }
+  return best;
+}
+
 template <typename T>
 int launch_prompt(const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMap &mv, const PromptArgs &a, unsigned grid,
                   cudaStream_t s) {
@@ -471,17 +679,30 @@ int launch_prompt(const CUtensorMap &mq, const CUtensorMap &mk, const CUtensorMa
   });
   if (rc != KITTY_OK) return rc;
   prompt_attn_kernel<T><<<grid, PROMPT_THREADS, PROMPT_SMEM, s>>>(mq, mk, mv, a);
-  return cudaGetLastError() == cudaSuccess ? KITTY_OK : KITTY_E_CUDA;
+  if (cudaGetLastError() != cudaSuccess) return KITTY_E_CUDA;
+  if (a.splits == 1) return KITTY_OK;
+  const int64_t rows = a.rows * a.G * a.h_kv;
+  const cudaError_t e = launch_after(prompt_join_kernel<T>, dim3(static_cast<unsigned>((rows + 7) / 8)), dim3(256), 0, s, a);
+  return (e == cudaSuccess && cudaGetLastError() == cudaSuccess) ? KITTY_OK : KITTY_E_CUDA;
 }
 
 }  // namespace kitty
 
 using namespace kitty;
 
+extern "C" int64_t kitty_prompt_workspace_bytes(int32_t B, int64_t Lq, int64_t Lk, int32_t h_q, int32_t h_kv, int causal,
+                                                int packed) {
+  if (B < 0 || Lq < 0 || Lk < 0 || h_q <= 0 || h_kv <= 0 || h_q % h_kv != 0) return KITTY_E_BADARG;
+  if (Lq > (1 << 30) || Lk > (1 << 30)) return KITTY_E_BADSHAPE;
+  const int s = prompt_splits(packed != 0, B, Lq, Lk, h_kv, h_q / h_kv, causal != 0);
+  return s == 1 ? 0 : (packed ? Lq : B * Lq) * h_q * s * (HD + 2) * 4;
+}
+
 extern "C" int kitty_prompt_attn(const void *q, const void *k, const void *v, int dtype, const int64_t *strides,
                                  int32_t B, int64_t Lq, int64_t Lk, int32_t h_q, int32_t h_kv, float scaling,
                                  int causal, const int32_t *q_lens, const int32_t *k_lens, const int32_t *cu_q,
-                                 const int32_t *cu_k, void *out, int zero_rest, int32_t *status, void *stream) {
+                                 const int32_t *cu_k, void *out, int zero_rest, int32_t *status, void *workspace,
+                                 int64_t workspace_bytes, void *stream) {
   if (!strides || B < 0 || Lq < 0 || Lk < 0 || h_q <= 0 || h_kv <= 0 || h_q % h_kv != 0) return KITTY_E_BADARG;
   if (dtype != KITTY_F16 && dtype != KITTY_BF16) return KITTY_E_BADARG;
   if (!(scaling > 0.0f) || !(scaling < INFINITY)) return KITTY_E_BADARG;
@@ -518,14 +739,21 @@ extern "C" int kitty_prompt_attn(const void *q, const void *k, const void *v, in
   a.causal = causal != 0;
   a.zero_rest = zero_rest != 0;
   a.c = scaling * 1.4426950408889634f;
-  int64_t grid;
-  if (packed) {
-    const int64_t nseq = static_cast<int64_t>(B) + a.zero_rest;
-    grid = (((Lq / PT + nseq) * a.G + 1) / 2 + nseq) * h_kv;      // most pairs of tiles that nseq sequences can need
-  } else {
-    a.pairs = static_cast<int32_t>(((Lq + PT - 1) / PT * a.G + 1) / 2);
-    grid = static_cast<int64_t>(a.pairs) * B * h_kv;
+  a.rows = packed ? Lq : B * Lq;
+  a.splits = 1;
+  if (workspace != nullptr) {
+    const int64_t need = kitty_prompt_workspace_bytes(B, Lq, Lk, h_q, h_kv, causal, packed);
+    if (workspace_bytes < need) return KITTY_E_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return KITTY_E_BADARG;
+    if (need > 0) {
+      a.splits = prompt_splits(packed, B, Lq, Lk, h_kv, a.G, a.causal);
+      a.part = static_cast<float *>(workspace);
+      a.part_ml = reinterpret_cast<float2 *>(a.part + a.splits * a.rows * h_q * HD);
+    }
   }
+  const int64_t pairs = prompt_pairs(packed, B, Lq, a.G, a.zero_rest);
+  if (!packed) a.pairs = static_cast<int32_t>(B > 0 ? pairs / B : 0);
+  const int64_t grid = pairs * h_kv * a.splits;
   if (grid > 0x7fffffff || (Lq + PT) / PT * a.G > 0x7fffffff) return KITTY_E_BADSHAPE;
   if (grid == 0) return KITTY_OK;
   const bool bf16 = dtype == KITTY_BF16;

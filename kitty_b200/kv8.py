@@ -67,14 +67,28 @@ class KV8Layer:
         self.tail_v = torch.zeros((MAX_BS, H_KV, BLOCK, D), dtype=dtype, device=dev)
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self._workspace_need: dict = {}
+        self._c_layer = self._c_table = None
 
     def c_layer(self) -> "_lib.KittyKV8Layer":
-        L = _lib.KittyKV8Layer(self.MAX_BS, self.MAX_PAGE, self.num_pages, self.H_KV, self.D, _lib.dtype_code(self.dtype))
-        for name in ("pages", "tail_k", "tail_v", "page_table", "status"):
-            t = getattr(self, name)
-            assert t.is_contiguous() and t.device == self.device, name
-            setattr(L, name, t.data_ptr())
-        assert tuple(self.page_table.shape) == (self.MAX_BS, self.MAX_PAGE) and self.page_table.dtype == torch.int64
+        """struct kitty_kv8_layer.  The buffers are the constructor's; the page table may have been replaced."""
+        L = self._c_layer
+        table = self.page_table
+        if L is None:
+            L = _lib.KittyKV8Layer(self.MAX_BS, self.MAX_PAGE, self.num_pages, self.H_KV, self.D,
+                                   _lib.dtype_code(self.dtype))
+            for name in ("pages", "tail_k", "tail_v", "status"):
+                t = getattr(self, name)
+                assert t.is_contiguous() and t.device == self.device, name
+                setattr(L, name, t.data_ptr())
+            self._c_layer = L
+        if self._c_table is not table:
+            if tuple(table.shape) != (self.MAX_BS, self.MAX_PAGE) or table.dtype != torch.int64 \
+                    or table.device != self.device or not table.is_contiguous():
+                raise ValueError(f"page_table must be contiguous int64 [{self.MAX_BS}, {self.MAX_PAGE}] on {self.device}")
+            # a new struct: another thread's call may be reading the old one
+            L = self._c_layer = _lib.KittyKV8Layer.from_buffer_copy(L)
+            L.page_table = table.data_ptr()
+            self._c_table = table
         return L
 
     def check(self) -> None:
@@ -99,17 +113,18 @@ class KV8Layer:
 
 
 def _row_tensor(x: torch.Tensor, what: str, B: int, layer: KV8Layer) -> torch.Tensor:
-    if not isinstance(x, torch.Tensor) or x.dtype != torch.int32 or tuple(x.shape) != (B,) or x.device != layer.device:
+    if not isinstance(x, torch.Tensor) or x.dtype != torch.int32 or x.shape != (B,) or x.device != layer.device:
         raise ValueError(f"{what} must be an int32 tensor [{B}] on {layer.device}")
     return x if x.is_contiguous() else x.contiguous()
 
 
 def _tokens(x: torch.Tensor, what: str, heads: int, layer: KV8Layer) -> torch.Tensor:
-    if x.dim() != 4 or x.shape[1] != heads or x.shape[3] != layer.D:
-        raise ValueError(f"expected {what} [B, {heads}, T, {layer.D}], got {tuple(x.shape)}")
-    if not x.is_cuda:
-        raise ValueError(f"kitty_b200 has no CPU path: the {what} must be on a CUDA device")
+    shape = x.shape
+    if len(shape) != 4 or shape[1] != heads or shape[3] != layer.D:
+        raise ValueError(f"expected {what} [B, {heads}, T, {layer.D}], got {tuple(shape)}")
     if x.dtype != layer.dtype or x.device != layer.device:
+        if not x.is_cuda:
+            raise ValueError(f"kitty_b200 has no CPU path: the {what} must be on a CUDA device")
         raise ValueError(f"the {what} must be {layer.dtype} on {layer.device}, got {x.dtype} on {x.device}")
     return x if x.stride(3) == 1 else x.contiguous()
 
@@ -145,16 +160,13 @@ def kv8_append(layer: KV8Layer, key: torch.Tensor, value: torch.Tensor, start: t
         out = torch.empty((B, h_q, T, layer.D), dtype=layer.dtype, device=layer.device)
         strides += _head_strides(query)
     else:
-        strides += [0, 0, 0]
+        strides += (0, 0, 0)
     if rotary is not None and rotary.device != layer.device:
         raise ValueError(f"the angles are on {rotary.device}, the cache on {layer.device}")
-    with torch.cuda.device(layer.device):
-        rc = _lib.lib().kitty_kv8_append(layer.c_layer(), k.data_ptr(), v.data_ptr(), _lib.i64_array(strides),
-                                         start.data_ptr(), None if lengths is None else lengths.data_ptr(), B, T,
-                                         None if rotary is None else rotary.c_plan(),
-                                         query.data_ptr() if h_q else None, out.data_ptr() if h_q else None, h_q,
-                                         _lib.stream_ptr(layer.device))
-    _lib.check(rc, "kitty_kv8_append")
+    _lib.call_on(layer.device, _lib.lib().kitty_kv8_append, "kitty_kv8_append", layer.c_layer(), k.data_ptr(),
+                 v.data_ptr(), _lib.i64_array(strides), start.data_ptr(), None if lengths is None else lengths.data_ptr(),
+                 B, T, None if rotary is None else rotary.c_plan(), query.data_ptr() if h_q else None,
+                 out.data_ptr() if h_q else None, h_q)
     return out
 
 
@@ -172,10 +184,8 @@ def kv8_expand(layer: KV8Layer, lengths: torch.Tensor, n: int, *, start: Optiona
         start = _row_tensor(start, "start", B, layer)
     k = torch.empty((B, layer.H_KV, n, layer.D), dtype=layer.dtype, device=layer.device)
     v = torch.empty_like(k)
-    with torch.cuda.device(layer.device):
-        rc = _lib.lib().kitty_kv8_expand(layer.c_layer(), lengths.data_ptr(), None if start is None else start.data_ptr(),
-                                         k.data_ptr(), v.data_ptr(), B, n, _lib.stream_ptr(layer.device))
-    _lib.check(rc, "kitty_kv8_expand")
+    _lib.call_on(layer.device, _lib.lib().kitty_kv8_expand, "kitty_kv8_expand", layer.c_layer(), lengths.data_ptr(),
+                 None if start is None else start.data_ptr(), k.data_ptr(), v.data_ptr(), B, n)
     return k, v
 
 
@@ -200,9 +210,7 @@ def kv8_attention(query: torch.Tensor, layer: KV8Layer, lengths: torch.Tensor, s
     elif tuple(out.shape) != (B, 1, h_q, D) or out.dtype != layer.dtype or out.device != layer.device \
             or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {layer.dtype} [{B}, 1, {h_q}, {D}] on {layer.device}")
-    with torch.cuda.device(layer.device):
-        ws = torch.empty(need, dtype=torch.uint8, device=layer.device)
-        rc = _lib.lib().kitty_kv8_attn(layer.c_layer(), lengths.data_ptr(), q.data_ptr(), B, h_q, float(scaling),
-                                       out.data_ptr(), ws.data_ptr(), need, _lib.stream_ptr(layer.device))
-    _lib.check(rc, "kitty_kv8_attn")
+    ws = torch.empty(need, dtype=torch.uint8, device=layer.device)
+    _lib.call_on(layer.device, _lib.lib().kitty_kv8_attn, "kitty_kv8_attn", layer.c_layer(), lengths.data_ptr(),
+                 q.data_ptr(), B, h_q, float(scaling), out.data_ptr(), ws.data_ptr(), need)
     return out

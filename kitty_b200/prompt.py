@@ -11,7 +11,6 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .rotary import _head_strides
 
 HEAD_DIM = 128
 _status: dict = {}
@@ -34,15 +33,34 @@ def prompt_attention_status(device="cuda") -> int:
 def _lengths(x, what: str, n: int, device) -> Optional[torch.Tensor]:
     if x is None:
         return None
-    if not isinstance(x, torch.Tensor) or x.dtype != torch.int32 or tuple(x.shape) != (n,) or x.device != device:
+    if not isinstance(x, torch.Tensor) or x.dtype != torch.int32 or x.shape != (n,) or x.device != device:
         raise ValueError(f"{what} must be an int32 tensor [{n}] on {device}")
     return x.contiguous()
 
 
-def _source(x: torch.Tensor) -> torch.Tensor:
-    """The tensor itself where the copies can read it in place: consecutive channels, no repeated dimension."""
-    bad = x.stride(-1) != 1 or any(n > 1 and s <= 0 for n, s in zip(x.shape, x.stride()))
-    return x.contiguous() if bad else x
+def _source(x: torch.Tensor, what: str, like: torch.Tensor, packed: bool):
+    """The tensor, in place where the copies can read it (consecutive channels, no repeated dimension), and its (batch,
+    head, token) strides."""
+    shape, dev = x.shape, x.device
+    if len(shape) != (3 if packed else 4) or shape[-1] != HEAD_DIM:
+        raise ValueError(f"expected {what} {'[T, H, 128]' if packed else '[B, H, T, 128]'}, got {tuple(shape)}")
+    if dev.type != "cuda":
+        raise ValueError(f"kitty_b200 has no CPU path: the {what} must be on a CUDA device")
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"prompt_attention takes float16 or bfloat16 tensors, got {x.dtype}")
+    if x is not like and (x.dtype != like.dtype or dev != like.device):
+        raise ValueError("query, key and value must agree in type and device")
+    for again in (False, True):
+        if packed:
+            t, h, d = x.stride()
+            st = (0, h if shape[1] > 1 else 0, t if shape[0] > 1 else 0)
+        else:
+            b, h, t, d = x.stride()
+            st = (b if shape[0] > 1 else 0, h if shape[1] > 1 else 0, t if shape[2] > 1 else 0)
+        if d == 1 and (shape[0] < 2 or packed or b > 0) and (shape[1] < 2 or h > 0) and (shape[-3 if packed else 2] < 2 or t > 0):
+            break
+        x = x.contiguous()
+    return x, st
 
 
 def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, scaling: float, *, causal: bool = True,
@@ -61,17 +79,9 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     causal: the last query of a sequence sees its last key, so with more keys than queries the queries are a further
     piece of a prompt.  A row that sees no key is zero.  What a row does not see does not reach it, whatever it holds."""
     packed = cu_seqlens is not None
-    dims = 3 if packed else 4
-    form = "[T, H, 128]" if packed else "[B, H, T, 128]"
-    for x, what in ((query, "query"), (key, "key"), (value, "value")):
-        if x.dim() != dims or x.shape[-1] != HEAD_DIM:
-            raise ValueError(f"expected {what} {form}, got {tuple(x.shape)}")
-        if not x.is_cuda:
-            raise ValueError(f"kitty_b200 has no CPU path: the {what} must be on a CUDA device")
-        if x.dtype not in (torch.float16, torch.bfloat16):
-            raise TypeError(f"prompt_attention takes float16 or bfloat16 tensors, got {x.dtype}")
-        if x.dtype != query.dtype or x.device != query.device:
-            raise ValueError("query, key and value must agree in type and device")
+    q, q_st = _source(query, "query", query, packed)
+    k, k_st = _source(key, "key", query, packed)
+    v, v_st = _source(value, "value", query, packed)
     if key.shape != value.shape:
         raise ValueError(f"key and value differ in shape: {tuple(key.shape)} and {tuple(value.shape)}")
     dev = query.device
@@ -107,14 +117,13 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         out = torch.empty(shape, dtype=query.dtype, device=dev)
     elif tuple(out.shape) != shape or out.dtype != query.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {query.dtype} {list(shape)} on {dev}")
-    q, k, v = _source(query), _source(key), _source(value)
-    order = (lambda x: [0] + [x.stride(i) if x.shape[i] > 1 else 0 for i in (1, 0)]) if packed else _head_strides
-    ptr = lambda x: None if x is None else x.data_ptr()  # noqa: E731
-    with torch.cuda.device(dev):
-        rc = _lib.lib().kitty_prompt_attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.dtype_code(q.dtype),
-                                          _lib.i64_array(order(q) + order(k) + order(v)), B, Lq, Lk, h_q, h_kv,
-                                          float(scaling), int(causal), ptr(q_len), ptr(k_len), ptr(cu_q), ptr(cu_k),
-                                          out.data_ptr(), int(zero_rest), _status_word(dev).data_ptr(),
-                                          _lib.stream_ptr(dev))
-    _lib.check(rc, "kitty_prompt_attn")
+    lib = _lib.lib()
+    need = lib.kitty_prompt_workspace_bytes(B, Lq, Lk, h_q, h_kv, int(causal), int(packed))
+    if need < 0:
+        _lib.check(int(need), "kitty_prompt_workspace_bytes")
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _lib.call_on(dev, lib.kitty_prompt_attn, "kitty_prompt_attn", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                 _lib.dtype_code(q.dtype), _lib.i64_array(q_st + k_st + v_st), B, Lq, Lk, h_q, h_kv, float(scaling),
+                 int(causal), *(None if x is None else x.data_ptr() for x in (q_len, k_len, cu_q, cu_k)), out.data_ptr(),
+                 int(zero_rest), _status_word(dev).data_ptr(), None if ws is None else ws.data_ptr(), need)
     return out

@@ -113,21 +113,22 @@ class RotaryEmbedding:
 
 def _head_strides(x: torch.Tensor):
     """(batch, head, token) strides; a dimension of size one has none (views may carry any number there)."""
-    return [x.stride(i) if x.shape[i] > 1 else 0 for i in range(3)]
+    a, b, c, _ = x.stride()
+    n, m, t, _ = x.shape
+    return (a if n > 1 else 0, b if m > 1 else 0, c if t > 1 else 0)
 
 
-def _rotary_input(x: torch.Tensor, what: str) -> torch.Tensor:
+def _rotary_input(x: torch.Tensor, what: str, device) -> torch.Tensor:
     if x.dim() != 4 or x.shape[3] != HEAD_DIM:
         raise ValueError(f"expected {what} [B, H, T, 128], got {tuple(x.shape)}")
-    if not x.is_cuda:
-        raise ValueError(f"kitty_b200 has no CPU path: the {what} must be on a CUDA device")
+    if x.device != device:
+        if not x.is_cuda:
+            raise ValueError(f"kitty_b200 has no CPU path: the {what} must be on a CUDA device")
+        raise ValueError(f"the angles are on {device}, the {what} on {x.device}")
     return x if x.stride(3) == 1 else x.contiguous()
 
 
-def _rotary_output(out: Optional[torch.Tensor], x: torch.Tensor, what: str) -> torch.Tensor:
-    """A new tensor in the input's own memory order, or the given one after its checks."""
-    if out is None:
-        return torch.empty_like(x)
+def _rotary_output(out: torch.Tensor, x: torch.Tensor, what: str) -> torch.Tensor:
     if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(3) != 1:
         raise ValueError(f"{what}_out must have the {what}'s shape, type and device, with consecutive channels")
     if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
@@ -156,27 +157,30 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
     `positions` (int64 [T], [1, T] or [B, T]).  Returns (query, key) turned, in new tensors of the same memory order,
     or in query_out / key_out, which may be query and key themselves (in place); other overlaps of outputs and inputs
     are the caller's error and refused where the views' spans show them."""
-    q, k = _rotary_input(query, "query"), _rotary_input(key, "key")
-    B, _, T, _ = q.shape
-    if k.shape[0] != B or k.shape[2] != T or k.dtype != q.dtype or k.device != q.device:
-        raise ValueError("query and key must agree in batch, tokens, type and device")
-    if rotary.device != q.device:
-        raise ValueError(f"the angles are on {rotary.device}, the query on {q.device}")
-    if positions.dim() == 1:
-        positions = positions.unsqueeze(0)
-    if positions.dim() != 2 or positions.shape[1] != T or positions.shape[0] not in (1, B):
-        raise ValueError(f"expected positions [T], [1, T] or [B, T] for B={B}, T={T}, got {tuple(positions.shape)}")
-    if positions.dtype != torch.int64 or positions.device != q.device:
-        raise ValueError("positions must be int64 on the query's device")
-    if T > 1 and positions.stride(1) != 1:
-        positions = positions.contiguous()
-    qo, ko = _rotary_output(query_out, q, "query"), _rotary_output(key_out, k, "key")
+    dev = rotary.device
+    q, k = _rotary_input(query, "query", dev), _rotary_input(key, "key", dev)
+    B, h_q, T, _ = q.shape
+    Bk, h_kv, Tk, _ = k.shape
+    if Bk != B or Tk != T or k.dtype != q.dtype:
+        raise ValueError("query and key must agree in batch, tokens and type")
     code = _lib.dtype_code(q.dtype)
+    shape = positions.shape
+    if len(shape) == 1:
+        rows, cols = 1, shape[0]
+    elif len(shape) == 2:
+        rows, cols = shape
+    else:
+        rows = cols = -1
+    if cols != T or rows not in (1, B):
+        raise ValueError(f"expected positions [T], [1, T] or [B, T] for B={B}, T={T}, got {tuple(shape)}")
+    if positions.dtype != torch.int64 or positions.device != dev:
+        raise ValueError("positions must be int64 on the query's device")
+    if T > 1 and positions.stride(-1) != 1:
+        positions = positions.contiguous()
+    qo = torch.empty_like(q) if query_out is None else _rotary_output(query_out, q, "query")
+    ko = torch.empty_like(k) if key_out is None else _rotary_output(key_out, k, "key")
     strides = _lib.i64_array(_head_strides(q) + _head_strides(k) + _head_strides(qo) + _head_strides(ko))
-    with torch.cuda.device(q.device):
-        rc = _lib.lib().kitty_rotary(rotary.c_plan(), q.data_ptr(), k.data_ptr(), positions.data_ptr(),
-                                     positions.stride(0) if positions.shape[0] > 1 else 0, qo.data_ptr(),
-                                     ko.data_ptr(), code, B, T, q.shape[1], k.shape[1], strides,
-                                     _lib.stream_ptr(q.device))
-    _lib.check(rc, "kitty_rotary")
+    _lib.call_on(dev, _lib.lib().kitty_rotary, "kitty_rotary", rotary.c_plan(), q.data_ptr(), k.data_ptr(),
+                 positions.data_ptr(), positions.stride(0) if rows > 1 else 0, qo.data_ptr(), ko.data_ptr(), code, B, T,
+                 h_q, h_kv, strides)
     return qo, ko

@@ -229,7 +229,7 @@ def _row_view(layer, b):
     one.MAX_BS = 1
     one.page_table = layer.page_table[b:b + 1].contiguous()
     one.tail_k, one.tail_v = layer.tail_k[b:b + 1], layer.tail_v[b:b + 1]
-    one._workspace_need = {}
+    one._workspace_need, one._c_layer = {}, None
     return one
 
 

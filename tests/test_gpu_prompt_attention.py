@@ -137,6 +137,53 @@ def test_what_a_row_does_not_see(kb, dtype):
     assert torch.isinf(got[0, 350:390, :, 7]).all()
     assert torch.isnan(got[0, 390:]).all()
     assert torch.isfinite(clean).all()
+    k3 = k.clone()
+    k3[0, 0, 3, 9] = float("nan")                                      # every row but the first three
+    got = kb.prompt_attention(q, k3, v, SC)
+    assert torch.isnan(got[0, 3:]).all() and torch.equal(got[0, :3], clean[0, :3])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,hq,h,Lq,Lk,causal", [(1, 8, 2, 1, 5000, True), (2, 4, 2, 130, 3001, True), (1, 7, 1, 3, 12000, True),
+                                                 (1, 4, 4, 257, 2500, False), (1, 1, 1, 700, 600, True)])
+def test_few_rows_over_many_keys(kb, dtype, B, hq, h, Lq, Lk, causal):
+    """Keys cut in parts and joined: ragged batches, rows that see nothing, values that a row does not see."""
+    from kitty_b200 import _lib
+
+    assert _lib.lib().kitty_prompt_workspace_bytes(B, Lq, Lk, hq, h, int(causal), 0) > 0 or Lk < 1000
+    q, k, v = _inputs((B, hq, Lq, 128), (B, h, Lk, 128), dtype, Lk)
+    got = kb.prompt_attention(q, k, v, SC, causal=causal)
+    for b in range(B):
+        _check_rows(got[b], *(x[b].transpose(0, 1) for x in (q, k, v)), SC, causal)
+    assert torch.equal(kb.prompt_attention(q, k, v, SC, causal=causal), got)
+    kl = torch.full((B,), Lk - 70, dtype=torch.int32, device=DEV)
+    kl[0] = 5 if B > 1 else Lk - 70
+    want = kb.prompt_attention(q[-1:], k[-1:, :, :Lk - 70].contiguous(), v[-1:, :, :Lk - 70].contiguous(), SC, causal=causal)
+    k[:, :, Lk - 70:], v[:, :, Lk - 70:] = float("nan"), float("inf")
+    got = kb.prompt_attention(q, k, v, SC, causal=causal, key_lengths=kl)
+    if B > 1:
+        n = Lq - 5                                                     # the first row's queries over five keys
+        assert (got[0, :n] == 0).all()
+        _check_rows(got[0, n:], q[0, :, n:].transpose(0, 1), k[0, :, :5].transpose(0, 1), v[0, :, :5].transpose(0, 1), SC, True)
+    _check_rows(got[-1], q[-1].transpose(0, 1), k[-1, :, :Lk - 70].transpose(0, 1), v[-1, :, :Lk - 70].transpose(0, 1), SC, causal)
+    # the same keys in other parts: two roundings of the same numbers
+    assert ((got[-1].float() - want[0].float()).abs() <= 4 * HALF[dtype] * v[-1, :, :Lk - 70].float().abs().max()).all()
+
+
+def test_packed_few_rows_over_many_keys(kb):
+    nq, nk = [2, 0, 40], [4000, 100, 6000]
+    q, _, _ = _inputs((45, 4, 128), (1, 1, 128), torch.float16, 1)
+    _, k, v = _inputs((1, 4, 128), (sum(nk), 1, 128), torch.float16, 2)
+    cq = torch.tensor([0, 2, 2, 42], dtype=torch.int32, device=DEV)
+    ck = torch.tensor([0, 4000, 4100, 10100], dtype=torch.int32, device=DEV)
+    k[4000:4100], v[4000:4100] = float("nan"), float("nan")
+    out = torch.full((45, 4, 128), 3.0, dtype=torch.float16, device=DEV)
+    kb.prompt_attention(q, k, v, SC, cu_seqlens=cq, cu_seqlens_k=ck, out=out)
+    assert (out[42:] == 3.0).all()
+    got = kb.prompt_attention(q, k, v, SC, cu_seqlens=cq, cu_seqlens_k=ck)
+    assert torch.equal(got[:42], out[:42]) and (got[42:] == 0).all()
+    _check_rows(got[:2], q[:2], k[:4000], v[:4000], SC, True)
+    _check_rows(got[2:42], q[2:42], k[4100:], v[4100:], SC, True)
 
 
 def test_extreme_logits(kb):

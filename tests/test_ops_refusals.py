@@ -44,9 +44,9 @@ def test_rotary_entry_point(L):
 
 
 def _prompt(L, q=P, k=P, v=P, dtype=0, st=(0,) * 9, B=1, Lq=1, Lk=1, hq=1, h=1, sc=1.0, ql=None, kl=None, cu=None, cuk=None,
-            out=P):
+            out=P, ws=None, nbytes=0):
     return L.lib().kitty_prompt_attn(q, k, v, dtype, L.i64_array(list(st)), B, Lq, Lk, hq, h, sc, 1, ql, kl, cu, cuk, out, 0,
-                                     None, None)
+                                     None, ws, nbytes, None)
 
 
 def test_prompt_entry_point(L):
@@ -55,6 +55,12 @@ def test_prompt_entry_point(L):
                dict(out=P + 4), dict(Lq=2), dict(Lq=2, st=(0, 0, 4) + (0,) * 6), dict(Lk=2, st=(0,) * 5 + (-128,) + (0,) * 3)):
         assert _prompt(L, **kw) == L.KITTY_E_BADARG, kw
     assert _prompt(L, Lq=(1 << 30) + 1) == L.KITTY_E_BADSHAPE
+    need = L.lib().kitty_prompt_workspace_bytes
+    assert need(1, 1, 100000, 8, 1, 1, 0) > 0 and need(16, 4096, 4096, 32, 8, 1, 0) == 0 and need(0, 0, 0, 1, 1, 1, 1) == 0
+    assert need(1, 1, 1, 3, 2, 1, 0) == L.KITTY_E_BADARG and need(1, 1 << 31, 1, 1, 1, 1, 0) == L.KITTY_E_BADSHAPE
+    far = dict(Lk=100000, hq=8, h=1, st=(0, 128, 0) + (0, 0, 128) * 2)
+    assert _prompt(L, ws=P, nbytes=16, **far) == L.KITTY_E_WORKSPACE
+    assert _prompt(L, ws=P + 8, nbytes=1 << 40, **far) == L.KITTY_E_BADARG
     assert _prompt(L, B=0) == L.KITTY_OK and _prompt(L, Lq=0) == L.KITTY_OK
 
 
@@ -115,8 +121,10 @@ def test_python_refusals_without_a_gpu():
                               "low_freq_factor": 4.0, "high_freq_factor": 4.0})):
         with pytest.raises(ValueError):
             kb.RotaryEmbedding(**{"device": "cpu", **bad})
+    import types
+
     with pytest.raises(ValueError, match="CUDA"):
-        kb.apply_rotary(x, x, torch.arange(4), None)
+        kb.apply_rotary(x, x, torch.arange(4), types.SimpleNamespace(device=torch.device("cuda", 0)))
     with pytest.raises(ValueError, match="CUDA"):
         kb.prompt_attention(x, x, x, 1.0)
     with pytest.raises(ValueError, match="expected query"):
