@@ -107,28 +107,23 @@ __device__ __forceinline__ uint32_t pack2(uint64_t p) {
   }
 }
 
-// Weights of 64 logits: 2^(v c - mc), their sum, and the 16-bit pairs in tensor memory.  POLY: every fourth pair goes
-// through the polynomial, which takes a quarter of the load off the 16-a-clock exponential unit.
+// Weights of 64 logits, 2^(v c - mc), as 16-bit pairs; returns their sum.  POLY: every fourth pair goes through the
+// polynomial, which takes a quarter of the load off the 16-a-clock exponential unit (for finite logits only).
 template <typename T, bool POLY>
-__device__ __forceinline__ uint64_t weights64(const float *v, uint64_t c2, uint64_t nmc2, uint32_t dst) {
+__device__ __forceinline__ uint64_t weights64(const float *v, uint64_t c2, uint64_t nmc2, uint32_t (&w)[32]) {
   uint64_t sum[2] = {0, 0};
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    uint32_t w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint64_t x = fma2(pk2(v[32 * q + 2 * i], v[32 * q + 2 * i + 1]), c2, nmc2);
-      uint64_t p;
-      if (POLY && (i & 3) == 3) {
-        p = ex2_poly2(x);
-      } else {
-        const float2 f = un2(x);
-        p = pk2(ex2(f.x), ex2(f.y));
-      }
-      sum[i & 1] = add2(sum[i & 1], p);
-      w[i] = pack2<T>(p);
+  for (int i = 0; i < 32; ++i) {
+    const uint64_t x = fma2(pk2(v[2 * i], v[2 * i + 1]), c2, nmc2);
+    uint64_t p;
+    if (POLY && (i & 3) == 3) {
+      p = ex2_poly2(x);
+    } else {
+      const float2 f = un2(x);
+      p = pk2(ex2(f.x), ex2(f.y));
     }
-    tmem_st16(dst + 16 * q, w);
+    sum[i & 1] = add2(sum[i & 1], p);
+    w[i] = pack2<T>(p);
   }
   return add2(sum[0], sum[1]);
 }
@@ -208,7 +203,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
   __shared__ __align__(8) uint64_t bar_q, bar_full[KV_STAGES], bar_empty[KV_STAGES], bar_s[2], bar_p[2][2], bar_o[2], bar_end;
   __shared__ uint32_t tmem_base;
   __shared__ int item_seq, item_pair;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
 
   // ---- which sequence, key head and pair of tiles
@@ -297,8 +292,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       for (int i = 0; i < KV_STAGES; ++i) mbar_init(smem_u32(&bar_full[i]), 1), mbar_init(smem_u32(&bar_empty[i]), 1);
       for (int x = 0; x < 2; ++x) {
         mbar_init(smem_u32(&bar_s[x]), 1);
-        mbar_init(smem_u32(&bar_p[x][0]), PT);
-        mbar_init(smem_u32(&bar_p[x][1]), PT);
+        mbar_init(smem_u32(&bar_p[x][0]), 4);
+        mbar_init(smem_u32(&bar_p[x][1]), 4);
         mbar_init(smem_u32(&bar_o[x]), 1);
       }
       mbar_init(smem_u32(&bar_end), 1);
@@ -318,7 +313,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 8) {
-      if (lane == 0 && n > 0) {
+      if (n > 0 && elect_one()) {
         const uint32_t bq = smem_u32(&bar_q);
         mbar_expect_tx(bq, (nblk[0] > 0 ? TILE_BYTES : 0) + (nblk[1] > 0 ? TILE_BYTES : 0));
         for (int x = 0; x < 2; ++x)
@@ -344,7 +339,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           for (int j = max(0, i - KV_STAGES); j < i; ++j) mbar_wait(smem_u32(&bar_full[j % KV_STAGES]), (j / KV_STAGES) & 1);
       }
     } else if (warp == 9) {
-      if (lane == 0 && n > 0) {
+      if (n > 0 && elect_one()) {
         constexpr uint32_t ID_S = umma_idesc(BF16, PT, PT, false), ID_O = umma_idesc(BF16, PT, HD, true);
         bool ok = true;
         auto wait = [&](uint64_t &bar, int phase) {
@@ -434,54 +429,74 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       const bool masked = (j0 + j + 1) * PT > all;
       const int seen = limit - (j0 + j) * PT;
       float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if (half == 1) tmem_wait_ld();
-        if (masked) {
-#pragma unroll
-          for (int i = 64 * half; i < 64 * half + 64; ++i) v[i] = i < seen ? v[i] : -INFINITY;
-        }
+      uint32_t w[32];
+      uint64_t sum = 0;
+      bool settled = false;
+      auto announce = [&](int half) {
+        tmem_st32(ts + 32 * half, w);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_p[x][half]));      // one arrival a warp: arrivals at one address queue up
+      };
+      auto largest = [&](int half) {
 #pragma unroll
         for (int i = 64 * half; i < 64 * half + 64; i += 8) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) t[e] = max3(t[e], v[i + 2 * e], v[i + 2 * e + 1]);
         }
-      }
-      const float top = max3(max3(t[0], t[1], t[2]), t[3], t[3]);
-      const bool grow = (top - m) * a.c > LAG || m == -INFINITY;
-      if (j == 0) {
-        m = top;
-      } else if (__any_sync(0xffffffffu, grow)) {
-        const float mn = grow ? fmaxf(m, top) : m;
-        const float f = grow ? ex2((m - (mn == -INFINITY ? 0.0f : mn)) * a.c) : 1.0f;
-        m = mn;
-        l *= f;
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          float o[32];
-          tmem_ld32(to + 32 * i, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= f;
-          tmem_st32(to + 32 * i, reinterpret_cast<const uint32_t *>(o));
+      };
+      if (j > 0 && !masked) {
+        // The maximum so far is mostly the one to use: the first weights are taken with it while the tile's own maximum
+        // is found, and count if no row has outgrown it (nor met a NaN, which this comparison does not pass).
+        const uint64_t nmc2 = pk2(-m * a.c, -m * a.c);
+        sum = weights64<T, true>(v, c2, nmc2, w);
+        largest(0);
+        tmem_wait_ld();
+        largest(1);
+        const float top = max3(max3(t[0], t[1], t[2]), t[3], t[3]);
+        settled = __all_sync(0xffffffffu, (top - m) * a.c <= LAG);
+        if (settled) {
+          announce(0);
+          sum = add2(sum, weights64<T, true>(v + 64, c2, nmc2, w));
+          announce(1);
         }
       }
-      const float mc = m == -INFINITY ? 0.0f : m * a.c;
-      const uint64_t nmc2 = pk2(-mc, -mc);
-      // the polynomial is for finite logits: a tile with masked ones, or a row that met an infinity or NaN, goes through
-      // the exponential unit alone
-      uint64_t sum;
-      const bool plain = masked || __any_sync(0xffffffffu, !(fabsf(top) < INFINITY));
-      if (plain) sum = weights64<T, false>(v, c2, nmc2, ts);
-      else sum = weights64<T, true>(v, c2, nmc2, ts);
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(smem_u32(&bar_p[x][0]));
-      if (plain) sum = add2(sum, weights64<T, false>(v + 64, c2, nmc2, ts + 32));
-      else sum = add2(sum, weights64<T, true>(v + 64, c2, nmc2, ts + 32));
-      tmem_wait_st();
-      tc_fence_before();
-      mbar_arrive(smem_u32(&bar_p[x][1]));
+      if (!settled) {
+        tmem_wait_ld();
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < PT; ++i) v[i] = i < seen ? v[i] : -INFINITY;
+        }
+        t[0] = t[1] = t[2] = t[3] = -INFINITY;
+        largest(0);
+        largest(1);
+        const float top = max3(max3(t[0], t[1], t[2]), t[3], t[3]);
+        const bool grow = (top - m) * a.c > LAG || m == -INFINITY;
+        if (j == 0) {
+          m = top;
+        } else if (__any_sync(0xffffffffu, grow)) {
+          const float mn = grow ? fmaxf(m, top) : m;
+          const float f = grow ? ex2((m - (mn == -INFINITY ? 0.0f : mn)) * a.c) : 1.0f;
+          m = mn;
+          l *= f;
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+            float o[32];
+            tmem_ld32(to + 32 * i, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= f;
+            tmem_st32(to + 32 * i, reinterpret_cast<const uint32_t *>(o));
+          }
+        }
+        const float mc = m == -INFINITY ? 0.0f : m * a.c;
+        const uint64_t nmc2 = pk2(-mc, -mc);
+        sum = weights64<T, false>(v, c2, nmc2, w);
+        announce(0);
+        sum = add2(sum, weights64<T, false>(v + 64, c2, nmc2, w));
+        announce(1);
+      }
       const float2 sf = un2(sum);
       l += sf.x + sf.y;
     }
