@@ -267,23 +267,21 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     s.out0 = s.q0;
   }
   const int tiles = (s.rows + PT - 1) / PT * a.G;           // (row tile, head) pairs of the key head
-  int row0[2], head[2], nblk[2];
-  bool live[2];
-#pragma unroll
-  for (int x = 0; x < 2; ++x) {
+  // row tile, head and key tiles of the block's query tile x
+  auto tile = [&](int x, int &row0, int &head) {
     const int f = 2 * pair + x;
-    live[x] = f < tiles;
-    row0[x] = f / a.G * PT;
-    head[x] = h * a.G + f % a.G;
-    const int last = min(row0[x] + PT, s.nq) - 1;
-    nblk[x] = live[x] && last >= row0[x] ? (key_limit(s, last, a.causal) + PT - 1) / PT : 0;
-  }
+    row0 = f / a.G * PT;
+    head = h * a.G + f % a.G;
+    const int last = min(row0 + PT, s.nq) - 1;
+    return f < tiles && last >= row0 ? (key_limit(s, last, a.causal) + PT - 1) / PT : 0;
+  };
+  int r_, h_;
+  const int all0 = tile(0, r_, h_), all1 = tile(1, r_, h_);
   // this block's key tiles: all of them, or the z-th part
-  const int most = max(nblk[0], nblk[1]);
+  const int most = max(all0, all1);
   const int j0 = static_cast<int>(static_cast<int64_t>(most) * z / a.splits);
   const int n = static_cast<int>(static_cast<int64_t>(most) * (z + 1) / a.splits) - j0;
-#pragma unroll
-  for (int x = 0; x < 2; ++x) nblk[x] = min(max(nblk[x] - j0, 0), n);
+  const int nb0 = min(max(all0 - j0, 0), n), nb1 = min(max(all1 - j0, 0), n);
 
   if (n > 0) {
     if (warp == 9) tmem_alloc(smem_u32(&tmem_base), 512);
@@ -309,22 +307,25 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
     if (a.status != nullptr) atomicExch(a.status, 1);
   };
 
-  // 384 threads start with 168 registers; the softmax threads take what the other group gives up (2 * 232 + 40 = 3 * 168)
+  // 384 threads start with 168 registers; the softmax threads take what the other group gives up (2 * 224 + 56 = 3 * 168)
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 8) {
       if (n > 0 && elect_one()) {
         const uint32_t bq = smem_u32(&bar_q);
-        mbar_expect_tx(bq, (nblk[0] > 0 ? TILE_BYTES : 0) + (nblk[1] > 0 ? TILE_BYTES : 0));
-        for (int x = 0; x < 2; ++x)
-          if (nblk[x] > 0)
+        mbar_expect_tx(bq, (nb0 > 0 ? TILE_BYTES : 0) + (nb1 > 0 ? TILE_BYTES : 0));
+        for (int x = 0; x < 2; ++x) {
+          int row0, head;
+          tile(x, row0, head);
+          if ((x ? nb1 : nb0) > 0)
             for (int c = 0; c < 2; ++c)
-              tma_load_4d(q_addr + x * TILE_BYTES + c * (TILE_BYTES / 2), &mq, bq, 64 * c, s.q0 + row0[x], head[x], s.b);
+              tma_load_4d(q_addr + x * TILE_BYTES + c * (TILE_BYTES / 2), &mq, bq, 64 * c, s.q0 + row0, head, s.b);
+        }
         int i = 0;
         bool ok = true;
         for (; i < 2 * n; ++i) {
           const int st = i % KV_STAGES, round = i / KV_STAGES;
-          if (round > 0 && !mbar_wait(smem_u32(&bar_empty[st]), (round - 1) & 1)) {
+          if (round > 0 && !mbar_wait_asleep(smem_u32(&bar_empty[st]), (round - 1) & 1)) {
             give_up();
             ok = false;
             break;
@@ -336,88 +337,107 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             tma_load_4d(kv_addr + st * TILE_BYTES + c * (TILE_BYTES / 2), m, bf, 64 * c, s.k0 + (j0 + (i >> 1)) * PT, h, s.b);
         }
         if (!ok)                                              // leave no copy in flight behind
-          for (int j = max(0, i - KV_STAGES); j < i; ++j) mbar_wait(smem_u32(&bar_full[j % KV_STAGES]), (j / KV_STAGES) & 1);
+          for (int j = max(0, i - KV_STAGES); j < i; ++j) mbar_wait_asleep(smem_u32(&bar_full[j % KV_STAGES]), (j / KV_STAGES) & 1);
       }
     } else if (warp == 9) {
       if (n > 0 && elect_one()) {
+        // This thread's instructions are the pace of the block: a straight line of them would miss the instruction cache at
+        // every step (the softmax code fills it), so everything is in short loops.
         constexpr uint32_t ID_S = umma_idesc(BF16, PT, PT, false), ID_O = umma_idesc(BF16, PT, HD, true);
+        constexpr uint32_t STAGE = TILE_BYTES >> 4;             // in units of a descriptor's address
+        const uint32_t full = smem_u32(&bar_full[0]), empty = smem_u32(&bar_empty[0]);
+        const uint32_t ready = smem_u32(&bar_s[0]), weights = smem_u32(&bar_p[0][0]), done = smem_u32(&bar_o[0]);
+        const uint32_t q_lo = umma_lo(q_addr, 16), k_lo = umma_lo(kv_addr, 16), v_lo = umma_lo(kv_addr, TILE_BYTES / 2);
+        uint32_t st = 0, ph = 0;                                // ring position of the next tile
         bool ok = true;
-        auto wait = [&](uint64_t &bar, int phase) {
-          if (ok && !mbar_wait(smem_u32(&bar), phase & 1)) {
-            ok = false;
-            give_up();
-          }
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+          ok = ok && mbar_wait_asleep(bar, parity);
           tc_fence_after();
           return ok;
         };
-        // logits of tile x against key tile j: contraction over 128 channels, 16 at a time, two swizzled halves
-        auto logits = [&](int x, int j) {
-          const uint32_t qa = umma_lo(q_addr + x * TILE_BYTES, 16);
-          const uint32_t ka = umma_lo(kv_addr + (2 * j % KV_STAGES) * TILE_BYTES, 16);
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            const uint32_t off = ((kk >> 2) * (TILE_BYTES / 2) + (kk & 3) * 32) >> 4;
-            umma_ss(tmem + x * PT, qa + off, umma_hi(1024), ka + off, umma_hi(1024), ID_S, kk > 0);
-          }
-          umma_commit(smem_u32(&bar_s[x]));
+        auto advance = [&] {
+          if (++st == KV_STAGES) st = 0, ph ^= 1;
         };
-        // accumulator of tile x += weights x value tile j: contraction over 128 keys, 16 at a time
-        auto values = [&](int x, int j) {
-          const uint32_t va = umma_lo(kv_addr + ((2 * j + 1) % KV_STAGES) * TILE_BYTES, TILE_BYTES / 2);
+        // logits of tile x: contraction over 128 channels, 16 at a time, two swizzled halves
+        auto logits = [&](uint32_t x, uint32_t stage) {
+          uint32_t ql = q_lo + x * STAGE, kl = k_lo + stage * STAGE;
+#pragma unroll 1
+          for (int c = 0; c < 2; ++c) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if (!wait(bar_p[x][half], j)) return;
-#pragma unroll
-            for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-              umma_ts(tmem + 2 * PT + x * HD, tmem + x * PT + kk * 8, va + (kk * 2048 >> 4), umma_hi(1024), ID_O, j > 0 || kk > 0);
+            for (int k = 0; k < 4; ++k)
+              umma_ss(tmem + x * PT, ql + 2 * k, umma_hi(1024), kl + 2 * k, umma_hi(1024), ID_S, (c | k) != 0);
+            ql += STAGE / 2;
+            kl += STAGE / 2;
           }
-          if (j + 1 == (x ? nblk[1] : nblk[0])) umma_commit(smem_u32(&bar_o[x]));
+          umma_commit(ready + 8 * x);
         };
-        wait(bar_q, 0);
-        if (wait(bar_full[0], 0)) {
+        wait(smem_u32(&bar_q), 0);
+        if (wait(full, 0)) {
 #pragma unroll 1
           for (int x = 0; x < 2; ++x)
-            if ((x ? nblk[1] : nblk[0]) > 0) logits(x, 0);
-          umma_commit(smem_u32(&bar_empty[0]));
+            if ((x ? nb1 : nb0) > 0) logits(x, 0);
+          umma_commit(empty);
+          advance();
         }
+#pragma unroll 1
         for (int j = 0; j < n && ok; ++j) {
-          const int sv = (2 * j + 1) % KV_STAGES, sk = (2 * j + 2) % KV_STAGES;
-          if (!wait(bar_full[sv], (2 * j + 1) / KV_STAGES)) break;
+          const uint32_t sv = st;
+          if (!wait(full + 8 * sv, ph)) break;
+          advance();
+          const bool more = j + 1 < n;
 #pragma unroll 1
           for (int x = 0; x < 2 && ok; ++x) {
-            const int nb = x ? nblk[1] : nblk[0];
+            const int nb = x ? nb1 : nb0;
             if (j < nb) {
-              values(x, j);
+              // accumulator of tile x += weights x value tile j: contraction over 128 keys, 16 at a time
+              uint32_t vl = v_lo + sv * STAGE, pa = tmem + x * PT;
+              uint32_t bar = weights + 16 * x;
+#pragma unroll 1
+              for (int c = 0; c < 2; ++c) {
+                if (!wait(bar, j & 1)) break;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  umma_ts(tmem + 2 * PT + x * HD, pa + 8 * k, vl + (2048 >> 4) * k, umma_hi(1024), ID_O, (j | c | k) != 0);
+                vl += 4 * (2048 >> 4);
+                pa += 32;
+                bar += 8;
+              }
               if (!ok) break;
+              if (j + 1 == nb) umma_commit(done + 8 * x);
             }
-            if (x == 1) umma_commit(smem_u32(&bar_empty[sv]));
-            if (j + 1 < n) {
-              if (x == 0 && !wait(bar_full[sk], (2 * j + 2) / KV_STAGES)) break;
-              if (j + 1 < nb) logits(x, j + 1);
-              if (x == 1) umma_commit(smem_u32(&bar_empty[sk]));
+            if (x == 1) umma_commit(empty + 8 * sv);
+            if (more) {
+              if (x == 0 && !wait(full + 8 * st, ph)) break;
+              if (j + 1 < nb) logits(x, st);
+              if (x == 1) umma_commit(empty + 8 * st);
             }
           }
+          if (more) advance();
         }
+        if (!ok) give_up();
         // every product is complete before the tensor memory is given back
         umma_commit(smem_u32(&bar_end));
-        mbar_wait(smem_u32(&bar_end), 0);
+        mbar_wait_asleep(smem_u32(&bar_end), 0);
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int x = warp >> 2;
     const uint32_t at = tmem + (static_cast<uint32_t>(warp & 3) << 21);     // the warp's 32 lanes
     const uint32_t ts = at + x * PT, to = at + 2 * PT + x * HD;
-    const int row = row0[x] + (threadIdx.x & 127);
+    int row0, head;
+    tile(x, row0, head);
+    const bool live = 2 * pair + x < tiles;
+    const int row = row0 + (threadIdx.x & 127);
     const int limit = key_limit(s, row, a.causal);
-    const int nb = nblk[x];
+    const int nb = x ? nb1 : nb0;
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     // keys that every row of the tile sees need no comparison
-    const int all = key_limit(s, min(row0[x], s.nq - 1), a.causal);
+    const int all = key_limit(s, min(row0, s.nq - 1), a.causal);
     const uint64_t c2 = pk2(a.c, a.c);
     for (int j = 0; j < nb; ++j) {
-      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_s[x]), j & 1));
+      ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_s[x]), j & 1));
       if (!ok) break;
       tc_fence_after();
       float v[PT];
@@ -500,12 +520,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       const float2 sf = un2(sum);
       l += sf.x + sf.y;
     }
-    if (nb > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar_o[x]), 0));
+    if (nb > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_o[x]), 0));
     if (!ok) give_up();
-    if (live[x] && ok) {
+    if (live && ok) {
       tc_fence_after();
       const bool mine = row < s.rows;
-      const int64_t at_out = (s.out0 + row) * static_cast<int64_t>(a.G) * a.h_kv + head[x];
+      const int64_t at_out = (s.out0 + row) * static_cast<int64_t>(a.G) * a.h_kv + head;
       bool odd = false;
       if (a.splits == 1) {
         const float inv = limit > 0 ? 1.0f / l : 0.0f;
@@ -556,7 +576,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         const int r = __ffs(again) - 1;
         again &= again - 1;
         const int hi = min((j0 + nb) * PT, a.Lk - s.k0);
-        repair_row<T>(a, s, __shfl_sync(0xffffffffu, row, r), head[x], __shfl_sync(0xffffffffu, limit, r), j0 * PT, hi, z);
+        repair_row<T>(a, s, __shfl_sync(0xffffffffu, row, r), head, __shfl_sync(0xffffffffu, limit, r), j0 * PT, hi, z);
       }
     }
     tc_fence_before();
