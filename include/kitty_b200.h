@@ -402,7 +402,7 @@ int kitty_prompt_attn(const void *q, const void *k, const void *v, int dtype, co
  * tokens were cut into calls.  The caller keeps the lengths; every call takes them as a device array, so the calls can
  * be captured in a CUDA graph and replayed.
  *
- * Block record (8208 bytes, byte = code + 128): 4096 B keys | 4096 B values | key scale, value scale (fp32) | 8 B.
+ * Block record (8208 bytes, a code per byte): 4096 B keys | 4096 B values | key scale, value scale (fp32) | 8 B.
  * Keys: 16-byte piece (i, half, lane = 4g + t) = channels 64*half + 16t ... + 15 of token 8*(g/2) + 2i + g%2.
  * Values: piece (x, lane) = channel 16x + g, tokens 8t ... 8t+7, then channel 16x + 8 + g, the same tokens: the order
  * in which the attention kernel's lanes hold them as matrix operands. */

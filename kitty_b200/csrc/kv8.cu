@@ -28,11 +28,11 @@ __device__ __forceinline__ void half_barrier(int half) {
   asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
 }
 
-// Four floats -> four biased codes in one word.
+// Four floats -> four codes (two's complement bytes) in one word.
 __device__ __forceinline__ uint32_t kv8_codes4(const float *x, float inv) {
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(__fadd_rd(fmaf(x[i], inv, 0.5f), 12582912.0f + 128.0f));
+  for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(__fadd_rd(fmaf(x[i], inv, 0.5f), 12582912.0f));
   return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
 }
 
@@ -282,7 +282,7 @@ __device__ __forceinline__ void expand16(uint4 codes, float scale, uint4 (&out)[
     Piece<T> p;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      p.f[e] = static_cast<float>(static_cast<int>((w[2 * c + (e >> 2)] >> (8 * (e & 3))) & 0xffu) - 128) * scale;
+      p.f[e] = static_cast<float>(static_cast<int8_t>(w[2 * c + (e >> 2)] >> (8 * (e & 3)))) * scale;
     out[c] = p.pack();
   }
 }

@@ -7,22 +7,29 @@
 // records in flight with bulk copies (one 8208-byte copy per unit) and needs no other warp until the end.  A row that
 // several warps share is joined by a second kernel from their (accumulator, maximum, sum) partials, in a fixed order.
 //
-// Arithmetic of a unit: 16 matrix rows = query heads, contraction over 16 channels or 16 tokens at a time
-// (mma.m16n8k16, fp16 operands, 32-bit sums).  A code byte becomes the fp16 number 1024 + byte by placing it in the low
-// mantissa bits; subtracting 1152 leaves the whole number exactly.  Records hold the bytes in operand order, so every
-// shared-memory read is one conflict-free 16-byte word per lane, and no transposing step is needed anywhere.  The key
-// scale multiplies the block's logits, the value scale the block's products, both in 32 bits.
-// The tensor units need neither tcgen05 nor shared-memory operands here: 16 of 128 tile rows would be used, and the
-// operands are made in registers.
+// Arithmetic of a unit: whole-number matrix products (mma.m16n8k32, 8-bit operands, exact 32-bit sums) on the stored
+// bytes as they are; records hold them in operand order, so every shared-memory read is one conflict-free 16-byte word
+// per lane.  The other operand is a 16-bit fixed-point number in two bytes, 256 hi + lo, which are two of the tile's
+// sixteen rows (eight heads):
+//   logits   query elements in units of (largest of the head) / 32512: off by at most 2^-16 of the head's largest
+//   weights  in units of (largest of the block's 32 tokens) / 32512: off by at most 2^-16 of that one, so a far larger
+//            weight elsewhere in the sequence costs nothing
+// Scales, exponentials, sums and accumulators are 32-bit floats.  Conversions of the codes to 16-bit floats, which an
+// fp16 product needs, cost twice the instructions in all and held the kernel at 79 % of the copy bandwidth.
+// tcgen05 has no use here: 16 of 128 tile rows would be filled.
 #include "kv8.cuh"
 #include "paged_core.cuh"
 
 namespace kitty {
 
-constexpr int KV8_WARPS = 8;            // per block of threads, one block per multiprocessor
-constexpr int KV8_STAGES = 3;
+#ifndef KV8_WARPS
+constexpr int KV8_WARPS = 12;           // per block of threads, one block per multiprocessor
+constexpr int KV8_STAGES = 2;
+#endif
 constexpr int KV8_MAX_SMS = 160;        // the workspace is sized for this many
 constexpr int KV8_WORKERS_MAX = KV8_MAX_SMS * KV8_WARPS;
+constexpr float KV8_FIX = 32512.0f;     // 127 * 256: both bytes of a fixed-point number stay in -128 .. 127
+constexpr float KV8_MAGIC = 12582912.0f;   // 1.5 * 2^23: x + this has the whole number x in its low bits
 
 struct Kv8AttnArgs {
   kitty_kv8_layer L;
@@ -35,24 +42,36 @@ struct Kv8AttnArgs {
   int32_t B, G, workers;
 };
 
-__device__ __forceinline__ int64_t kv8_first_unit(int64_t w, int64_t units, int64_t workers) { return w * units / workers; }
-__device__ __forceinline__ int64_t kv8_worker_of(int64_t u, int64_t units, int64_t workers) {
-  return ((u + 1) * workers - 1) / units;
+// Worker w takes units kv8_first_unit(w) .. kv8_first_unit(w + 1) - 1: a part each, the first units % workers one more.
+__device__ __forceinline__ int kv8_first_unit(int w, int units, int workers) {
+  return w * (units / workers) + min(w, units % workers);
+}
+__device__ __forceinline__ int kv8_worker_of(int u, int units, int workers) {
+  const int q = units / workers, r = units % workers;
+  return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q;
 }
 
-// Two code bytes of a word (sel 0x4140: bytes 0, 1; 0x4342: bytes 2, 3) as exact fp16 whole numbers.
-template <uint32_t SEL>
-__device__ __forceinline__ uint32_t code2(uint32_t w) {
-  const uint32_t r = __byte_perm(w, 0x64646464u, SEL);
-  const __half2 d = __hsub2(*reinterpret_cast<const __half2 *>(&r), __float2half2_rn(1152.0f));
-  return *reinterpret_cast<const uint32_t *>(&d);
-}
-
-__device__ __forceinline__ void mma16816_zero(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void imma(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Four fixed-point numbers (in the low bits of the words) -> their high and low bytes.
+__device__ __forceinline__ void fix_bytes(const float *x, uint32_t &hi, uint32_t &lo) {
+  uint32_t v[4], y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[e] = __float_as_uint(x[e]);
+    y[e] = v[e] + 128u;
+  }
+  lo = __byte_perm(__byte_perm(v[0], v[1], 0x0040), __byte_perm(v[2], v[3], 0x0040), 0x5410);
+  hi = __byte_perm(__byte_perm(y[0], y[1], 0x0051), __byte_perm(y[2], y[3], 0x0051), 0x5410);
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
 }
 template <typename T>
 __device__ __forceinline__ void mma_t(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -77,50 +96,47 @@ __device__ __forceinline__ uint32_t pack_t(float lo, float hi) {
 // Place of a unit: sequence, key head, block, the number of units of the sequence's rows and the tokens it holds.
 struct Kv8Cursor {
   int b, h, blk, nblk, len;
-  const int32_t *lengths;
-  int cap;
-  __device__ __forceinline__ void enter(const int32_t *prefix) {
+  __device__ __forceinline__ void enter(const Kv8AttnArgs &a, const int32_t *prefix) {
     nblk = prefix[b + 1] - prefix[b];
-    len = max(0, min(lengths[b], cap));
+    len = max(0, min(a.lengths[b], a.L.max_page * PAGE));
   }
   __device__ __forceinline__ int tokens() const { return min(KV8_BLOCK, len - blk * KV8_BLOCK); }
-  __device__ __forceinline__ void seek(int64_t u, const int32_t *prefix, int B, int H) {
-    // prefix[b] * H <= u < prefix[b + 1] * H
-    int lo = 0, hi = B;
+  __device__ __forceinline__ void seek(int u, const Kv8AttnArgs &a, const int32_t *prefix) {
+    // prefix[b] * h_kv <= u < prefix[b + 1] * h_kv
+    int lo = 0, hi = a.B;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (static_cast<int64_t>(prefix[mid]) * H <= u) lo = mid;
+      if (prefix[mid] * a.L.h_kv <= u) lo = mid;
       else hi = mid;
     }
     b = lo;
-    enter(prefix);
-    const int64_t rest = u - static_cast<int64_t>(prefix[b]) * H;
-    h = static_cast<int>(rest / nblk);
-    blk = static_cast<int>(rest % nblk);
+    enter(a, prefix);
+    const int rest = u - prefix[b] * a.L.h_kv;
+    h = rest / nblk;
+    blk = rest - h * nblk;
   }
   // true when the next unit belongs to another row
-  __device__ __forceinline__ bool next(const int32_t *prefix, int B, int H) {
+  __device__ __forceinline__ bool next(const Kv8AttnArgs &a, const int32_t *prefix) {
     if (++blk < nblk) return false;
     blk = 0;
-    if (++h == H) {
+    if (++h == a.L.h_kv) {
       h = 0;
       do {
         ++b;
-      } while (b < B && prefix[b + 1] == prefix[b]);
-      if (b < B) enter(prefix);
+      } while (b < a.B && prefix[b + 1] == prefix[b]);
+      if (b < a.B) enter(a, prefix);
     }
     return true;
   }
 };
 
-// MT: 1 for groups of up to 8 query heads (matrix rows 8..15 idle), 2 for up to 16.
+// MT: 1 for groups of up to 8 query heads, 2 for up to 16 (two matrix tiles).
 template <typename T, int MT>
 __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[KV8_WARPS][KV8_STAGES];
   __shared__ int32_t scan[KV8_WARPS];
   __shared__ int32_t skipped[KV8_WARPS][KV8_STAGES];      // stages without a record
-  uint8_t *ring_all = smem;
   int32_t *prefix = reinterpret_cast<int32_t *>(smem + KV8_WARPS * KV8_STAGES * KV8_REC);
   const kitty_kv8_layer &L = a.L;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -130,7 +146,6 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __gri
     for (int s = 0; s < KV8_STAGES; ++s) mbar_init(smem_u32(&bars[warp][s]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  dep_wait();
   // units before each sequence: every block of threads scans the lengths
   {
     const int per = (B + KV8_WARPS * 32 - 1) / (KV8_WARPS * 32), i0 = min(B, per * static_cast<int>(threadIdx.x));
@@ -158,48 +173,57 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __gri
       for (int i = threadIdx.x; i <= B; i += KV8_WARPS * 32) a.prefix[i] = prefix[i];
   }
   dep_release();
-  const int64_t units = static_cast<int64_t>(prefix[B]) * H;
-  const int64_t worker = static_cast<int64_t>(blockIdx.x) * KV8_WARPS + warp;
+  const int units = prefix[B] * H;
+  // neighbouring workers sit on different multiprocessors, so that a few units spread over all of them
+  const int worker = warp * gridDim.x + blockIdx.x;
   if (units == 0) return;
-  const int64_t u0 = kv8_first_unit(worker, units, a.workers), u1 = kv8_first_unit(worker + 1, units, a.workers);
+  const int u0 = kv8_first_unit(worker, units, a.workers), u1 = kv8_first_unit(worker + 1, units, a.workers);
   if (u0 >= u1) return;
 
-  const uint32_t ring = smem_u32(ring_all) + warp * KV8_STAGES * KV8_REC;
-  const uint8_t *ring_p = ring_all + warp * KV8_STAGES * KV8_REC;
-  // request the record of a unit; an open block has none (its 16-bit tokens are read when their turn comes)
-  auto request = [&](const Kv8Cursor &c, int stage) {
+  const uint8_t *ring_p = smem + warp * KV8_STAGES * KV8_REC;
+  const uint32_t ring = smem_u32(ring_p);
+  Kv8Cursor cur, ahead;
+  cur.seek(u0, a, prefix);
+  ahead = cur;
+  int ua = u0;
+  int64_t page = 0;                        // page row of the unit that is requested next, looked up a unit early
+  auto look_up = [&] {
+    if (lane == 0 && ua < u1 && ahead.tokens() == KV8_BLOCK) page = kv8_page(L, ahead.b, ahead.blk);
+  };
+  // request the unit `ahead`: the record of a whole block, or the 16-bit values of an open one
+  auto request = [&](int stage) {
     if (lane == 0) {
       const uint32_t bar = smem_u32(&bars[warp][stage]);
-      const int64_t page = c.tokens() == KV8_BLOCK ? kv8_page(L, c.b, c.blk) : -1;
-      skipped[warp][stage] = page < 0;
-      if (page >= 0) {
+      const bool whole = ahead.tokens() == KV8_BLOCK;
+      skipped[warp][stage] = whole && page < 0;
+      if (!whole) {
+        constexpr uint32_t BYTES = KV8_BLOCK * HD * sizeof(T);
+        mbar_expect_tx(bar, BYTES);
+        bulk_g2s(ring + stage * KV8_REC, static_cast<const T *>(L.tail_v) + (static_cast<int64_t>(ahead.b) * H + ahead.h) * KV8_BLOCK * HD,
+                 BYTES, bar);
+      } else if (page >= 0) {
         mbar_expect_tx(bar, KV8_REC);
-        bulk_g2s(ring + stage * KV8_REC, kv8_record(L, page, c.h, c.blk & 3), KV8_REC, bar);
+        bulk_g2s(ring + stage * KV8_REC, kv8_record(L, page, ahead.h, ahead.blk & 3), KV8_REC, bar);
       } else {
         mbar_expect_tx(bar, 0);
       }
     }
+    ahead.next(a, prefix);
+    ++ua;
+    look_up();
   };
-  Kv8Cursor cur, ahead;
-  cur.lengths = a.lengths;
-  cur.cap = L.max_page * PAGE;
-  cur.seek(u0, prefix, B, H);
-  ahead = cur;
-  int64_t ua = u0;
+  look_up();
   for (int s = 0; s < KV8_STAGES; ++s)
-    if (ua < u1) {
-      request(ahead, s);
-      ahead.next(prefix, B, H);
-      ++ua;
-    }
+    if (ua < u1) request(s);
 
-  uint32_t qa[8][4];          // query heads as matrix rows g (and g + 8), fp16, scaled by a power of two
+  uint32_t qa[MT][4][4];      // [tile][32 channels][operand]: rows g = high bytes of head g (+ 8), rows g + 8 = low bytes
   float acc[16][2 * MT], mx[MT], sum[MT], qs[MT];
-  bool fresh = true;
+  bool fresh = true, from_start = false;
   int stage = 0, phase = 0;
-  for (int64_t u = u0; u < u1; ++u) {
+  for (int u = u0; u < u1; ++u) {
     if (fresh) {
       fresh = false;
+      from_start = cur.blk == 0;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const int head = g + 8 * m;
@@ -209,29 +233,35 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __gri
 #pragma unroll
           for (int c = 0; c < 4; ++c) w[c] = *reinterpret_cast<const uint4 *>(qp + (c >> 1) * 64 + (c & 1) * 8);
         }
-        // a power of two brings the row's largest element to [1, 2): bf16 values then fit fp16 exactly, except those
-        // 2^-14 and more below the largest, which lose low bits that are 2^-24 of it at most
-        float top = 0.0f;
-        float x[4][8];
+        float x[4][8], top = 0.0f;
+        bool odd = false;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           Vec8<T>::unpack(w[c], x[c]);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[c][e]));
+          for (int e = 0; e < 8; ++e) {
+            top = fmaxf(top, fabsf(x[c][e]));
+            odd |= !(fabsf(x[c][e]) < INFINITY);
+          }
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        odd = (__ballot_sync(0xffffffffu, odd) >> (lane & 28) & 15u) != 0;
+        // the largest element is brought to [1, 2) by a power of two first, which keeps its reciprocal in range
         int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
         ex = max(-100, min(100, ex));
         const float down = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
-        qs[m] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);
+        const float inv = top > 0.0f && !odd ? KV8_FIX / (top * down) * down : 0.0f;
+        qs[m] = odd ? __uint_as_float(0x7fc00000u) : a.scale_log2 * (top / KV8_FIX);
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          const float *z = &x[ks >> 1][(ks & 1) * 4];
-          qa[ks][m] = pack_h2(z[0] * down, z[1] * down);
-          qa[ks][2 + m] = pack_h2(z[2] * down, z[3] * down);
-          if (MT == 1) qa[ks][1] = qa[ks][3] = 0;
-        }
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {
+            float z[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z[e] = fmaf(x[ks][4 * o + e], inv, KV8_MAGIC);
+            fix_bytes(z, qa[m][ks][2 * o], qa[m][ks][2 * o + 1]);
+          }
         mx[m] = -INFINITY;
         sum[m] = 0.0f;
       }
@@ -241,59 +271,56 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __gri
         for (int e = 0; e < 2 * MT; ++e) acc[n][e] = 0.0f;
     }
     const int cnt = cur.tokens();
-    const uint32_t bar = smem_u32(&bars[warp][stage]);
-    if (!mbar_wait(bar, phase)) {
+    const bool packed = cnt == KV8_BLOCK;
+    if (!mbar_wait(smem_u32(&bars[warp][stage]), phase)) {
       if (lane == 0) atomicOr(L.status, KITTY_KV8_TIMEOUT);
-      for (int64_t v = u; v < ua; ++v) {          // leave no copy of this warp in flight behind
+      for (int v = u; v < ua; ++v) {          // leave no copy of this warp in flight behind
         mbar_wait(smem_u32(&bars[warp][stage]), phase);
         if (++stage == KV8_STAGES) stage = 0, phase ^= 1;
       }
       return;
     }
-    float p[4][2 * MT];           // logits, then weights: tile i, columns 2t, 2t+1 of rows g (and g + 8)
     const uint8_t *rec = ring_p + stage * KV8_REC;
-    const bool packed = cnt == KV8_BLOCK;
-    const bool valid = !packed || skipped[warp][stage] == 0;
+    float p[4][2 * MT];           // logits, then weights: tile i, columns 2t, 2t+1 of head g (and g + 8)
     float vscale = 1.0f;
     if (packed) {
       const float2 sc = *reinterpret_cast<const float2 *>(rec + KV8_OFF_SCALE);
       vscale = sc.y;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float c[4];
+        int c[MT][4] = {};
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          const uint4 w4 = *reinterpret_cast<const uint4 *>(rec + i * 1024 + hf * 512 + lane * 16);
-          const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+          const uint4 w = *reinterpret_cast<const uint4 *>(rec + i * 1024 + hf * 512 + lane * 16);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t b0 = code2<0x4140>(w[j]), b1 = code2<0x4342>(w[j]);
-            if (hf == 0 && j == 0) mma16816_zero(c, qa[0], b0, b1);
-            else mma16816(c, qa[4 * hf + j][0], qa[4 * hf + j][1], qa[4 * hf + j][2], qa[4 * hf + j][3], b0, b1);
+          for (int m = 0; m < MT; ++m) {
+            imma(c[m], qa[m][2 * hf], w.x, w.y);
+            imma(c[m], qa[m][2 * hf + 1], w.z, w.w);
           }
         }
 #pragma unroll
-        for (int e = 0; e < 2 * MT; ++e) p[i][e] = c[e] * (sc.x * qs[e >> 1]);
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) p[i][2 * m + e] = static_cast<float>(c[m][e] * 256 + c[m][2 + e]) * (sc.x * qs[m]);
       }
     } else {
       // open block: 16-bit keys straight from memory, the query in its own type
-      const int64_t at = ((static_cast<int64_t>(cur.b) * H + cur.h) * KV8_BLOCK) * HD;
-      const T *kt = static_cast<const T *>(L.tail_k) + at;
+      const T *kt = static_cast<const T *>(L.tail_k) + (static_cast<int64_t>(cur.b) * H + cur.h) * KV8_BLOCK * HD + 16 * t;
       const T *qp = static_cast<const T *>(a.q) + (static_cast<int64_t>(cur.b) * H * G + cur.h * G) * HD + 16 * t;
       float c[4][4] = {};
 #pragma unroll
       for (int ch = 0; ch < 4; ++ch) {
         const int off = (ch >> 1) * 64 + (ch & 1) * 8;
-        uint4 q0 = {}, q1 = {};
+        uint4 q0 = {}, q1 = {}, k4[4] = {};
         if (g < G) q0 = *reinterpret_cast<const uint4 *>(qp + g * HD + off);
         if (MT == 2 && g + 8 < G) q1 = *reinterpret_cast<const uint4 *>(qp + (g + 8) * HD + off);
 #pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (kv8_key_token(i, g) < cnt) k4[i] = *reinterpret_cast<const uint4 *>(kt + kv8_key_token(i, g) * HD + off);
+#pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int tk = kv8_key_token(i, g);
-          uint4 k4 = {};
-          if (tk < cnt) k4 = *reinterpret_cast<const uint4 *>(kt + tk * HD + 16 * t + off);
-          mma_t<T>(c[i], q0.x, q1.x, q0.y, q1.y, k4.x, k4.y);
-          mma_t<T>(c[i], q0.z, q1.z, q0.w, q1.w, k4.z, k4.w);
+          mma_t<T>(c[i], q0.x, q1.x, q0.y, q1.y, k4[i].x, k4[i].y);
+          mma_t<T>(c[i], q0.z, q1.z, q0.w, q1.w, k4[i].z, k4[i].w);
         }
       }
 #pragma unroll
@@ -302,37 +329,37 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __gri
         for (int e = 0; e < 2 * MT; ++e)
           p[i][e] = 8 * t + 2 * i + (e & 1) < cnt ? c[i][e] * a.scale_log2 : -INFINITY;
     }
-    if (!valid) {
+    if (skipped[warp][stage]) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int e = 0; e < 2 * MT; ++e) p[i][e] = -INFINITY;
       vscale = 0.0f;
     }
-    // running maximum and sum (base 2)
-    float corr[MT];
+    // the block's own maximum and weights, and the running maximum and sum (base 2)
+    float corr[MT], part[MT];
+    bool moved = false;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      float top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(p[i][2 * m], p[i][2 * m + 1]));
+      float top = fmaxf(fmaxf(fmaxf(p[0][2 * m], p[0][2 * m + 1]), fmaxf(p[1][2 * m], p[1][2 * m + 1])),
+                        fmaxf(fmaxf(p[2][2 * m], p[2][2 * m + 1]), fmaxf(p[3][2 * m], p[3][2 * m + 1])));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float mn = fmaxf(mx[m], top);
-      const float ref = mn == -INFINITY ? 0.0f : mn;
+      const float own = top == -INFINITY ? 0.0f : top;
+      const float mn = fmaxf(mx[m], top), ref = mn == -INFINITY ? 0.0f : mn;
       corr[m] = ex2(mx[m] - ref);
+      part[m] = top == -INFINITY ? 0.0f : ex2(top - ref);
+      moved |= corr[m] != 1.0f;
       mx[m] = mn;
       float add = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[i][2 * m] = ex2(p[i][2 * m] - ref);
-        p[i][2 * m + 1] = ex2(p[i][2 * m + 1] - ref);
+        p[i][2 * m] = ex2(p[i][2 * m] - own);
+        p[i][2 * m + 1] = ex2(p[i][2 * m + 1] - own);
         add += p[i][2 * m] + p[i][2 * m + 1];
       }
-      sum[m] = sum[m] * corr[m] + add;
+      sum[m] = fmaf(sum[m], corr[m], add * part[m]);
     }
-    bool moved = corr[0] != 1.0f;
-    if (MT == 2) moved |= corr[MT - 1] != 1.0f;
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
       for (int n = 0; n < 16; ++n)
@@ -340,34 +367,41 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __gri
         for (int e = 0; e < 2 * MT; ++e) acc[n][e] *= corr[e >> 1];
     }
     if (packed) {
-      uint32_t pa[2][4];        // weights as matrix rows, 16 tokens each
+      uint32_t pa[MT][4];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        pa[s][0] = pack_h2(p[2 * s][0], p[2 * s][1]);
-        pa[s][2] = pack_h2(p[2 * s + 1][0], p[2 * s + 1][1]);
-        pa[s][1] = MT == 2 ? pack_h2(p[2 * s][2 * MT - 2], p[2 * s][2 * MT - 1]) : 0;
-        pa[s][3] = MT == 2 ? pack_h2(p[2 * s + 1][2 * MT - 2], p[2 * s + 1][2 * MT - 1]) : 0;
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          float z[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) z[e] = fmaf(p[2 * o + (e >> 1)][2 * m + (e & 1)], KV8_FIX, KV8_MAGIC);
+          fix_bytes(z, pa[m][2 * o], pa[m][2 * o + 1]);
+        }
+        part[m] *= vscale * (1.0f / KV8_FIX);
       }
 #pragma unroll
       for (int x = 0; x < 8; ++x) {
-        const uint4 w4 = *reinterpret_cast<const uint4 *>(rec + KV8_OFF_V + x * 512 + lane * 16);
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+        const uint4 w = *reinterpret_cast<const uint4 *>(rec + KV8_OFF_V + x * 512 + lane * 16);
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          float c[4];
-          mma16816_zero(c, pa[0], code2<0x4140>(w[2 * y]), code2<0x4342>(w[2 * y]));
-          mma16816(c, pa[1][0], pa[1][1], pa[1][2], pa[1][3], code2<0x4140>(w[2 * y + 1]), code2<0x4342>(w[2 * y + 1]));
+        for (int m = 0; m < MT; ++m) {
+          int c0[4] = {}, c1[4] = {};
+          imma(c0, pa[m], w.x, w.y);
+          imma(c1, pa[m], w.z, w.w);
 #pragma unroll
-          for (int e = 0; e < 2 * MT; ++e) acc[2 * x + y][e] = fmaf(vscale, c[e], acc[2 * x + y][e]);
+          for (int e = 0; e < 2; ++e) {
+            acc[2 * x][2 * m + e] = fmaf(static_cast<float>(c0[e] * 256 + c0[2 + e]), part[m], acc[2 * x][2 * m + e]);
+            acc[2 * x + 1][2 * m + e] = fmaf(static_cast<float>(c1[e] * 256 + c1[2 + e]), part[m], acc[2 * x + 1][2 * m + e]);
+          }
         }
       }
     } else {
-      // 16-bit values of the open block; weights as a sum of two 16-bit numbers, so that the bf16 form loses nothing
-      const int64_t at = ((static_cast<int64_t>(cur.b) * H + cur.h) * KV8_BLOCK) * HD;
-      const T *vp = static_cast<const T *>(L.tail_v) + at;
-      uint32_t hi[4][MT], lo[4][MT];
+      // 16-bit values of the open block, in the stage; weights as a sum of two 16-bit numbers, so that the bf16 form loses
+      // nothing; tokens behind the last one are nothing, whatever they hold
+      uint32_t hi[4][MT], lo[4][MT], keep[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i) {
+        const int tk = 8 * t + 2 * i;
+        keep[i] = (tk < cnt ? 0x0000ffffu : 0u) | (tk + 1 < cnt ? 0xffff0000u : 0u);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           const float p0 = p[i][2 * m], p1 = p[i][2 * m + 1];
@@ -375,18 +409,17 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __gri
           hi[i][m] = pack_t<T>(r0, r1);
           lo[i][m] = pack_t<T>(p0 - r0, p1 - r1);
         }
-#pragma unroll 4
+      }
+      // lane l names row l % 8 of matrix l / 8: the token that row 2t' + e of tile i stands for
+      const int mi = lane >> 3, mr = lane & 7;
+      const uint32_t row = ring + stage * KV8_REC + kv8_key_token(mi, mr) * HD * sizeof(T);
+#pragma unroll
       for (int n = 0; n < 16; ++n) {
         float c[4] = {};
         uint32_t bv[4];
+        ldmatrix4_trans(bv, row + n * 16);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tk = 8 * t + 2 * i;
-          uint16_t e0 = 0, e1 = 0;
-          if (tk < cnt) e0 = *reinterpret_cast<const uint16_t *>(vp + tk * HD + 8 * n + g);
-          if (tk + 1 < cnt) e1 = *reinterpret_cast<const uint16_t *>(vp + (tk + 1) * HD + 8 * n + g);
-          bv[i] = e0 | static_cast<uint32_t>(e1) << 16;
-        }
+        for (int i = 0; i < 4; ++i) bv[i] &= keep[i];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           mma_t<T>(c, hi[2 * s][0], MT == 2 ? hi[2 * s][MT - 1] : 0, hi[2 * s + 1][0], MT == 2 ? hi[2 * s + 1][MT - 1] : 0,
@@ -395,34 +428,33 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __gri
                    bv[2 * s], bv[2 * s + 1]);
         }
 #pragma unroll
-        for (int n2 = 0; n2 < 16; ++n2)
-          if (n2 == n) {
-#pragma unroll
-            for (int e = 0; e < 2 * MT; ++e) acc[n2][e] += c[e];
-          }
+        for (int e = 0; e < 2 * MT; ++e) acc[n][e] = fmaf(c[e], part[e >> 1], acc[n][e]);
       }
     }
     // the stage is read: request the unit that comes KV8_STAGES later into it
     __syncwarp();
-    if (ua < u1) {
-      request(ahead, stage);
-      ahead.next(prefix, B, H);
-      ++ua;
-    }
+    if (ua < u1) request(stage);
     if (++stage == KV8_STAGES) stage = 0, phase ^= 1;
-    const int row = cur.b * H + cur.h;
-    const bool ends = cur.next(prefix, B, H);
+    const int b = cur.b, h = cur.h;
+    const bool ends = cur.next(a, prefix);
     if (ends || u + 1 == u1) {
       fresh = true;
-      float *dst = a.partials + (worker + row) * G * PART;
+      const bool all = from_start && ends;          // the whole row: no one else has a part of it
+      const int64_t row = static_cast<int64_t>(b) * H + h;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         float s = sum[m];
         s += __shfl_xor_sync(0xffffffffu, s, 1);
         s += __shfl_xor_sync(0xffffffffu, s, 2);
         const int head = g + 8 * m;
-        if (head < G) {
-          float *o = dst + head * PART;
+        if (head < G && all) {
+          T *o = static_cast<T *>(a.out) + (row * G + head) * HD + 2 * t;
+          const float inv = 1.0f / s;
+#pragma unroll
+          for (int n = 0; n < 16; ++n)
+            *reinterpret_cast<uint32_t *>(o + 8 * n) = pack_t<T>(acc[n][2 * m] * inv, acc[n][2 * m + 1] * inv);
+        } else if (head < G) {
+          float *o = a.partials + ((worker + row) * G + head) * PART;
 #pragma unroll
           for (int n = 0; n < 16; ++n)
             *reinterpret_cast<float2 *>(o + 8 * n + 2 * t) = make_float2(acc[n][2 * m], acc[n][2 * m + 1]);
@@ -443,24 +475,22 @@ __global__ void __launch_bounds__(512) kv8_join_kernel(const __grid_constant__ K
   const int c = threadIdx.x & 127, grp = threadIdx.x >> 7;
   dep_wait();
   dep_release();
-  const int64_t units = static_cast<int64_t>(a.prefix[a.B]) * H;
-  const int64_t before = static_cast<int64_t>(a.prefix[b]) * H, nblk = a.prefix[b + 1] - a.prefix[b];
+  const int units = a.prefix[a.B] * H, before = a.prefix[b] * H, nblk = a.prefix[b + 1] - a.prefix[b];
   float m = -INFINITY, l = 0.0f, acc = 0.0f;
   if (nblk > 0) {
-    const int64_t f = before + h * nblk;
-    const int64_t w0 = kv8_worker_of(f, units, a.workers), w1 = kv8_worker_of(f + nblk - 1, units, a.workers);
+    const int f = before + h * nblk;
+    const int w0 = kv8_worker_of(f, units, a.workers), w1 = kv8_worker_of(f + nblk - 1, units, a.workers);
+    if (w0 == w1) return;                    // one worker had the whole row and has written it
     const float *p = a.partials + ((b * static_cast<int64_t>(H) + h) * G + head % G) * PART;
     const int64_t step = static_cast<int64_t>(G) * PART;
-    for (int64_t w = w0 + grp; w <= w1; w += 16) {       // four of the group's partials at once
+    for (int w = w0 + grp; w <= w1; w += 16) {       // four of the group's partials at once
       float pm[4], pl[4], pv[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int64_t wj = w + 4 * j;
         pm[j] = -INFINITY;
         pl[j] = pv[j] = 0.0f;
-        // a worker without units has no partial
-        if (wj <= w1 && kv8_first_unit(wj, units, a.workers) < kv8_first_unit(wj + 1, units, a.workers)) {
-          const float *o = p + wj * step;
+        if (w + 4 * j <= w1) {               // workers between two that have units have units
+          const float *o = p + (w + 4 * j) * step;
           const float2 x = *reinterpret_cast<const float2 *>(o + HD);
           pm[j] = x.x;
           pl[j] = x.y;
@@ -540,8 +570,8 @@ extern "C" int kitty_kv8_attn(const kitty_kv8_layer *layer, const int32_t *lengt
   if ((reinterpret_cast<uintptr_t>(query) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return KITTY_E_BADARG;
   if (workspace_bytes < need) return KITTY_E_WORKSPACE;
-  // units are counted in 32 bits per head
-  if (static_cast<int64_t>(B) * layer->max_page * 4 > 0x7fffffff) return KITTY_E_BADSHAPE;
+  // units are counted in 32 bits
+  if (static_cast<int64_t>(B) * layer->max_page * 4 > 0x7fffffff / layer->h_kv) return KITTY_E_BADSHAPE;
   const int sms = sm_count() < KV8_MAX_SMS ? sm_count() : KV8_MAX_SMS;
   Kv8AttnArgs a{};
   a.L = *layer;

@@ -112,7 +112,7 @@ def read_records(layer, lengths):
         ks, vs = torch.zeros(H, nb), torch.zeros(H, nb)
         for j in range(nb):
             rec = pages[table[b, j // 4], :, j % 4]                              # [H, 8208]
-            code = rec[:, :8192].to(torch.float64) - 128.0
+            code = rec[:, :8192].view(torch.int8).to(torch.float64)
             kp, vp = code[:, :4096].reshape(H, 256, 16), code[:, 4096:].reshape(H, 256, 16)
             for e in range(16):
                 kc[:, j, k_tok, k_ch + e] = kp[:, :, e]

@@ -151,11 +151,17 @@ def _attention_check(got, q, layer, lengths, tails, scaling):
         kk = torch.cat((kk.to(DEV), tails[0][b][:, full:n].double()), 1)
         vv = torch.cat((vv.to(DEV), tails[1][b][:, full:n].double()), 1)
         for x in range(hq):
-            qx = q[b, x].double()
-            want, mag = attend_fast(qx, kk[x // G], vv[x // G], scaling, torch.tensor([n], device=DEV))
-            # weights are fp16 numbers in the products; those below its normal range lose at most 2^-25 each
-            bound = attention_bound(want, mag, q.dtype, HALF[torch.float16], logit_error(qx, kk[x // G], scaling))
-            bound = bound + 2.0 ** -25 * vv[x // G].abs().sum(0) + 2.0 ** -23 * n * vv[x // G].abs().max()
+            qx, kx, vx = q[b, x].double(), kk[x // G], vv[x // G]
+            want, mag = attend_fast(qx, kx, vx, scaling, torch.tensor([n], device=DEV))
+            # query elements are within half of (largest of the head) / 32512 of their value, 2^-15.98 of the largest
+            delta = logit_error(qx, kx, scaling) + 2.0 ** -15.9 * (qx.abs().max() * kx.abs().sum(1).max()).item() * scaling
+            # weights within the same part of their block's largest; those of the open block are sums of two 16-bit numbers
+            # (2^-16 of their own size)
+            bound = attention_bound(want, mag, q.dtype, 2.0 ** -16, delta)
+            if full:
+                p = torch.softmax((kx @ qx[0]) * scaling, 0)[:full].view(-1, 32)
+                share = p.amax(1) @ vx[:full].abs().view(-1, 32, 128).sum(1)
+                bound = bound + 2.0 ** -15.9 * share * (1.0 + 2.0 * delta)
             off = (got[b, :, x].double() - want).abs()
             assert (off <= bound).all(), (b, x, n, off.max().item(), bound.max().item())
 
