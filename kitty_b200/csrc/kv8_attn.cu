@@ -465,68 +465,139 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __gri
   }
 }
 
-// Joins the partials of one (sequence, query head): four groups of 128 threads, a channel each, take every fourth
-// partial; weights 2^(max - largest max) in 32 bits.
+// Workers that share the row of (sequence b, key head h): first and last; false when nothing is left to do (one worker
+// had the whole row and has written it).
+__device__ __forceinline__ bool kv8_shared_row(const Kv8AttnArgs &a, int b, int h, int &w0, int &w1, int &nblk) {
+  const int H = a.L.h_kv, units = a.prefix[a.B] * H, before = a.prefix[b] * H;
+  nblk = a.prefix[b + 1] - a.prefix[b];
+  w0 = w1 = 0;
+  if (nblk == 0) return true;
+  const int f = before + h * nblk;
+  w0 = kv8_worker_of(f, units, a.workers);
+  w1 = kv8_worker_of(f + nblk - 1, units, a.workers);
+  return w0 != w1;
+}
+
+// Joins the partials of rows that several workers share, weights 2^(max - largest max) in 32 bits, partials in the order
+// of the workers.  Two shapes, by how many partials a row can have (about workers / rows + 2):
+// many rows, few partials: a warp per (sequence, query head), four channels a lane.
 template <typename T>
-__global__ void __launch_bounds__(512) kv8_join_kernel(const __grid_constant__ Kv8AttnArgs a) {
-  __shared__ float red[4][HD], ms[4][2];
+__global__ void __launch_bounds__(256) kv8_join_rows_kernel(const __grid_constant__ Kv8AttnArgs a) {
   const int H = a.L.h_kv, G = a.G, hq = H * G;
-  const int b = blockIdx.x / hq, head = blockIdx.x % hq, h = head / G;
-  const int c = threadIdx.x & 127, grp = threadIdx.x >> 7;
+  const int at = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   dep_wait();
-  dep_release();
-  const int units = a.prefix[a.B] * H, before = a.prefix[b] * H, nblk = a.prefix[b + 1] - a.prefix[b];
-  float m = -INFINITY, l = 0.0f, acc = 0.0f;
-  if (nblk > 0) {
-    const int f = before + h * nblk;
-    const int w0 = kv8_worker_of(f, units, a.workers), w1 = kv8_worker_of(f + nblk - 1, units, a.workers);
-    if (w0 == w1) return;                    // one worker had the whole row and has written it
-    const float *p = a.partials + ((b * static_cast<int64_t>(H) + h) * G + head % G) * PART;
-    const int64_t step = static_cast<int64_t>(G) * PART;
-    for (int w = w0 + grp; w <= w1; w += 16) {       // four of the group's partials at once
-      float pm[4], pl[4], pv[4];
+  if (at >= a.B * hq) return;
+  const int b = at / hq, head = at % hq, h = head / G;
+  int w0, w1, nblk;
+  if (!kv8_shared_row(a, b, h, w0, w1, nblk)) return;
+  T *out = static_cast<T *>(a.out) + static_cast<int64_t>(at) * HD + 4 * lane;
+  float m = -INFINITY, l = 0.0f, acc[4] = {};
+  const float *p = a.partials + ((static_cast<int64_t>(b) * H + h) * G + head % G) * PART;
+  const int64_t step = static_cast<int64_t>(G) * PART;
+  if (nblk > 0)
+    for (int w = w0; w <= w1; w += 4) {
+      float2 ml[4], v[4][2];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        pm[j] = -INFINITY;
-        pl[j] = pv[j] = 0.0f;
-        if (w + 4 * j <= w1) {               // workers between two that have units have units
-          const float *o = p + (w + 4 * j) * step;
-          const float2 x = *reinterpret_cast<const float2 *>(o + HD);
-          pm[j] = x.x;
-          pl[j] = x.y;
-          pv[j] = o[c];
+        ml[j] = make_float2(-INFINITY, 0.0f);
+        v[j][0] = v[j][1] = make_float2(0.0f, 0.0f);
+        if (w + j <= w1) {
+          const float *o = p + (w + j) * step;
+          ml[j] = *reinterpret_cast<const float2 *>(o + HD);
+          v[j][0] = *reinterpret_cast<const float2 *>(o + 4 * lane);
+          v[j][1] = *reinterpret_cast<const float2 *>(o + 4 * lane + 2);
         }
       }
-      float mn = m;
+      const float mn = fmaxf(fmaxf(m, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x));
+      const float ref = mn == -INFINITY ? 0.0f : mn, f = ex2(m - ref);
+      l *= f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mn = fmaxf(mn, pm[j]);
-      const float ref = mn == -INFINITY ? 0.0f : mn;
-      const float f0 = ex2(m - ref);
-      l *= f0;
-      acc *= f0;
+      for (int e = 0; e < 4; ++e) acc[e] *= f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float wgt = ex2(pm[j] - ref);
-        l = fmaf(pl[j], wgt, l);
-        acc = fmaf(pv[j], wgt, acc);
+        const float g = ex2(ml[j].x - ref);
+        l = fmaf(ml[j].y, g, l);
+        acc[0] = fmaf(v[j][0].x, g, acc[0]);
+        acc[1] = fmaf(v[j][0].y, g, acc[1]);
+        acc[2] = fmaf(v[j][1].x, g, acc[2]);
+        acc[3] = fmaf(v[j][1].y, g, acc[3]);
       }
       m = mn;
     }
+  const float inv = nblk > 0 ? 1.0f / l : 0.0f;
+  uint2 o;
+  o.x = pack_t<T>(acc[0] * inv, acc[1] * inv);
+  o.y = pack_t<T>(acc[2] * inv, acc[3] * inv);
+  *reinterpret_cast<uint2 *>(out) = o;
+}
+
+// few rows, many partials: a block per (sequence, query head); thread s first turns the maximum of partial s into its
+// weight, while every thread already has its channel of the first partials of its group in flight.
+template <typename T, int KV8_JOIN_GROUPS>
+__global__ void __launch_bounds__(HD * KV8_JOIN_GROUPS) kv8_join_kernel(const __grid_constant__ Kv8AttnArgs a) {
+  constexpr int NT = HD * KV8_JOIN_GROUPS, NW = NT / 32;
+  __shared__ float wgt[NT], red[KV8_JOIN_GROUPS][HD], wm[NW], wl[NW];
+  const int H = a.L.h_kv, G = a.G, hq = H * G;
+  const int b = blockIdx.x / hq, head = blockIdx.x % hq, h = head / G;
+  const int c = threadIdx.x & (HD - 1), grp = threadIdx.x / HD, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  dep_wait();
+  int w0, w1, nblk;
+  if (!kv8_shared_row(a, b, h, w0, w1, nblk)) return;
+  const float *p = a.partials + ((static_cast<int64_t>(b) * H + h + w0) * G + head % G) * PART;
+  const int64_t step = static_cast<int64_t>(G) * PART;
+  const int n = nblk > 0 ? w1 - w0 + 1 : 0;
+  float m = -INFINITY, l = 0.0f, acc = 0.0f;
+  for (int s0 = 0; s0 < n; s0 += NT) {               // one pass unless a row has over a thousand partials
+    const int nn = min(NT, n - s0);
+    constexpr int U = 2 * KV8_JOIN_GROUPS;
+    float v[U];
+    auto fetch = [&](int s) {
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int sj = s + j * KV8_JOIN_GROUPS;
+        v[j] = sj < nn ? p[(s0 + sj) * step + c] : 0.0f;
+      }
+    };
+    fetch(grp);
+    float2 ml = make_float2(-INFINITY, 0.0f);
+    if (static_cast<int>(threadIdx.x) < nn) ml = *reinterpret_cast<const float2 *>(p + (s0 + threadIdx.x) * step + HD);
+    float top = ml.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    __syncthreads();
+    if (lane == 0) wm[warp] = top;
+    __syncthreads();
+    float mn = m;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) mn = fmaxf(mn, wm[i]);
+    const float ref = mn == -INFINITY ? 0.0f : mn, f = ex2(m - ref), g = ex2(ml.x - ref);
+    m = mn;
+    wgt[threadIdx.x] = g;
+    float part = ml.y * g;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    if (lane == 0) wl[warp] = part;
+    __syncthreads();
+    l *= f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) l += wl[i];
+    acc *= f;
+    for (int s = grp; s < nn; s += U * KV8_JOIN_GROUPS) {
+      if (s != grp) fetch(s);
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int sj = s + j * KV8_JOIN_GROUPS;
+        acc = fmaf(v[j], sj < nn ? wgt[sj] : 0.0f, acc);
+      }
+    }
   }
   red[grp][c] = acc;
-  if (c == 0) ms[grp][0] = m, ms[grp][1] = l;
   __syncthreads();
   if (grp != 0) return;
-  float mn = fmaxf(fmaxf(ms[0][0], ms[1][0]), fmaxf(ms[2][0], ms[3][0]));
-  if (mn == -INFINITY) mn = 0.0f;
-  float tot = 0.0f, ls = 0.0f;
+  float tot = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float wgt = ex2(ms[i][0] - mn);
-    tot = fmaf(red[i][c], wgt, tot);
-    ls = fmaf(ms[i][1], wgt, ls);
-  }
-  static_cast<T *>(a.out)[static_cast<int64_t>(blockIdx.x) * HD + c] = from_f32<T>(nblk > 0 ? tot / ls : 0.0f);
+  for (int i = 0; i < KV8_JOIN_GROUPS; ++i) tot += red[i][c];
+  static_cast<T *>(a.out)[static_cast<int64_t>(blockIdx.x) * HD + c] = from_f32<T>(nblk > 0 ? tot / l : 0.0f);
 }
 
 template <typename T, int MT>
@@ -541,7 +612,14 @@ int launch_kv8_attn(const Kv8AttnArgs &a, int blocks, int smem, cudaStream_t s) 
   if (rc != KITTY_OK) return rc;
   kv8_attn_kernel<T, MT><<<blocks, KV8_WARPS * 32, smem, s>>>(a);
   if (cudaGetLastError() != cudaSuccess) return KITTY_E_CUDA;
-  const cudaError_t e = launch_after(kv8_join_kernel<T>, dim3(a.B * a.L.h_kv * a.G), dim3(512), 0, s, a);
+  // From 256 rows on a row has nine partials or fewer (1776 workers): folded by a warp each (1024 rows: 5 us, 25 us as
+  // blocks).  Below, a block each: 1024 threads for a few rows of hundreds of partials (8 rows of 222: 9 us, 16 us with
+  // 512 threads), 512 threads when there are more blocks than multiprocessors (64 rows of 28: 7 us, 11 us with 1024).
+  const int heads = a.B * a.L.h_kv * a.G;
+  cudaError_t e;
+  if (a.B * a.L.h_kv >= 256) e = launch_after(kv8_join_rows_kernel<T>, dim3((heads + 7) / 8), dim3(256), 0, s, a);
+  else if (heads > blocks) e = launch_after(kv8_join_kernel<T, 4>, dim3(heads), dim3(HD * 4), 0, s, a);
+  else e = launch_after(kv8_join_kernel<T, 8>, dim3(heads), dim3(HD * 8), 0, s, a);
   return (e == cudaSuccess && cudaGetLastError() == cudaSuccess) ? KITTY_OK : KITTY_E_CUDA;
 }
 
