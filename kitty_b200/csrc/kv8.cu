@@ -36,13 +36,70 @@ __device__ __forceinline__ uint32_t kv8_codes4(const float *x, float inv) {
   return __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
 }
 
+// The angle table of the append kernel: entries of the 32 tokens side by side in the order in which the four threads of
+// a key token hold its channels (thread t: channels 16t .. 16t + 15 and 64 + 16t ... as sixteen pairs), two pairs a word.
+// Pairs in halves of a fully rotated head: pair 16t + e; neighbouring pairs: 8t + e, then 32 + 8t + e - 8.  A partly
+// rotated head in halves keeps the first form, its pairs in order.
 template <typename T, int MODE>
-__global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__ AppendArgs a) {
+struct BlockTable {
+  using U = RotUnits<T, MODE>;
+  static constexpr bool INTER = MODE == ROT_INTER || MODE == ROT_INTER_SCALAR;
+  const float4 *tab;       // [8][128]
+  int tk;
+  // word and half of pair p of token tk
+  static __device__ __forceinline__ int word(int p, int tk) {
+    const int t = INTER ? (p >> 3) & 3 : p >> 4, e = INTER ? (p & 7) + 8 * (p >> 5) : p & 15;
+    return (e >> 1) * 128 + 4 * tk + t;
+  }
+  __device__ __forceinline__ float4 pairs(int p) const { return tab[word(p, tk)]; }          // p even: pairs p, p + 1
+  __device__ __forceinline__ float4 two(int u, int k) const { return pairs(u * U::PV + 2 * k); }
+  __device__ __forceinline__ float2 one(int p) const {
+    const float4 x = pairs(p & ~1);
+    return p & 1 ? make_float2(x.z, x.w) : make_float2(x.x, x.y);
+  }
+};
+
+// 4 x 4 bytes the other way round: byte j of out[i] = byte i of in[j].
+__device__ __forceinline__ void transpose4(const uint32_t (&in)[4], uint32_t (&out)[4]) {
+  const uint32_t a = __byte_perm(in[0], in[1], 0x5140), b = __byte_perm(in[2], in[3], 0x5140);
+  const uint32_t c = __byte_perm(in[0], in[1], 0x7362), d = __byte_perm(in[2], in[3], 0x7362);
+  out[0] = __byte_perm(a, b, 0x5410);
+  out[1] = __byte_perm(a, b, 0x7632);
+  out[2] = __byte_perm(c, d, 0x5410);
+  out[3] = __byte_perm(c, d, 0x7632);
+}
+
+// Scale of a block whose largest magnitude has the 16-bit pattern m, and the factor that takes its numbers to codes.
+template <typename T>
+__device__ __forceinline__ float kv8_scale(uint32_t m, float &inv, float &pre) {
+  constexpr uint32_t INF16 = __is_same(T, __half) ? 0x7c00u : 0x7f80u;
+  pre = 1.0f;
+  inv = 0.0f;
+  if (m >= INF16) return __uint_as_float(0x7fc00000u);
+  if (m == 0) return 1.0f;
+  const uint16_t mb = static_cast<uint16_t>(m);
+  const float top = to_f32<T>(*reinterpret_cast<const T *>(&mb));
+  if (top < 0x1p-100f) pre = 0x1p100f;                  // keeps the reciprocal in range
+  inv = __fdiv_rn(127.0f, top * pre) * (1.0f + 0x1p-21f);
+  return __fdiv_rn(top, 127.0f);
+}
+
+__device__ __forceinline__ uint32_t max_abs16(uint32_t m, uint32_t w) { return __vmaxu2(m, w & 0x7fff7fffu); }
+
+// Blocks of threads per multiprocessor: the forms with more state in registers take fewer.
+template <int MODE>
+constexpr int APPEND_BLOCKS = MODE == ROT_NONE ? 4 : MODE == ROT_HALF || MODE == ROT_INTER ? 3 : 2;
+
+// A block walks over the heads with the next head's loads in flight
+// behind the current one's work.  Warps 0-3 take the keys, a token per four threads (both members of a pair in one
+// thread, angles from the shared table); warps 4-7 the values, eight tokens a warp, four channels a thread, so that the
+// tokens of a channel end up side by side in registers.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(256, APPEND_BLOCKS<MODE>) kv8_append_kernel(const __grid_constant__ AppendArgs a) {
   using U = RotUnits<T, MODE>;
   constexpr bool HALF = MODE == ROT_HALF || MODE == ROT_HALF_SCALAR;
-  constexpr uint32_t INF16 = sizeof(T) == 2 && __is_same(T, __half) ? 0x7c00u : 0x7f80u;
-  __shared__ __align__(16) float2 tab[MODE == ROT_NONE ? 1 : KV8_BLOCK][HD / 2];
-  __shared__ __align__(16) uint8_t vt[HD][36];
+  __shared__ __align__(16) float4 tab[MODE == ROT_NONE ? 1 : 8 * 128];
+  __shared__ __align__(16) uint8_t vt[KV8_OFF_V];
   __shared__ __align__(16) T stage[HALF ? KV8_BLOCK : 1][HD + 8];
   __shared__ uint32_t red[2][8];
   const kitty_kv8_layer &L = a.L;
@@ -58,200 +115,260 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__
   const int end = s + n, fb = s / KV8_BLOCK, eb = end / KV8_BLOCK;
   const int h0 = blockIdx.y * a.heads, h1 = min(h0 + a.heads, L.h_kv);
   const int r = a.pl.rotary_dim, np = r / 2;
-  const int half = threadIdx.x >> 7, tid = threadIdx.x & 127;
+  const int half = threadIdx.x >> 7, tid = threadIdx.x & 127, warp = tid >> 5, lane = tid & 31;
 
   auto process = [&](int blk, bool kv, bool rows_q) {
     const int t0 = blk * KV8_BLOCK - s;                 // input index of the block's first token
+    const bool full = (blk + 1) * KV8_BLOCK <= end;
+    const int64_t tail_row = static_cast<int64_t>(b) * L.h_kv * KV8_BLOCK * HD;
+    // keys: thread t of token tk holds chunks of eight channels, chunk c from 16t + 8 (c & 1) + 64 (c >> 1)
+    const int tk = tid >> 2, t = tid & 3, ik = t0 + tk;
+    const bool fresh = ik >= 0 && ik < n, kept = ik < 0 && full;
+    auto channel = [&](int c) { return (c >> 1) * 64 + 16 * t + (c & 1) * 8; };
+    T *tail_k = static_cast<T *>(L.tail_k) + tail_row + tk * HD;
+    auto fetch_k = [&](int h, uint4 (&w)[4]) {
+      const T *src = fresh ? static_cast<const T *>(a.k) + b * a.ks[0] + h * a.ks[1] + ik * a.ks[2]
+                           : tail_k + static_cast<int64_t>(h) * KV8_BLOCK * HD;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) w[c] = fresh || kept ? *reinterpret_cast<const uint4 *>(src + channel(c)) : make_uint4(0, 0, 0, 0);
+    };
+    // values: a warp's lane holds four channels of eight tokens
+    const int iv = t0 + 8 * warp;
+    T *tail_v = static_cast<T *>(L.tail_v) + tail_row + 8 * warp * HD + 4 * lane;
+    auto fetch_v = [&](int h, uint4 (&w)[4]) {
+      const T *in = static_cast<const T *>(a.v) + b * a.vs[0] + h * a.vs[1] + 4 * lane;
+      uint2 z[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = iv + j;
+        z[j] = make_uint2(0, 0);
+        if (i >= 0 && i < n) z[j] = *reinterpret_cast<const uint2 *>(in + i * a.vs[2]);
+        else if (i < 0 && full) z[j] = *reinterpret_cast<const uint2 *>(tail_v + (static_cast<int64_t>(h) * KV8_BLOCK + j) * HD);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) w[c] = make_uint4(z[2 * c].x, z[2 * c].y, z[2 * c + 1].x, z[2 * c + 1].y);
+    };
+    uint4 w[4];
+    if (kv) {                                           // on their way while the angles are made
+      if (half == 0) fetch_k(h0, w);
+      else fetch_v(h0, w);
+    }
     if constexpr (MODE != ROT_NONE) {
       const int last = rows_q ? a.T : n;
       for (int i = threadIdx.x; i < KV8_BLOCK * np; i += 256) {
         const int tk = i / np, p = i - tk * np;
-        if (t0 + tk >= 0 && t0 + tk < last) tab[tk][U::slot(p, r)] = rot_angle(a.pl, static_cast<int64_t>(raw) + t0 + tk, p);
+        if (t0 + tk >= 0 && t0 + tk < last)
+          reinterpret_cast<float2 *>(tab)[2 * BlockTable<T, MODE>::word(p, tk) + (p & 1)] =
+              rot_angle(a.pl, static_cast<int64_t>(raw) + t0 + tk, p);
       }
       __syncthreads();
     }
-    if (kv) {
-      const int tk = tid >> 2, t = tid & 3, warp = tid >> 5;
-      const int i = t0 + tk;
-      const bool full = (blk + 1) * KV8_BLOCK <= end;
-      const bool fresh = i >= 0 && i < n, kept = i < 0 && full;
-      const bool turn = MODE != ROT_NONE && half == 0 && fresh;
-      // A thread holds channels 16t .. 16t+15 and 64+16t .. 64+16t+15 of its token: for a fully rotated head in halves,
-      // and for neighbouring pairs, both members of sixteen pairs, whose angles stay in registers over the heads.
-      const bool in_regs = !HALF || r == HD;
-      float cs[16], sn[16];
-      if constexpr (MODE != ROT_NONE) {
-        if (turn && in_regs) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int p = HALF ? 16 * t + e : 8 * t + (e & 7) + 32 * (e >> 3);
-            const float2 x = p < np ? tab[tk][U::slot(p, r)] : make_float2(1.f, 0.f);
-            cs[e] = x.x;
-            sn[e] = x.y;
-          }
-        }
-      }
-      const int64_t page = full ? kv8_page(L, b, blk) : -1;
-      T *tail = static_cast<T *>(half ? L.tail_v : L.tail_k);
-      const int64_t *st = half ? a.vs : a.ks;
-      const T *in = static_cast<const T *>(half ? a.v : a.k) + b * st[0] + i * st[2];
+    const int64_t page = kv && full ? kv8_page(L, b, blk) : -1;
+    if (kv && half == 0) {
+      const bool turn = MODE != ROT_NONE && fresh;
+      const BlockTable<T, MODE> table{tab, tk};
       for (int h = h0; h < h1; ++h) {
-        T *trow = tail + ((static_cast<int64_t>(b) * L.h_kv + h) * KV8_BLOCK + tk) * HD;
-        uint4 w[4] = {};
-        if (fresh || kept) {
-          const T *src = fresh ? in + h * st[1] : trow;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) w[c] = *reinterpret_cast<const uint4 *>(src + (c >> 1) * 64 + t * 16 + (c & 1) * 8);
-        }
+        uint4 nx[4];
+        if (h + 1 < h1) fetch_k(h + 1, nx);
         if constexpr (MODE != ROT_NONE) {
-          if (turn && in_regs) {
-            float x[4][8];
+          if (HALF && r != HD) {                // a pair's members are in two threads of the token's four
 #pragma unroll
-            for (int c = 0; c < 4; ++c) Vec8<T>::unpack(w[c], x[c]);
+            for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4 *>(&stage[tk][channel(c)]) = w[c];
+            __syncwarp();
+            if (turn) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              if constexpr (HALF) {
-                const float u = x[e >> 3][e & 7], v = x[2 + (e >> 3)][e & 7];
-                x[e >> 3][e & 7] = fmaf(u, cs[e], -v * sn[e]);
-                x[2 + (e >> 3)][e & 7] = fmaf(v, cs[e], u * sn[e]);
-              } else {
-                float &u = x[e >> 2][(2 * e) & 7], &v = x[e >> 2][(2 * e + 1) & 7];
-                if (8 * t + (e & 7) + 32 * (e >> 3) < np) {      // an untouched pair may hold infinities
-                  const float u0 = u;
-                  u = fmaf(u0, cs[e], -v * sn[e]);
-                  v = fmaf(v, cs[e], u0 * sn[e]);
-                }
-              }
-            }
+              for (int c = 0; c < 4; ++c) {
+                const int d = channel(c);
+                if (d >= r) continue;
+                Piece<T> x;
+                x.unpack(w[c]);
+                if constexpr (MODE == ROT_HALF) {       // whole chunks on either side
+                  Piece<T> y;
+                  y.unpack(*reinterpret_cast<const uint4 *>(&stage[tk][d < np ? d + np : d - np]));
+                  const float sg = d < np ? -1.0f : 1.0f;
+                  const int p = d < np ? d : d - np;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              Piece<T> p;
-#pragma unroll
-              for (int e = 0; e < 8; ++e) p.f[e] = x[c][e];
-              w[c] = p.pack();
-            }
-          }
-          if constexpr (HALF) {
-            if (r != HD && half == 0) {        // a pair's members are in two threads of the token's four
-#pragma unroll
-              for (int c = 0; c < 4; ++c)
-                *reinterpret_cast<uint4 *>(&stage[tk][(c >> 1) * 64 + t * 16 + (c & 1) * 8]) = w[c];
-              __syncwarp();
-              if (turn) {
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                  Piece<T> p;
-                  p.unpack(w[c]);
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) {
-                    const int d = (c >> 1) * 64 + t * 16 + (c & 1) * 8 + e;
-                    if (d < r) {
-                      const int q = d < np ? d : d - np;
-                      const float2 z = tab[tk][U::slot(q, r)];
-                      const float o = to_f32<T>(stage[tk][d < np ? d + np : d - np]);
-                      p.f[e] = d < np ? fmaf(p.f[e], z.x, -o * z.y) : fmaf(p.f[e], z.x, o * z.y);
-                    }
+                  for (int e = 0; e < 8; e += 2) {
+                    const float4 z = table.pairs(p + e);
+                    x.f[e] = fmaf(x.f[e], z.x, sg * (y.f[e] * z.y));
+                    x.f[e + 1] = fmaf(x.f[e + 1], z.z, sg * (y.f[e + 1] * z.w));
                   }
-                  w[c] = p.pack();
+                } else {
+#pragma unroll
+                  for (int e = 0; e < 8; ++e)
+                    if (d + e < r) {
+                      const bool first = d + e < np;
+                      const float2 z = table.one(first ? d + e : d + e - np);
+                      const float o = to_f32<T>(stage[tk][first ? d + e + np : d + e - np]);
+                      x.f[e] = fmaf(x.f[e], z.x, first ? -o * z.y : o * z.y);
+                    }
+                }
+                w[c] = x.pack();
+              }
+            }
+            __syncwarp();
+          } else if (turn) {
+#pragma unroll
+            for (int c = 0; c < (HALF ? 2 : 4); ++c) {
+              Piece<T> x;
+              x.unpack(w[c]);
+              if constexpr (HALF) {             // channels 16t + e and 64 + 16t + e: both here
+                Piece<T> y;
+                y.unpack(w[c + 2]);
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                  const float4 z = table.pairs(16 * t + 8 * c + e);
+                  const float x0 = x.f[e], y0 = y.f[e], x1 = x.f[e + 1], y1 = y.f[e + 1];
+                  x.f[e] = fmaf(x0, z.x, -y0 * z.y);
+                  y.f[e] = fmaf(y0, z.x, x0 * z.y);
+                  x.f[e + 1] = fmaf(x1, z.z, -y1 * z.w);
+                  y.f[e + 1] = fmaf(y1, z.z, x1 * z.w);
+                }
+                w[c + 2] = y.pack();
+              } else {
+                const int p = channel(c) / 2;
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                  const float4 z = table.pairs(p + e);
+                  const float x0 = x.f[2 * e], x1 = x.f[2 * e + 1], x2 = x.f[2 * e + 2], x3 = x.f[2 * e + 3];
+                  if (p + e < np) {             // an untouched pair may hold infinities
+                    x.f[2 * e] = fmaf(x0, z.x, -x1 * z.y);
+                    x.f[2 * e + 1] = fmaf(x1, z.x, x0 * z.y);
+                  }
+                  if (p + e + 1 < np) {
+                    x.f[2 * e + 2] = fmaf(x2, z.z, -x3 * z.w);
+                    x.f[2 * e + 3] = fmaf(x3, z.z, x2 * z.w);
+                  }
                 }
               }
-              __syncwarp();
+              w[c] = x.pack();
             }
           }
         }
         if (!full) {
           if (fresh) {
+            T *o = tail_k + static_cast<int64_t>(h) * KV8_BLOCK * HD;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4 *>(trow + (c >> 1) * 64 + t * 16 + (c & 1) * 8) = w[c];
-          }
-          continue;
-        }
-        // largest magnitude of the block: 16-bit patterns without the sign order like the numbers
-        uint32_t m = 0;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          m = __vmaxu2(m, w[c].x & 0x7fff7fffu);
-          m = __vmaxu2(m, w[c].y & 0x7fff7fffu);
-          m = __vmaxu2(m, w[c].z & 0x7fff7fffu);
-          m = __vmaxu2(m, w[c].w & 0x7fff7fffu);
-        }
-        m = max(m & 0xffffu, m >> 16);
-        m = __reduce_max_sync(0xffffffffu, m);
-        uint32_t *rd = red[h & 1] + 4 * half;
-        if ((tid & 31) == 0) rd[warp] = m;
-        half_barrier(half);
-        m = max(max(rd[0], rd[1]), max(rd[2], rd[3]));
-        const uint16_t mb = static_cast<uint16_t>(m);
-        const float top = to_f32<T>(*reinterpret_cast<const T *>(&mb));
-        float scale, inv;
-        float pre = 1.0f;
-        if (m >= INF16) scale = __uint_as_float(0x7fc00000u), inv = 0.0f;
-        else if (m == 0) scale = 1.0f, inv = 0.0f;
-        else {
-          if (top < 0x1p-100f) pre = 0x1p100f;           // keeps the reciprocal in range
-          scale = __fdiv_rn(top, 127.0f);
-          inv = __fdiv_rn(127.0f, top * pre) * (1.0f + 0x1p-21f);
-        }
-        uint8_t *rec = page >= 0 ? kv8_record(L, page, h, blk & 3) : nullptr;
-        if (rec != nullptr && tid == 0) *reinterpret_cast<float *>(rec + KV8_OFF_SCALE + 4 * half) = scale;
-        uint4 code[2];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float x[8];
-          Vec8<T>::unpack(w[c], x);
-          if (pre != 1.0f) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] *= pre;
-          }
-          const uint32_t lo = kv8_codes4(x, inv), hi = kv8_codes4(x + 4, inv);
-          if (c & 1) code[c >> 1].z = lo, code[c >> 1].w = hi;
-          else code[c >> 1].x = lo, code[c >> 1].y = hi;
-        }
-        if (half == 0) {
-          if (rec != nullptr) {
-            const int i4 = (tk >> 1) & 3, g = 2 * (tk >> 3) + (tk & 1);
-            uint8_t *o = rec + i4 * 1024 + (4 * g + t) * 16;
-            *reinterpret_cast<uint4 *>(o) = code[0];
-            *reinterpret_cast<uint4 *>(o + 512) = code[1];
+            for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4 *>(o + channel(c)) = w[c];
           }
         } else {
-          // values go out with their tokens side by side
+          // largest magnitude of the block: 16-bit patterns without the sign order like the numbers
+          uint32_t m = 0;
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const uint32_t q4[4] = {code[c].x, code[c].y, code[c].z, code[c].w};
+          for (int c = 0; c < 4; ++c) m = max_abs16(max_abs16(max_abs16(max_abs16(m, w[c].x), w[c].y), w[c].z), w[c].w);
+          m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+          if (lane == 0) red[h & 1][warp] = m;
+          half_barrier(0);
+          m = max(max(red[h & 1][0], red[h & 1][1]), max(red[h & 1][2], red[h & 1][3]));
+          float inv, pre;
+          const float scale = kv8_scale<T>(m, inv, pre);
+          if (page >= 0) {
+            uint8_t *rec = kv8_record(L, page, h, blk & 3);
+            if (tid == 0) *reinterpret_cast<float *>(rec + KV8_OFF_SCALE) = scale;
+            uint8_t *o = rec + ((tk >> 1) & 3) * 1024 + (4 * (2 * (tk >> 3) + (tk & 1)) + t) * 16;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) vt[64 * c + 16 * t + e][tk] = static_cast<uint8_t>(q4[e >> 2] >> (8 * (e & 3)));
-          }
-          half_barrier(half);
-          if (rec != nullptr) {
+            for (int c = 0; c < 4; c += 2) {
+              uint32_t code[4];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int p = tid + 128 * j, x = p >> 5, g = (p >> 2) & 7, tt = p & 3;
-              const uint32_t *r0 = reinterpret_cast<const uint32_t *>(&vt[16 * x + g][8 * tt]);
-              const uint32_t *r1 = reinterpret_cast<const uint32_t *>(&vt[16 * x + 8 + g][8 * tt]);
-              *reinterpret_cast<uint4 *>(rec + KV8_OFF_V + p * 16) = make_uint4(r0[0], r0[1], r1[0], r1[1]);
+              for (int y = 0; y < 2; ++y) {
+                Piece<T> x;
+                x.unpack(w[c + y]);
+                if (pre != 1.0f) {
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) x.f[e] *= pre;
+                }
+                code[2 * y] = kv8_codes4(x.f, inv);
+                code[2 * y + 1] = kv8_codes4(x.f + 4, inv);
+              }
+              *reinterpret_cast<uint4 *>(o + (c >> 1) * 512) = make_uint4(code[0], code[1], code[2], code[3]);
             }
           }
         }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w[c] = nx[c];
+      }
+    } else if (kv) {
+      for (int h = h0; h < h1; ++h) {
+        uint4 nx[4];
+        if (h + 1 < h1) fetch_v(h + 1, nx);
+        if (!full) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint4 z = w[j >> 1];
+            if (iv + j >= 0 && iv + j < n)
+              *reinterpret_cast<uint2 *>(tail_v + (static_cast<int64_t>(h) * KV8_BLOCK + j) * HD) = j & 1 ? make_uint2(z.z, z.w) : make_uint2(z.x, z.y);
+          }
+        } else {
+          uint32_t m = 0;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) m = max_abs16(max_abs16(max_abs16(max_abs16(m, w[c].x), w[c].y), w[c].z), w[c].w);
+          m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+          if (lane == 0) red[h & 1][4 + warp] = m;
+          half_barrier(1);
+          m = max(max(red[h & 1][4], red[h & 1][5]), max(red[h & 1][6], red[h & 1][7]));
+          float inv, pre;
+          const float scale = kv8_scale<T>(m, inv, pre);
+          uint32_t out[2][4];                   // [tokens 4y .. 4y + 3][channel 4 lane + j]
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            uint32_t code[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint4 q4 = w[2 * y + (j >> 1)];
+              const uint2 z = j & 1 ? make_uint2(q4.z, q4.w) : make_uint2(q4.x, q4.y);
+              T v4[4];
+              memcpy(v4, &z, 8);
+              float x[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] = to_f32<T>(v4[e]) * pre;
+              code[j] = kv8_codes4(x, inv);
+            }
+            transpose4(code, out[y]);
+          }
+          // channel c: piece c / 16, half (c / 8) % 2, lane 4 (c % 8) + the tokens' eight (the warp)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int c = 4 * lane + j;
+            *reinterpret_cast<uint2 *>(vt + (c >> 4) * 512 + (4 * (c & 7) + warp) * 16 + ((c >> 3) & 1) * 8) = make_uint2(out[0][j], out[1][j]);
+          }
+          half_barrier(1);
+          if (page >= 0) {
+            uint8_t *rec = kv8_record(L, page, h, blk & 3);
+            if (tid == 0) *reinterpret_cast<float *>(rec + KV8_OFF_SCALE + 4) = scale;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              *reinterpret_cast<uint4 *>(rec + KV8_OFF_V + (tid + 128 * j) * 16) = *reinterpret_cast<const uint4 *>(vt + (tid + 128 * j) * 16);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w[c] = nx[c];
       }
     }
     if constexpr (MODE != ROT_NONE) {
       if (rows_q) {
-        constexpr int LPR = U::VEC ? (MODE == ROT_HALF ? 8 : 16) : 32;
+        constexpr int LPR = U::VEC ? (MODE == ROT_HALF ? 8 : 16) : 32, ROWS = 4;
         const int q0 = static_cast<int>(static_cast<int64_t>(a.h_q) * blockIdx.y / gridDim.y);
         const int q1 = static_cast<int>(static_cast<int64_t>(a.h_q) * (blockIdx.y + 1) / gridDim.y);
         const int first = max(0, -t0), toks = min(KV8_BLOCK, a.T - t0) - first, nh = q1 - q0;
         const int nu = U::turned(r) + U::copied(r);
-        for (int row = threadIdx.x / LPR; row < toks * nh; row += 256 / LPR) {
-          const int tk = first + row / nh, h = q0 + row % nh;
-          const T *src = static_cast<const T *>(a.q) + b * a.qs[0] + h * a.qs[1] + (t0 + tk) * a.qs[2];
-          T *dst = static_cast<T *>(a.q_out) + ((static_cast<int64_t>(b) * a.h_q + h) * a.T + t0 + tk) * HD;
+        constexpr int STEP = 256 / LPR;
+        for (int base = threadIdx.x / LPR; base < toks * nh; base += STEP * ROWS)
           for (int u = threadIdx.x % LPR; u < nu; u += LPR) {
-            RotUnit<T, MODE> x;
-            x.load(src, u, r);
-            x.store(dst, u, r, tab[tk]);
+            RotUnit<T, MODE> x[ROWS];
+#pragma unroll
+            for (int j = 0; j < ROWS; ++j) {
+              const int row = base + j * STEP, tk = first + row / nh, h = q0 + row % nh;
+              if (row < toks * nh)
+                x[j].load(static_cast<const T *>(a.q) + b * a.qs[0] + h * a.qs[1] + (t0 + tk) * a.qs[2], u, r);
+            }
+#pragma unroll
+            for (int j = 0; j < ROWS; ++j) {
+              const int row = base + j * STEP, tk = first + row / nh, h = q0 + row % nh;
+              if (row < toks * nh)
+                x[j].store(static_cast<T *>(a.q_out) + ((static_cast<int64_t>(b) * a.h_q + h) * a.T + t0 + tk) * HD, u, r,
+                           BlockTable<T, MODE>{tab, tk});
+            }
           }
-        }
       }
     }
     __syncthreads();
@@ -289,7 +406,8 @@ __device__ __forceinline__ void expand16(uint4 codes, float scale, uint4 (&out)[
 
 template <typename T>
 __global__ void __launch_bounds__(256) kv8_expand_kernel(const __grid_constant__ ExpandArgs a) {
-  __shared__ __align__(16) uint8_t vt[KV8_BLOCK][HD + 16];
+  // rows of 148 bytes: eight rows on is eight banks on, so the four token groups of a warp write to different banks
+  __shared__ __align__(16) uint8_t vt[KV8_BLOCK][HD + 20];
   const kitty_kv8_layer &L = a.L;
   const int b = blockIdx.z, h = blockIdx.y, cap = L.max_page * PAGE;
   const int len = kv8_clamp_len(L, a.lengths[b]);
@@ -329,7 +447,8 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const __grid_constant__
     }
     __syncthreads();
     const int tk = threadIdx.x >> 3, c = (threadIdx.x & 7) * 16;
-    expand16<T>(*reinterpret_cast<const uint4 *>(&vt[tk][c]), sc.y, x);
+    const uint32_t *vw = reinterpret_cast<const uint32_t *>(&vt[tk][c]);
+    expand16<T>(make_uint4(vw[0], vw[1], vw[2], vw[3]), sc.y, x);
     put(vo, tk, c, x);
   } else {
     const int tk = threadIdx.x >> 3, c = (threadIdx.x & 7) * 16;

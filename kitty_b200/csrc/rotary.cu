@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
   };
   for (int i = threadIdx.x; i < ntok * np; i += 256) {
     const int tok = i / np, p = i - tok * np;
-    tab[tok][U::slot(p, r)] = rot_angle(a.pl, a.pos[b * a.pos_b + t0 + tok], p);
+    tab[tok][RotTable<T, MODE>::slot(p, nt)] = rot_angle(a.pl, a.pos[b * a.pos_b + t0 + tok], p);
   }
   __syncthreads();
   for (int base = row0; base < rows; base += STEP * ROWS) {
@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
         }
 #pragma unroll
       for (int j = 0; j < ROWS; ++j)
-        if (base + j * STEP < rows) x[j].store(dst[j], u, r, tab[tok[j]]);
+        if (base + j * STEP < rows) x[j].store(dst[j], u, r, RotTable<T, MODE>{tab[tok[j]], nt});
     }
   }
 }
@@ -73,11 +73,11 @@ int launch_rotary(const RotArgs &a, dim3 grid, cudaStream_t s) {
   switch (rot_mode(a.pl, sizeof(T))) {
     case ROT_HALF: {
       // units of a full-width head: 8 (16 bit) or 16 (32 bit); a partly rotated head has up to twice as many
-      if (sizeof(T) == 2 && a.pl.rotary_dim == HD) rotary_kernel<T, ROT_HALF, 8, 4><<<grid, 256, 0, s>>>(a);
-      else rotary_kernel<T, ROT_HALF, 16, 4><<<grid, 256, 0, s>>>(a);
+      if (sizeof(T) == 2 && a.pl.rotary_dim == HD) rotary_kernel<T, ROT_HALF, 8, 2><<<grid, 256, 0, s>>>(a);
+      else rotary_kernel<T, ROT_HALF, 16, 2><<<grid, 256, 0, s>>>(a);
       break;
     }
-    case ROT_INTER: rotary_kernel<T, ROT_INTER, 16, 4><<<grid, 256, 0, s>>>(a); break;
+    case ROT_INTER: rotary_kernel<T, ROT_INTER, 16, 2><<<grid, 256, 0, s>>>(a); break;
     case ROT_HALF_SCALAR: rotary_kernel<T, ROT_HALF_SCALAR, 32, 4><<<grid, 256, 0, s>>>(a); break;
     default: rotary_kernel<T, ROT_INTER_SCALAR, 32, 4><<<grid, 256, 0, s>>>(a); break;
   }

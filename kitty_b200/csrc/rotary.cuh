@@ -17,21 +17,32 @@ enum RotMode { ROT_HALF = 0, ROT_INTER = 1, ROT_HALF_SCALAR = 2, ROT_INTER_SCALA
 
 // How a head row is cut into units: a unit of the vector modes is one 16-byte piece (interleaved) or the two pieces
 // that hold both halves of its pairs (half); scalar modes take one pair per unit (rotary_dim that does not split into
-// whole pieces).  Channels from rotary_dim on are copied, in pieces (vector) or one by one (scalar).
+// whole pieces).  Channels from rotary_dim on are copied: one by one up to the next piece, then piece by piece.
 template <typename T, int MODE>
 struct RotUnits {
   static constexpr int V = 16 / sizeof(T);                       // channels of a piece
   static constexpr int PV = MODE == ROT_HALF ? V : MODE == ROT_INTER ? V / 2 : 1;   // pairs of a unit
   static constexpr bool VEC = MODE == ROT_HALF || MODE == ROT_INTER;
   static __device__ __forceinline__ int turned(int r) { return r / 2 / PV; }        // units that turn pairs
-  static __device__ __forceinline__ int copied(int r) { return VEC ? (HD - r) / V : HD - r; }
-  // Where pair p sits in a token's table row (float2, at most 64 of them): the pairs of all units are interleaved two
-  // by two, so that a row of threads reads consecutive 16-byte words.
-  static __device__ __forceinline__ int slot(int p, int r) {
-    if (PV == 1) return p;
-    const int u = p / PV, e = p % PV;
-    return ((e >> 1) * turned(r) + u) * 2 + (e & 1);
+  static __device__ __forceinline__ int loose(int r) { return VEC ? 0 : (V - r % V) % V; }      // channels copied singly
+  static __device__ __forceinline__ int copied(int r) { return loose(r) + (HD - r) / V; }
+};
+
+// The angle table of a block of threads in the order of the rotary kernel's units: token by token (64 entries each), the
+// pairs of all units two by two, so that a row of threads reads consecutive 16-byte words.
+template <typename T, int MODE>
+struct RotTable {
+  using U = RotUnits<T, MODE>;
+  const float2 *tab;       // the token's entries
+  int nt;
+  static __device__ __forceinline__ int slot(int p, int nt) {
+    if (U::PV == 1) return p;
+    const int u = p / U::PV, e = p % U::PV;
+    return ((e >> 1) * nt + u) * 2 + (e & 1);
   }
+  // pairs 2k and 2k + 1 of unit u
+  __device__ __forceinline__ float4 two(int u, int k) const { return *reinterpret_cast<const float4 *>(tab + (k * nt + u) * 2); }
+  __device__ __forceinline__ float2 one(int p) const { return tab[p]; }
 };
 
 __device__ __forceinline__ float2 rot_angle(const kitty_rotary_plan &pl, int64_t pos, int p) {
@@ -85,12 +96,15 @@ struct RotUnit {
       if (u < nt) {
         s0 = row[MODE == ROT_HALF_SCALAR ? u : 2 * u];
         s1 = row[MODE == ROT_HALF_SCALAR ? u + r / 2 : 2 * u + 1];
-      } else {
+      } else if (u < nt + U::loose(r)) {
         s0 = row[r + (u - nt)];
+      } else {
+        a = *reinterpret_cast<const uint4 *>(row + r + U::loose(r) + (u - nt - U::loose(r)) * U::V);
       }
     }
   }
-  __device__ __forceinline__ void store(T *out, int u, int r, const float2 *tab) const {
+  template <typename Table>
+  __device__ __forceinline__ void store(T *out, int u, int r, const Table &tab) const {
     const int nt = U::turned(r);
     if constexpr (MODE == ROT_HALF) {
       if (u < nt) {
@@ -99,7 +113,7 @@ struct RotUnit {
         y.unpack(b);
 #pragma unroll
         for (int e = 0; e < U::V; e += 2) {
-          const float4 cs = *reinterpret_cast<const float4 *>(tab + ((e >> 1) * nt + u) * 2);
+          const float4 cs = tab.two(u, e >> 1);
           const float x0 = x.f[e], y0 = y.f[e], x1 = x.f[e + 1], y1 = y.f[e + 1];
           x.f[e] = fmaf(x0, cs.x, -y0 * cs.y);
           y.f[e] = fmaf(y0, cs.x, x0 * cs.y);
@@ -116,11 +130,13 @@ struct RotUnit {
         Piece<T> x;
         x.unpack(a);
 #pragma unroll
-        for (int e = 0; e < U::PV; ++e) {
-          const float2 cs = tab[((e >> 1) * nt + u) * 2 + (e & 1)];
-          const float x0 = x.f[2 * e], x1 = x.f[2 * e + 1];
+        for (int e = 0; e < U::PV; e += 2) {
+          const float4 cs = tab.two(u, e >> 1);
+          const float x0 = x.f[2 * e], x1 = x.f[2 * e + 1], x2 = x.f[2 * e + 2], x3 = x.f[2 * e + 3];
           x.f[2 * e] = fmaf(x0, cs.x, -x1 * cs.y);
           x.f[2 * e + 1] = fmaf(x1, cs.x, x0 * cs.y);
+          x.f[2 * e + 2] = fmaf(x2, cs.z, -x3 * cs.w);
+          x.f[2 * e + 3] = fmaf(x3, cs.z, x2 * cs.w);
         }
         *reinterpret_cast<uint4 *>(out + u * U::V) = x.pack();
       } else {
@@ -128,12 +144,14 @@ struct RotUnit {
       }
     } else {
       if (u < nt) {
-        const float2 cs = tab[u];
+        const float2 cs = tab.one(u);
         const float x0 = to_f32<T>(s0), x1 = to_f32<T>(s1);
         out[MODE == ROT_HALF_SCALAR ? u : 2 * u] = from_f32<T>(fmaf(x0, cs.x, -x1 * cs.y));
         out[MODE == ROT_HALF_SCALAR ? u + r / 2 : 2 * u + 1] = from_f32<T>(fmaf(x1, cs.x, x0 * cs.y));
-      } else {
+      } else if (u < nt + U::loose(r)) {
         out[r + (u - nt)] = s0;
+      } else {
+        *reinterpret_cast<uint4 *>(out + r + U::loose(r) + (u - nt - U::loose(r)) * U::V) = a;
       }
     }
   }
