@@ -200,6 +200,17 @@ def dtype_code(dtype) -> int:
         raise TypeError(f"kitty_b200 supports float16, bfloat16 and float32 tensors, got {dtype}") from None
 
 
+def empty(shape, dtype, device):
+    """torch.empty for a contiguous tensor by the way that costs least on the host."""
+    import torch
+
+    strides, n = [], 1
+    for d in reversed(shape):
+        strides.append(n)
+        n *= d if d > 1 else 1
+    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=device)
+
+
 def call_on(device, fn, where: str, *args) -> None:
     """Call an entry point with the current stream of `device` (a CUDA device with an index) as its last argument and
     that device current, and raise if it refuses.  A small call costs more on the host than on the device, so the device

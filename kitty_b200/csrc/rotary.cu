@@ -21,8 +21,8 @@ struct RotArgs {
 
 constexpr int ROT_TOK = 8;         // tokens of a block's table
 
-// LPR threads per head row; each thread keeps ROWS rows in flight.
-template <typename T, int MODE, int LPR, int ROWS>
+// LPR threads per head row, UPT units of a row per thread; each thread keeps ROWS rows in flight.
+template <typename T, int MODE, int LPR, int UPT, int ROWS>
 __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotArgs a) {
   using U = RotUnits<T, MODE>;
   __shared__ __align__(16) float2 tab[ROT_TOK][HD / 2];
@@ -50,36 +50,42 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
   }
   __syncthreads();
   for (int base = row0; base < rows; base += STEP * ROWS) {
-    for (int u = lane; u < nu; u += LPR) {
-      RotUnit<T, MODE> x[ROWS];
-      const T *src;
-      T *dst[ROWS];
-      int tok[ROWS];
+    RotUnit<T, MODE> x[ROWS][UPT];
+    T *dst[ROWS];
+    int tok[ROWS];
+    for (int u0 = lane; u0 < nu; u0 += LPR * UPT) {            // one pass, but for the scalar modes
 #pragma unroll
       for (int j = 0; j < ROWS; ++j)
         if (base + j * STEP < rows) {
+          const T *src;
           locate(base + j * STEP, src, dst[j], tok[j]);
-          x[j].load(src, u, r);
+#pragma unroll
+          for (int k = 0; k < UPT; ++k)
+            if (u0 + k * LPR < nu) x[j][k].load(src, u0 + k * LPR, r);
         }
 #pragma unroll
       for (int j = 0; j < ROWS; ++j)
-        if (base + j * STEP < rows) x[j].store(dst[j], u, r, RotTable<T, MODE>{tab[tok[j]], nt});
+        if (base + j * STEP < rows) {
+#pragma unroll
+          for (int k = 0; k < UPT; ++k)
+            if (u0 + k * LPR < nu) x[j][k].store(dst[j], u0 + k * LPR, r, RotTable<T, MODE>{tab[tok[j]], nt});
+        }
     }
   }
 }
 
 template <typename T>
 int launch_rotary(const RotArgs &a, dim3 grid, cudaStream_t s) {
+  constexpr int LPR = sizeof(T) == 2 ? 8 : 16;
   switch (rot_mode(a.pl, sizeof(T))) {
-    case ROT_HALF: {
+    case ROT_HALF:
       // units of a full-width head: 8 (16 bit) or 16 (32 bit); a partly rotated head has up to twice as many
-      if (sizeof(T) == 2 && a.pl.rotary_dim == HD) rotary_kernel<T, ROT_HALF, 8, 2><<<grid, 256, 0, s>>>(a);
-      else rotary_kernel<T, ROT_HALF, 16, 2><<<grid, 256, 0, s>>>(a);
+      if (a.pl.rotary_dim == HD) rotary_kernel<T, ROT_HALF, LPR, 1, 2><<<grid, 256, 0, s>>>(a);
+      else rotary_kernel<T, ROT_HALF, LPR, 2, 2><<<grid, 256, 0, s>>>(a);
       break;
-    }
-    case ROT_INTER: rotary_kernel<T, ROT_INTER, 16, 2><<<grid, 256, 0, s>>>(a); break;
-    case ROT_HALF_SCALAR: rotary_kernel<T, ROT_HALF_SCALAR, 32, 4><<<grid, 256, 0, s>>>(a); break;
-    default: rotary_kernel<T, ROT_INTER_SCALAR, 32, 4><<<grid, 256, 0, s>>>(a); break;
+    case ROT_INTER: rotary_kernel<T, ROT_INTER, LPR, 2, 2><<<grid, 256, 0, s>>>(a); break;
+    case ROT_HALF_SCALAR: rotary_kernel<T, ROT_HALF_SCALAR, 16, 2, 2><<<grid, 256, 0, s>>>(a); break;
+    default: rotary_kernel<T, ROT_INTER_SCALAR, 16, 2, 2><<<grid, 256, 0, s>>>(a); break;
   }
   return cudaGetLastError() == cudaSuccess ? KITTY_OK : KITTY_E_CUDA;
 }

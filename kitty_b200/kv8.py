@@ -157,7 +157,7 @@ def kv8_append(layer: KV8Layer, key: torch.Tensor, value: torch.Tensor, start: t
             raise ValueError(f"expected query [{B}, H_Q, {T}, {layer.D}], got {tuple(query.shape)}")
         h_q = query.shape[1]
         query = _tokens(query, "query", h_q, layer)
-        out = torch.empty((B, h_q, T, layer.D), dtype=layer.dtype, device=layer.device)
+        out = _lib.empty((B, h_q, T, layer.D), layer.dtype, layer.device)
         strides += _head_strides(query)
     else:
         strides += (0, 0, 0)
@@ -182,8 +182,8 @@ def kv8_expand(layer: KV8Layer, lengths: torch.Tensor, n: int, *, start: Optiona
     lengths = _row_tensor(lengths, "lengths", B, layer)
     if start is not None:
         start = _row_tensor(start, "start", B, layer)
-    k = torch.empty((B, layer.H_KV, n, layer.D), dtype=layer.dtype, device=layer.device)
-    v = torch.empty_like(k)
+    shape = (B, layer.H_KV, n, layer.D)
+    k, v = _lib.empty(shape, layer.dtype, layer.device), _lib.empty(shape, layer.dtype, layer.device)
     _lib.call_on(layer.device, _lib.lib().kitty_kv8_expand, "kitty_kv8_expand", layer.c_layer(), lengths.data_ptr(),
                  None if start is None else start.data_ptr(), k.data_ptr(), v.data_ptr(), B, n)
     return k, v
@@ -206,11 +206,11 @@ def kv8_attention(query: torch.Tensor, layer: KV8Layer, lengths: torch.Tensor, s
     lengths = _row_tensor(lengths, "lengths", B, layer)
     need = layer.workspace_bytes(B, h_q)
     if out is None:
-        out = torch.empty((B, 1, h_q, D), dtype=layer.dtype, device=layer.device)
+        out = _lib.empty((B, 1, h_q, D), layer.dtype, layer.device)
     elif tuple(out.shape) != (B, 1, h_q, D) or out.dtype != layer.dtype or out.device != layer.device \
             or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {layer.dtype} [{B}, 1, {h_q}, {D}] on {layer.device}")
-    ws = torch.empty(need, dtype=torch.uint8, device=layer.device)
+    ws = _lib.empty((need,), torch.uint8, layer.device)
     _lib.call_on(layer.device, _lib.lib().kitty_kv8_attn, "kitty_kv8_attn", layer.c_layer(), lengths.data_ptr(),
                  q.data_ptr(), B, h_q, float(scaling), out.data_ptr(), ws.data_ptr(), need)
     return out

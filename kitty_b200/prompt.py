@@ -6,6 +6,7 @@ batches of different lengths.  `decode_attention` and `kv8_attention` take over 
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
@@ -21,6 +22,15 @@ def _status_word(device: torch.device) -> torch.Tensor:
     if st is None:
         st = _status[device] = torch.zeros(1, dtype=torch.int32, device=device)
     return st
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_need(device, B: int, Lq: int, Lk: int, h_q: int, h_kv: int, causal: bool, packed: bool) -> int:
+    with torch.cuda.device(device):                     # the plan depends on the device's multiprocessors
+        need = _lib.lib().kitty_prompt_workspace_bytes(B, Lq, Lk, h_q, h_kv, int(causal), int(packed))
+    if need < 0:
+        _lib.check(int(need), "kitty_prompt_workspace_bytes")
+    return int(need)
 
 
 def prompt_attention_status(device="cuda") -> int:
@@ -114,15 +124,12 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
         shape = (B, Lq, h_q, HEAD_DIM)
     zero_rest = out is None
     if out is None:
-        out = torch.empty(shape, dtype=query.dtype, device=dev)
+        out = _lib.empty(shape, query.dtype, dev)
     elif tuple(out.shape) != shape or out.dtype != query.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {query.dtype} {list(shape)} on {dev}")
-    lib = _lib.lib()
-    need = lib.kitty_prompt_workspace_bytes(B, Lq, Lk, h_q, h_kv, int(causal), int(packed))
-    if need < 0:
-        _lib.check(int(need), "kitty_prompt_workspace_bytes")
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _lib.call_on(dev, lib.kitty_prompt_attn, "kitty_prompt_attn", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+    need = _workspace_need(dev, B, Lq, Lk, h_q, h_kv, bool(causal), packed)
+    ws = _lib.empty((need,), torch.uint8, dev) if need else None
+    _lib.call_on(dev, _lib.lib().kitty_prompt_attn, "kitty_prompt_attn", q.data_ptr(), k.data_ptr(), v.data_ptr(),
                  _lib.dtype_code(q.dtype), _lib.i64_array(q_st + k_st + v_st), B, Lq, Lk, h_q, h_kv, float(scaling),
                  int(causal), *(None if x is None else x.data_ptr() for x in (q_len, k_len, cu_q, cu_k)), out.data_ptr(),
                  int(zero_rest), _status_word(dev).data_ptr(), None if ws is None else ws.data_ptr(), need)
