@@ -46,7 +46,7 @@ struct PromptArgs {
   float *part;                                 // splits > 1: [splits][rows][h_q][128] accumulators,
   float2 *part_ml;                             // [splits][rows][h_q] (maximum in base 2, sum; sum -1: sees nothing)
   int64_t rows;                                // output rows of one head
-  int32_t B, Lq, Lk, G, h_kv, pairs, causal, zero_rest, splits;
+  int32_t B, Lq, Lk, G, h_kv, pairs, causal, zero_rest, splits, items;
   float c;                                     // scaling * log2 e
 };
 
@@ -107,8 +107,9 @@ __device__ __forceinline__ uint32_t pack2(uint64_t p) {
   }
 }
 
-// Weights of 64 logits, 2^(v c - mc), as 16-bit pairs; returns their sum.  POLY: every fourth pair goes through the
-// polynomial, which takes a quarter of the load off the 16-a-clock exponential unit (for finite logits only).
+// Weights of 64 logits, 2^(v c - mc), as 16-bit pairs; returns their sum.  POLY: every eighth pair goes through the
+// polynomial, which takes some of the load off the 16-a-clock exponential unit (for finite logits only): 1.36 PFLOP/s
+// over long unmasked rows; with none, a quarter or three eighths of them 1.35, 1.30 and 1.28.
 template <typename T, bool POLY>
 __device__ __forceinline__ uint64_t weights64(const float *v, uint64_t c2, uint64_t nmc2, uint32_t (&w)[32]) {
   uint64_t sum[2] = {0, 0};
@@ -116,7 +117,7 @@ __device__ __forceinline__ uint64_t weights64(const float *v, uint64_t c2, uint6
   for (int i = 0; i < 32; ++i) {
     const uint64_t x = fma2(pk2(v[2 * i], v[2 * i + 1]), c2, nmc2);
     uint64_t p;
-    if (POLY && (i & 3) == 3) {
+    if (POLY && (i & 7) == 7) {
       p = ex2_poly2(x);
     } else {
       const float2 f = un2(x);
@@ -194,45 +195,77 @@ __device__ __noinline__ void repair_row(const PromptArgs &a, const Seq &s, int r
   *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + at * HD + 4 * lane) = *reinterpret_cast<const uint2 *>(o);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(PROMPT_THREADS, 1)
-    prompt_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-                       const __grid_constant__ CUtensorMap mv, const __grid_constant__ PromptArgs a) {
-  constexpr bool BF16 = __is_same(T, __nv_bfloat16);
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bar_q, bar_full[KV_STAGES], bar_empty[KV_STAGES], bar_s[2], bar_p[2][2], bar_o[2], bar_end;
-  __shared__ uint32_t tmem_base;
-  __shared__ int item_seq, item_pair;
-  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
-
-  // ---- which sequence, key head and pair of tiles
+// One piece of work of a block: a pair of query tiles of one key head against its key tiles (or the z-th part of them).
+struct Item {
   Seq s;
-  int h, pair;
-  const int z = blockIdx.x % a.splits, item = blockIdx.x / a.splits;      // neighbours share query tiles
+  int h, pair, z;
+  int j0, n;          // first key tile and their number
+  int nb[2];          // how many of them each tile sees
+  int more;           // 0: there is no further item
+};
+
+// Row tile and head of query tile x of an item; the key tiles that its last row sees (0: none, or no such tile).
+__device__ __forceinline__ int tile_of(const PromptArgs &a, const Seq &s, int h, int pair, int x, int &row0, int &head) {
+  const int f = 2 * pair + x;
+  row0 = f / a.G * PT;
+  head = h * a.G + f % a.G;
+  const int last = min(row0 + PT, s.nq) - 1;
+  return f < (s.rows + PT - 1) / PT * a.G && last >= row0 ? (key_limit(s, last, a.causal) + PT - 1) / PT : 0;
+}
+
+// Rows of packed sequence i (i = a.B: the rows behind the last sequence).
+__device__ __forceinline__ void packed_rows(const PromptArgs &a, int i, int &lo, int &hi) {
+  lo = clampi(a.cu_q[i], 0, a.Lq);
+  hi = i < a.B ? clampi(a.cu_q[i + 1], lo, a.Lq) : a.Lq;
+}
+__device__ __forceinline__ int packed_pairs(const PromptArgs &a, int i) {
+  int lo, hi;
+  packed_rows(a, i, lo, hi);
+  return ((hi - lo + PT - 1) / PT * a.G + 1) / 2;
+}
+
+// Work item number `id` (by one warp); false when the packed sequences have no such item.
+__device__ __forceinline__ bool find_item(const PromptArgs &a, int id, Item &w) {
+  const int lane = threadIdx.x & 31;
+  w.z = id % a.splits;
+  id /= a.splits;
+  Seq &s = w.s;
   if (a.cu_q == nullptr) {
-    const int sh = item % (a.B * a.h_kv);
-    pair = a.pairs - 1 - item / (a.B * a.h_kv);      // the longest rows first
+    const int sh = id % (a.B * a.h_kv);
+    w.pair = a.pairs - 1 - id / (a.B * a.h_kv);             // the longest rows first
     s.b = sh / a.h_kv;
-    h = sh % a.h_kv;
+    w.h = sh % a.h_kv;
     s.q0 = s.k0 = 0;
     s.nq = a.q_lens != nullptr ? clampi(a.q_lens[s.b], 0, a.Lq) : a.Lq;
     s.nk = a.k_lens != nullptr ? clampi(a.k_lens[s.b], 0, a.Lk) : a.Lk;
     s.rows = a.Lq;
     s.out0 = static_cast<int64_t>(s.b) * a.Lq;
   } else {
-    h = item % a.h_kv;
-    const int want = item / a.h_kv;
-    if (warp == 0) {
-      const int nseq = a.B + (a.zero_rest ? 1 : 0);
-      int base = 0, found = -1, fp = 0;
-      for (int i0 = 0; i0 < nseq && found < 0; i0 += 32) {
-        const int i = i0 + lane;
-        int np = 0;
-        if (i < nseq) {
-          const int lo = clampi(a.cu_q[i], 0, a.Lq), hi = i < a.B ? clampi(a.cu_q[i + 1], lo, a.Lq) : a.Lq;
-          np = ((hi - lo + PT - 1) / PT * a.G + 1) / 2;
-        }
+    w.h = id % a.h_kv;
+    const int want = id / a.h_kv, nseq = a.B + (a.zero_rest ? 1 : 0);
+    int seq = -1;
+    if (nseq <= 64) {
+      // The longest rows of all sequences first.  level(p) = pairs with number p or above, over all sequences; the item
+      // is one of those with the largest p for which level(p) is above its own number.
+      const int n0 = lane < nseq ? packed_pairs(a, lane) : 0, n1 = lane + 32 < nseq ? packed_pairs(a, lane + 32) : 0;
+      auto level = [&](int p) { return __reduce_add_sync(0xffffffffu, max(n0 - p, 0) + max(n1 - p, 0)); };
+      if (level(0) <= want) return false;
+      int lo = 0, hi = __reduce_max_sync(0xffffffffu, max(n0, n1));      // level(lo) > want >= level(hi)
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (level(mid) > want) lo = mid;
+        else hi = mid;
+      }
+      const int r = want - level(hi);                       // the r-th sequence that has a pair lo
+      const unsigned b0 = __ballot_sync(0xffffffffu, n0 > lo), b1 = __ballot_sync(0xffffffffu, n1 > lo);
+      const int c0 = __popc(b0);
+      seq = r < c0 ? static_cast<int>(__fns(b0, 0, r + 1)) : 32 + static_cast<int>(__fns(b1, 0, r - c0 + 1));
+      w.pair = lo;
+    } else {
+      // many sequences: one after the other
+      int base = 0;
+      for (int i0 = 0; i0 < nseq && seq < 0; i0 += 32) {
+        const int np = i0 + lane < nseq ? packed_pairs(a, i0 + lane) : 0;
         int inc = np;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -243,350 +276,421 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         if (hit) {
           const int l = __ffs(hit) - 1;
           const int upto = __shfl_sync(0xffffffffu, inc, l), n1 = __shfl_sync(0xffffffffu, np, l);
-          found = i0 + l;
-          fp = n1 - 1 - (want - (base + upto - n1));       // the longest rows first
+          seq = i0 + l;
+          w.pair = n1 - 1 - (want - (base + upto - n1));
         }
         base += __shfl_sync(0xffffffffu, inc, 31);
       }
-      if (lane == 0) item_seq = found, item_pair = fp;
+      if (seq < 0) return false;
     }
-    __syncthreads();
-    const int i = item_seq;
-    if (i < 0) return;                                      // the grid covers the most that Lq rows can need
-    pair = item_pair;
     s.b = 0;
-    s.q0 = clampi(a.cu_q[i], 0, a.Lq);
-    s.nq = (i < a.B ? clampi(a.cu_q[i + 1], s.q0, a.Lq) : a.Lq) - s.q0;
+    int hi;
+    packed_rows(a, seq, s.q0, hi);
+    s.nq = hi - s.q0;
     s.k0 = s.nk = 0;
-    if (i < a.B) {
+    if (seq < a.B) {
       const int32_t *cu = a.cu_k != nullptr ? a.cu_k : a.cu_q;
-      s.k0 = clampi(cu[i], 0, a.Lk);
-      s.nk = clampi(cu[i + 1], s.k0, a.Lk) - s.k0;
+      s.k0 = clampi(cu[seq], 0, a.Lk);
+      s.nk = clampi(cu[seq + 1], s.k0, a.Lk) - s.k0;
     }
     s.rows = s.nq;
     s.out0 = s.q0;
   }
-  const int tiles = (s.rows + PT - 1) / PT * a.G;           // (row tile, head) pairs of the key head
-  // row tile, head and key tiles of the block's query tile x
-  auto tile = [&](int x, int &row0, int &head) {
-    const int f = 2 * pair + x;
-    row0 = f / a.G * PT;
-    head = h * a.G + f % a.G;
-    const int last = min(row0 + PT, s.nq) - 1;
-    return f < tiles && last >= row0 ? (key_limit(s, last, a.causal) + PT - 1) / PT : 0;
-  };
-  int r_, h_;
-  const int all0 = tile(0, r_, h_), all1 = tile(1, r_, h_);
-  // this block's key tiles: all of them, or the z-th part
+  int row0, head;
+  const int all0 = tile_of(a, s, w.h, w.pair, 0, row0, head), all1 = tile_of(a, s, w.h, w.pair, 1, row0, head);
   const int most = max(all0, all1);
-  const int j0 = static_cast<int>(static_cast<int64_t>(most) * z / a.splits);
-  const int n = static_cast<int>(static_cast<int64_t>(most) * (z + 1) / a.splits) - j0;
-  const int nb0 = min(max(all0 - j0, 0), n), nb1 = min(max(all1 - j0, 0), n);
+  w.j0 = static_cast<int>(static_cast<int64_t>(most) * w.z / a.splits);
+  w.n = static_cast<int>(static_cast<int64_t>(most) * (w.z + 1) / a.splits) - w.j0;
+  w.nb[0] = min(max(all0 - w.j0, 0), w.n);
+  w.nb[1] = min(max(all1 - w.j0, 0), w.n);
+  w.more = 1;
+  return true;
+}
 
-  if (n > 0) {
-    if (warp == 9) tmem_alloc(smem_u32(&tmem_base), 512);
-    if (threadIdx.x == 0) {
-      mbar_init(smem_u32(&bar_q), 1);
-      for (int i = 0; i < KV_STAGES; ++i) mbar_init(smem_u32(&bar_full[i]), 1), mbar_init(smem_u32(&bar_empty[i]), 1);
-      for (int x = 0; x < 2; ++x) {
-        mbar_init(smem_u32(&bar_s[x]), 1);
-        mbar_init(smem_u32(&bar_p[x][0]), 4);
-        mbar_init(smem_u32(&bar_p[x][1]), 4);
-        mbar_init(smem_u32(&bar_o[x]), 1);
-      }
-      mbar_init(smem_u32(&bar_end), 1);
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+template <typename T>
+__global__ void __launch_bounds__(PROMPT_THREADS, 1)
+    prompt_attn_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                       const __grid_constant__ CUtensorMap mv, const __grid_constant__ PromptArgs a) {
+  constexpr bool BF16 = __is_same(T, __nv_bfloat16);
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bar_q, bar_q_free, bar_full[KV_STAGES], bar_empty[KV_STAGES], bar_s[2], bar_p[2][2], bar_o[2],
+      bar_item[2], bar_item_free[2], bar_end;
+  __shared__ uint32_t tmem_base;
+  __shared__ Item items[2];
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  if (warp == 9) tmem_alloc(smem_u32(&tmem_base), 512);
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&bar_q), 1);
+    mbar_init(smem_u32(&bar_q_free), 1);
+    for (int i = 0; i < KV_STAGES; ++i) mbar_init(smem_u32(&bar_full[i]), 1), mbar_init(smem_u32(&bar_empty[i]), 1);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(smem_u32(&bar_s[x]), 1);
+      mbar_init(smem_u32(&bar_p[x][0]), 4);
+      mbar_init(smem_u32(&bar_p[x][1]), 4);
+      mbar_init(smem_u32(&bar_o[x]), 1);
+      mbar_init(smem_u32(&bar_item[x]), 1);
+      mbar_init(smem_u32(&bar_item_free[x]), 9);            // the issuing warp and eight softmax warps
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
+    mbar_init(smem_u32(&bar_end), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  const uint32_t tmem = n > 0 ? tmem_base : 0;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
   const uint32_t q_addr = smem, kv_addr = smem + 2 * TILE_BYTES;
   auto give_up = [&] {
     if (a.status != nullptr) atomicExch(a.status, 1);
+  };
+  // the c-th item of this block, as the copying warp has published it
+  auto next_item = [&](int c, Item &w) {
+    const bool ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_item[c & 1]), (c >> 1) & 1));
+    if (!ok) return false;
+    w = items[c & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&bar_item_free[c & 1]));
+    return w.more != 0;
   };
 
   // 384 threads start with 168 registers; the softmax threads take what the other group gives up (2 * 224 + 56 = 3 * 168)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 8) {
-      if (n > 0 && elect_one()) {
-        const uint32_t bq = smem_u32(&bar_q);
-        mbar_expect_tx(bq, (nb0 > 0 ? TILE_BYTES : 0) + (nb1 > 0 ? TILE_BYTES : 0));
-        for (int x = 0; x < 2; ++x) {
-          int row0, head;
-          tile(x, row0, head);
-          if ((x ? nb1 : nb0) > 0)
+      // ---- copies, and the list of items: items are numbered from the most work to the least, and the blocks take them
+      // in turn, there and back (first to last, last to first, ...), which leaves every block about the same
+      uint32_t pos = 0;                                     // key and value tiles requested so far
+      int published = 0, loaded = 0;
+      bool ok = true;
+      auto publish = [&](const Item &w) {
+        const int c = published++;
+        if (c >= 2) ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_item_free[c & 1]), ((c >> 1) - 1) & 1));
+        if (ok && lane == 0) {
+          items[c & 1] = w;
+          mbar_arrive(smem_u32(&bar_item[c & 1]));
+        }
+        __syncwarp();
+      };
+      for (int k = 0; ok && static_cast<int64_t>(k) * gridDim.x < a.items; ++k) {
+        const int id = k * gridDim.x + (k & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        Item w;
+        if (id >= a.items || !find_item(a, id, w)) continue;
+        publish(w);
+        if (!ok || w.n == 0) continue;
+        if (elect_one()) {
+          // the query tiles' place is free when the last logits of the item before are complete
+          if (loaded > 0) ok = mbar_wait_asleep(smem_u32(&bar_q_free), (loaded - 1) & 1);
+          if (ok) {
+            const uint32_t bq = smem_u32(&bar_q);
+            mbar_expect_tx(bq, (w.nb[0] > 0 ? TILE_BYTES : 0) + (w.nb[1] > 0 ? TILE_BYTES : 0));
+            for (int x = 0; x < 2; ++x) {
+              int row0, head;
+              tile_of(a, w.s, w.h, w.pair, x, row0, head);
+              if (w.nb[x] > 0)
+                for (int c = 0; c < 2; ++c)
+                  tma_load_4d(q_addr + x * TILE_BYTES + c * (TILE_BYTES / 2), &mq, bq, 64 * c, w.s.q0 + row0, head, w.s.b);
+            }
+          }
+          uint32_t at = pos;
+          for (int i = 0; i < 2 * w.n && ok; ++i, ++at) {
+            const uint32_t st = at % KV_STAGES, round = at / KV_STAGES;
+            if (round > 0 && !mbar_wait_asleep(smem_u32(&bar_empty[st]), (round - 1) & 1)) {
+              ok = false;
+              break;
+            }
+            const uint32_t bf = smem_u32(&bar_full[st]);
+            mbar_expect_tx(bf, TILE_BYTES);
+            const CUtensorMap *m = (i & 1) ? &mv : &mk;
             for (int c = 0; c < 2; ++c)
-              tma_load_4d(q_addr + x * TILE_BYTES + c * (TILE_BYTES / 2), &mq, bq, 64 * c, s.q0 + row0, head, s.b);
-        }
-        int i = 0;
-        bool ok = true;
-        for (; i < 2 * n; ++i) {
-          const int st = i % KV_STAGES, round = i / KV_STAGES;
-          if (round > 0 && !mbar_wait_asleep(smem_u32(&bar_empty[st]), (round - 1) & 1)) {
+              tma_load_4d(kv_addr + st * TILE_BYTES + c * (TILE_BYTES / 2), m, bf, 64 * c, w.s.k0 + (w.j0 + (i >> 1)) * PT, w.h, w.s.b);
+          }
+          if (!ok) {                                        // leave no copy in flight behind
             give_up();
-            ok = false;
-            break;
+            mbar_wait_asleep(smem_u32(&bar_q), loaded & 1);
+            for (uint32_t j = at > KV_STAGES ? at - KV_STAGES : 0; j < at; ++j)
+              mbar_wait_asleep(smem_u32(&bar_full[j % KV_STAGES]), (j / KV_STAGES) & 1);
           }
-          const uint32_t bf = smem_u32(&bar_full[st]);
-          mbar_expect_tx(bf, TILE_BYTES);
-          const CUtensorMap *m = (i & 1) ? &mv : &mk;
-          for (int c = 0; c < 2; ++c)
-            tma_load_4d(kv_addr + st * TILE_BYTES + c * (TILE_BYTES / 2), m, bf, 64 * c, s.k0 + (j0 + (i >> 1)) * PT, h, s.b);
         }
-        if (!ok)                                              // leave no copy in flight behind
-          for (int j = max(0, i - KV_STAGES); j < i; ++j) mbar_wait_asleep(smem_u32(&bar_full[j % KV_STAGES]), (j / KV_STAGES) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        pos += 2 * w.n;
+        ++loaded;
       }
+      Item end{};
+      if (ok) publish(end);
     } else if (warp == 9) {
-      if (n > 0 && elect_one()) {
-        // This thread's instructions are the pace of the block: a straight line of them would miss the instruction cache at
-        // every step (the softmax code fills it), so everything is in short loops.
-        constexpr uint32_t ID_S = umma_idesc(BF16, PT, PT, false), ID_O = umma_idesc(BF16, PT, HD, true);
-        constexpr uint32_t STAGE = TILE_BYTES >> 4;             // in units of a descriptor's address
-        const uint32_t full = smem_u32(&bar_full[0]), empty = smem_u32(&bar_empty[0]);
-        const uint32_t ready = smem_u32(&bar_s[0]), weights = smem_u32(&bar_p[0][0]), done = smem_u32(&bar_o[0]);
-        const uint32_t q_lo = umma_lo(q_addr, 16), k_lo = umma_lo(kv_addr, 16), v_lo = umma_lo(kv_addr, TILE_BYTES / 2);
-        uint32_t st = 0, ph = 0;                                // ring position of the next tile
-        bool ok = true;
-        auto wait = [&](uint32_t bar, uint32_t parity) {
-          ok = ok && mbar_wait_asleep(bar, parity);
-          tc_fence_after();
-          return ok;
-        };
-        auto advance = [&] {
-          if (++st == KV_STAGES) st = 0, ph ^= 1;
-        };
-        // logits of tile x: contraction over 128 channels, 16 at a time, two swizzled halves
-        auto logits = [&](uint32_t x, uint32_t stage) {
-          uint32_t ql = q_lo + x * STAGE, kl = k_lo + stage * STAGE;
+      // ---- products.  The issuing thread's instructions are the pace of the block: a straight line of them would miss the
+      // instruction cache at every step (the softmax code fills it), so everything is in short loops.
+      constexpr uint32_t ID_S = umma_idesc(BF16, PT, PT, false), ID_O = umma_idesc(BF16, PT, HD, true);
+      constexpr uint32_t STAGE = TILE_BYTES >> 4;             // in units of a descriptor's address
+      const uint32_t full = smem_u32(&bar_full[0]), empty = smem_u32(&bar_empty[0]);
+      const uint32_t ready = smem_u32(&bar_s[0]), weights = smem_u32(&bar_p[0][0]), done = smem_u32(&bar_o[0]);
+      const uint32_t q_lo = umma_lo(q_addr, 16), k_lo = umma_lo(kv_addr, 16), v_lo = umma_lo(kv_addr, TILE_BYTES / 2);
+      uint32_t pos = 0, step0 = 0, step1 = 0;               // tiles read; weights of either query tile taken, so far
+      int loaded = 0;
+      bool ok = true;
+      Item w;
+      for (int c = 0; ok && next_item(c, w); ++c) {
+        if (w.n == 0) continue;
+        const int n = w.n, nb0 = w.nb[0], nb1 = w.nb[1];
+        if (elect_one()) {
+          uint32_t st = pos % KV_STAGES, ph = pos / KV_STAGES & 1;      // ring position of the next tile
+          auto wait = [&](uint32_t bar, uint32_t parity) {
+            ok = ok && mbar_wait_asleep(bar, parity);
+            tc_fence_after();
+            return ok;
+          };
+          auto advance = [&] {
+            if (++st == KV_STAGES) st = 0, ph ^= 1;
+          };
+          // logits of tile x: contraction over 128 channels, 16 at a time, two swizzled halves
+          auto logits = [&](uint32_t x, uint32_t stage) {
+            uint32_t ql = q_lo + x * STAGE, kl = k_lo + stage * STAGE;
 #pragma unroll 1
-          for (int c = 0; c < 2; ++c) {
+            for (int y = 0; y < 2; ++y) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_ss(tmem + x * PT, ql + 2 * k, umma_hi(1024), kl + 2 * k, umma_hi(1024), ID_S, (c | k) != 0);
-            ql += STAGE / 2;
-            kl += STAGE / 2;
+              for (int k = 0; k < 4; ++k)
+                umma_ss(tmem + x * PT, ql + 2 * k, umma_hi(1024), kl + 2 * k, umma_hi(1024), ID_S, (y | k) != 0);
+              ql += STAGE / 2;
+              kl += STAGE / 2;
+            }
+            umma_commit(ready + 8 * x);
+          };
+          wait(smem_u32(&bar_q), loaded & 1);
+          if (wait(full + 8 * st, ph)) {
+#pragma unroll 1
+            for (int x = 0; x < 2; ++x)
+              if ((x ? nb1 : nb0) > 0) logits(x, st);
+            umma_commit(empty + 8 * st);
+            if (n == 1) umma_commit(smem_u32(&bar_q_free));
+            advance();
           }
-          umma_commit(ready + 8 * x);
-        };
-        wait(smem_u32(&bar_q), 0);
-        if (wait(full, 0)) {
 #pragma unroll 1
-          for (int x = 0; x < 2; ++x)
-            if ((x ? nb1 : nb0) > 0) logits(x, 0);
-          umma_commit(empty);
-          advance();
-        }
+          for (int j = 0; j < n && ok; ++j) {
+            const uint32_t sv = st;
+            if (!wait(full + 8 * sv, ph)) break;
+            advance();
+            const bool more = j + 1 < n;
 #pragma unroll 1
-        for (int j = 0; j < n && ok; ++j) {
-          const uint32_t sv = st;
-          if (!wait(full + 8 * sv, ph)) break;
-          advance();
-          const bool more = j + 1 < n;
+            for (int x = 0; x < 2 && ok; ++x) {
+              const int nb = x ? nb1 : nb0;
+              if (j < nb) {
+                // accumulator of tile x += weights x value tile j: contraction over 128 keys, 16 at a time
+                uint32_t vl = v_lo + sv * STAGE, pa = tmem + x * PT;
+                uint32_t bar = weights + 16 * x;
+                const uint32_t parity = ((x ? step1 : step0) + j) & 1;
 #pragma unroll 1
-          for (int x = 0; x < 2 && ok; ++x) {
-            const int nb = x ? nb1 : nb0;
-            if (j < nb) {
-              // accumulator of tile x += weights x value tile j: contraction over 128 keys, 16 at a time
-              uint32_t vl = v_lo + sv * STAGE, pa = tmem + x * PT;
-              uint32_t bar = weights + 16 * x;
-#pragma unroll 1
-              for (int c = 0; c < 2; ++c) {
-                if (!wait(bar, j & 1)) break;
+                for (int y = 0; y < 2; ++y) {
+                  if (!wait(bar, parity)) break;
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  umma_ts(tmem + 2 * PT + x * HD, pa + 8 * k, vl + (2048 >> 4) * k, umma_hi(1024), ID_O, (j | c | k) != 0);
-                vl += 4 * (2048 >> 4);
-                pa += 32;
-                bar += 8;
+                  for (int k = 0; k < 4; ++k)
+                    umma_ts(tmem + 2 * PT + x * HD, pa + 8 * k, vl + (2048 >> 4) * k, umma_hi(1024), ID_O, (j | y | k) != 0);
+                  vl += 4 * (2048 >> 4);
+                  pa += 32;
+                  bar += 8;
+                }
+                if (!ok) break;
+                if (j + 1 == nb) umma_commit(done + 8 * x);
               }
-              if (!ok) break;
-              if (j + 1 == nb) umma_commit(done + 8 * x);
+              if (x == 1) umma_commit(empty + 8 * sv);
+              if (more) {
+                if (x == 0 && !wait(full + 8 * st, ph)) break;
+                if (j + 1 < nb) logits(x, st);
+                if (x == 1) {
+                  umma_commit(empty + 8 * st);
+                  if (j + 2 == n) umma_commit(smem_u32(&bar_q_free));
+                }
+              }
             }
-            if (x == 1) umma_commit(empty + 8 * sv);
-            if (more) {
-              if (x == 0 && !wait(full + 8 * st, ph)) break;
-              if (j + 1 < nb) logits(x, st);
-              if (x == 1) umma_commit(empty + 8 * st);
-            }
+            if (more) advance();
           }
-          if (more) advance();
+          if (!ok) give_up();
         }
-        if (!ok) give_up();
-        // every product is complete before the tensor memory is given back
+        ok = __all_sync(0xffffffffu, ok);
+        pos += 2 * n;
+        step0 += nb0;
+        step1 += nb1;
+        ++loaded;
+      }
+      // every product is complete before the tensor memory is given back
+      if (elect_one()) {
         umma_commit(smem_u32(&bar_end));
         mbar_wait_asleep(smem_u32(&bar_end), 0);
       }
+      __syncwarp();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int x = warp >> 2;
     const uint32_t at = tmem + (static_cast<uint32_t>(warp & 3) << 21);     // the warp's 32 lanes
     const uint32_t ts = at + x * PT, to = at + 2 * PT + x * HD;
-    int row0, head;
-    tile(x, row0, head);
-    const bool live = 2 * pair + x < tiles;
-    const int row = row0 + (threadIdx.x & 127);
-    const int limit = key_limit(s, row, a.causal);
-    const int nb = x ? nb1 : nb0;
-    float m = -INFINITY, l = 0.0f;
-    bool ok = true;
-    // keys that every row of the tile sees need no comparison
-    const int all = key_limit(s, min(row0, s.nq - 1), a.causal);
     const uint64_t c2 = pk2(a.c, a.c);
-    for (int j = 0; j < nb; ++j) {
-      ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_s[x]), j & 1));
-      if (!ok) break;
-      tc_fence_after();
-      float v[PT];
-      tmem_ld32(ts, v);
-      tmem_ld32(ts + 32, v + 32);
-      tmem_wait_ld();
-      tmem_ld32(ts + 64, v + 64);
-      tmem_ld32(ts + 96, v + 96);
-      const bool masked = (j0 + j + 1) * PT > all;
-      const int seen = limit - (j0 + j) * PT;
-      float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      uint32_t w[32];
-      uint64_t sum = 0;
-      bool settled = false;
-      auto announce = [&](int half) {
-        tmem_st32(ts + 32 * half, w);
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&bar_p[x][half]));      // one arrival a warp: arrivals at one address queue up
-      };
-      auto largest = [&](int half) {
-#pragma unroll
-        for (int i = 64 * half; i < 64 * half + 64; i += 8) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) t[e] = max3(t[e], v[i + 2 * e], v[i + 2 * e + 1]);
-        }
-      };
-      if (j > 0 && !masked) {
-        // The maximum so far is mostly the one to use: the first weights are taken with it while the tile's own maximum
-        // is found, and count if no row has outgrown it (nor met a NaN, which this comparison does not pass).
-        const uint64_t nmc2 = pk2(-m * a.c, -m * a.c);
-        sum = weights64<T, true>(v, c2, nmc2, w);
-        largest(0);
+    uint32_t step = 0, outs = 0;             // tiles of logits and accumulators taken so far
+    bool ok = true;
+    Item w_;
+    for (int count = 0; ok && next_item(count, w_); ++count) {
+      const Seq s = w_.s;
+      const int j0 = w_.j0, nb = x ? w_.nb[1] : w_.nb[0];
+      int row0, head;
+      tile_of(a, s, w_.h, w_.pair, x, row0, head);
+      const bool live = 2 * w_.pair + x < (s.rows + PT - 1) / PT * a.G;
+      const int z = w_.z;
+      const int row = row0 + (threadIdx.x & 127);
+      const int limit = key_limit(s, row, a.causal);
+      float m = -INFINITY, l = 0.0f;
+      // keys that every row of the tile sees need no comparison
+      const int all = key_limit(s, min(row0, s.nq - 1), a.causal);
+      for (int j = 0; j < nb; ++j) {
+        ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_s[x]), (step + j) & 1));
+        if (!ok) break;
+        tc_fence_after();
+        float v[PT];
+        tmem_ld32(ts, v);
+        tmem_ld32(ts + 32, v + 32);
         tmem_wait_ld();
-        largest(1);
-        const float top = max3(max3(t[0], t[1], t[2]), t[3], t[3]);
-        settled = __all_sync(0xffffffffu, (top - m) * a.c <= LAG);
-        if (settled) {
+        tmem_ld32(ts + 64, v + 64);
+        tmem_ld32(ts + 96, v + 96);
+        const bool masked = (j0 + j + 1) * PT > all;
+        const int seen = limit - (j0 + j) * PT;
+        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        uint32_t w[32];
+        uint64_t sum = 0;
+        bool settled = false;
+        auto announce = [&](int half) {
+          tmem_st32(ts + 32 * half, w);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&bar_p[x][half]));      // one arrival a warp: arrivals at one address queue up
+        };
+        auto largest = [&](int half) {
+#pragma unroll
+          for (int i = 64 * half; i < 64 * half + 64; i += 8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] = max3(t[e], v[i + 2 * e], v[i + 2 * e + 1]);
+          }
+        };
+        if (j > 0 && !masked) {
+          // The maximum so far is mostly the one to use: the first weights are taken with it while the tile's own maximum
+          // is found, and count if no row has outgrown it (nor met a NaN, which this comparison does not pass).
+          const uint64_t nmc2 = pk2(-m * a.c, -m * a.c);
+          sum = weights64<T, true>(v, c2, nmc2, w);
+          largest(0);
+          tmem_wait_ld();
+          largest(1);
+          const float top = max3(max3(t[0], t[1], t[2]), t[3], t[3]);
+          settled = __all_sync(0xffffffffu, (top - m) * a.c <= LAG);
+          if (settled) {
+            announce(0);
+            sum = add2(sum, weights64<T, true>(v + 64, c2, nmc2, w));
+            announce(1);
+          }
+        }
+        if (!settled) {
+          tmem_wait_ld();
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < PT; ++i) v[i] = i < seen ? v[i] : -INFINITY;
+          }
+          t[0] = t[1] = t[2] = t[3] = -INFINITY;
+          largest(0);
+          largest(1);
+          const float top = max3(max3(t[0], t[1], t[2]), t[3], t[3]);
+          const bool grow = (top - m) * a.c > LAG || m == -INFINITY;
+          if (j == 0) {
+            m = top;
+          } else if (__any_sync(0xffffffffu, grow)) {
+            const float mn = grow ? fmaxf(m, top) : m;
+            const float f = grow ? ex2((m - (mn == -INFINITY ? 0.0f : mn)) * a.c) : 1.0f;
+            m = mn;
+            l *= f;
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+              float o[32];
+              tmem_ld32(to + 32 * i, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] *= f;
+              tmem_st32(to + 32 * i, reinterpret_cast<const uint32_t *>(o));
+            }
+          }
+          const float mc = m == -INFINITY ? 0.0f : m * a.c;
+          const uint64_t nmc2 = pk2(-mc, -mc);
+          sum = weights64<T, false>(v, c2, nmc2, w);
           announce(0);
-          sum = add2(sum, weights64<T, true>(v + 64, c2, nmc2, w));
+          sum = add2(sum, weights64<T, false>(v + 64, c2, nmc2, w));
           announce(1);
         }
+        const float2 sf = un2(sum);
+        l += sf.x + sf.y;
       }
-      if (!settled) {
-        tmem_wait_ld();
-        if (masked) {
+      if (nb > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_o[x]), outs & 1));
+      step += nb;
+      outs += nb > 0;
+      if (live && ok) {
+        tc_fence_after();
+        const bool mine = row < s.rows;
+        const int64_t at_out = (s.out0 + row) * static_cast<int64_t>(a.G) * a.h_kv + head;
+        bool odd = false;
+        if (a.splits == 1) {
+          const float inv = limit > 0 ? 1.0f / l : 0.0f;
+          T *dst = static_cast<T *>(a.out) + at_out * HD;
+#pragma unroll 1
+          for (int i = 0; i < 4; ++i) {
+            float o[32];
+            if (nb > 0) {
+              tmem_ld32(to + 32 * i, o);
+              tmem_wait_ld();
+            }
+            uint4 w[4];
+            T *t = reinterpret_cast<T *>(w);
 #pragma unroll
-          for (int i = 0; i < PT; ++i) v[i] = i < seen ? v[i] : -INFINITY;
+            for (int e = 0; e < 32; ++e) {
+              const float y = limit > 0 ? o[e] * inv : 0.0f;
+              odd |= !(fabsf(y) < INFINITY);
+              t[e] = from_f32<T>(y);
+            }
+            if (mine) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) reinterpret_cast<uint4 *>(dst + 32 * i)[e] = w[e];
+            }
+          }
+        } else if (mine) {
+          // a part of the keys: the accumulator as it is, the maximum and the sum; no accumulator without a sum
+          const int64_t pa = z * a.rows * a.G * a.h_kv + at_out;
+          const bool some = limit > j0 * PT && nb > 0;
+          a.part_ml[pa] = limit == 0 ? make_float2(-INFINITY, -1.0f) : some ? make_float2(m == -INFINITY ? m : m * a.c, l) : make_float2(-INFINITY, 0.0f);
         }
-        t[0] = t[1] = t[2] = t[3] = -INFINITY;
-        largest(0);
-        largest(1);
-        const float top = max3(max3(t[0], t[1], t[2]), t[3], t[3]);
-        const bool grow = (top - m) * a.c > LAG || m == -INFINITY;
-        if (j == 0) {
-          m = top;
-        } else if (__any_sync(0xffffffffu, grow)) {
-          const float mn = grow ? fmaxf(m, top) : m;
-          const float f = grow ? ex2((m - (mn == -INFINITY ? 0.0f : mn)) * a.c) : 1.0f;
-          m = mn;
-          l *= f;
+        if (a.splits > 1 && nb > 0) {
+          float *dst = a.part + (z * a.rows * a.G * a.h_kv + at_out) * HD;
 #pragma unroll 1
           for (int i = 0; i < 4; ++i) {
             float o[32];
             tmem_ld32(to + 32 * i, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= f;
-            tmem_st32(to + 32 * i, reinterpret_cast<const uint32_t *>(o));
+            for (int e = 0; e < 32; ++e) odd |= limit > 0 && !(fabsf(o[e]) < INFINITY);
+            if (mine && limit > j0 * PT) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(dst + 32 * i + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
           }
         }
-        const float mc = m == -INFINITY ? 0.0f : m * a.c;
-        const uint64_t nmc2 = pk2(-mc, -mc);
-        sum = weights64<T, false>(v, c2, nmc2, w);
-        announce(0);
-        sum = add2(sum, weights64<T, false>(v + 64, c2, nmc2, w));
-        announce(1);
+        unsigned again = __ballot_sync(0xffffffffu, odd && mine);
+        while (again) {
+          const int r = __ffs(again) - 1;
+          again &= again - 1;
+          const int hi = min((j0 + nb) * PT, a.Lk - s.k0);
+          repair_row<T>(a, s, __shfl_sync(0xffffffffu, row, r), head, __shfl_sync(0xffffffffu, limit, r), j0 * PT, hi, z);
+        }
       }
-      const float2 sf = un2(sum);
-      l += sf.x + sf.y;
     }
-    if (nb > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_o[x]), 0));
     if (!ok) give_up();
-    if (live && ok) {
-      tc_fence_after();
-      const bool mine = row < s.rows;
-      const int64_t at_out = (s.out0 + row) * static_cast<int64_t>(a.G) * a.h_kv + head;
-      bool odd = false;
-      if (a.splits == 1) {
-        const float inv = limit > 0 ? 1.0f / l : 0.0f;
-        T *dst = static_cast<T *>(a.out) + at_out * HD;
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          float o[32];
-          if (nb > 0) {
-            tmem_ld32(to + 32 * i, o);
-            tmem_wait_ld();
-          }
-          uint4 w[4];
-          T *t = reinterpret_cast<T *>(w);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float y = limit > 0 ? o[e] * inv : 0.0f;
-            odd |= !(fabsf(y) < INFINITY);
-            t[e] = from_f32<T>(y);
-          }
-          if (mine) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) reinterpret_cast<uint4 *>(dst + 32 * i)[e] = w[e];
-          }
-        }
-      } else if (mine) {
-        // a part of the keys: the accumulator as it is, the maximum and the sum; no accumulator without a sum
-        const int64_t pa = z * a.rows * a.G * a.h_kv + at_out;
-        const bool some = limit > j0 * PT && nb > 0;
-        a.part_ml[pa] = limit == 0 ? make_float2(-INFINITY, -1.0f) : some ? make_float2(m == -INFINITY ? m : m * a.c, l) : make_float2(-INFINITY, 0.0f);
-      }
-      if (a.splits > 1 && nb > 0) {
-        float *dst = a.part + (z * a.rows * a.G * a.h_kv + at_out) * HD;
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          float o[32];
-          tmem_ld32(to + 32 * i, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) odd |= limit > 0 && !(fabsf(o[e]) < INFINITY);
-          if (mine && limit > j0 * PT) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(dst + 32 * i + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          }
-        }
-      }
-      unsigned again = __ballot_sync(0xffffffffu, odd && mine);
-      while (again) {
-        const int r = __ffs(again) - 1;
-        again &= again - 1;
-        const int hi = min((j0 + nb) * PT, a.Lk - s.k0);
-        repair_row<T>(a, s, __shfl_sync(0xffffffffu, row, r), head, __shfl_sync(0xffffffffu, limit, r), j0 * PT, hi, z);
-      }
-    }
     tc_fence_before();
   }
-  if (n > 0) {
-    __syncthreads();
-    __syncwarp();
-    tc_fence_after();
-    if (warp == 9) tmem_free(tmem, 512);
-  }
+  __syncthreads();
+  __syncwarp();
+  tc_fence_after();
+  if (warp == 9) tmem_free(tmem, 512);
 }
 
 // Joins the parts of split keys: one warp per (row, query head), four channels a lane.
@@ -788,9 +892,11 @@ extern "C" int kitty_prompt_attn(const void *q, const void *k, const void *v, in
   }
   const int64_t pairs = prompt_pairs(packed, B, Lq, a.G, a.zero_rest);
   if (!packed) a.pairs = static_cast<int32_t>(B > 0 ? pairs / B : 0);
-  const int64_t grid = pairs * h_kv * a.splits;
-  if (grid > 0x7fffffff || (Lq + PT) / PT * a.G > 0x7fffffff) return KITTY_E_BADSHAPE;
-  if (grid == 0) return KITTY_OK;
+  const int64_t items = pairs * h_kv * a.splits;
+  if (items > 0x3fffffff || (Lq + PT) / PT * a.G > 0x7fffffff) return KITTY_E_BADSHAPE;
+  if (items == 0) return KITTY_OK;
+  a.items = static_cast<int32_t>(items);
+  const unsigned grid = static_cast<unsigned>(items < sm_count() ? items : sm_count());
   const bool bf16 = dtype == KITTY_BF16;
   CUtensorMap mq, mk, mv;
   // without keys nothing is copied through their maps; they only have to be well formed
@@ -799,6 +905,6 @@ extern "C" int kitty_prompt_attn(const void *q, const void *k, const void *v, in
   else if (!make_map(&mk, k, bf16, Lk, h_kv, packed ? 1 : B, a.ks) || !make_map(&mv, v, bf16, Lk, h_kv, packed ? 1 : B, a.vs))
     return KITTY_E_CUDA;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return bf16 ? launch_prompt<__nv_bfloat16>(mq, mk, mv, a, static_cast<unsigned>(grid), s)
-              : launch_prompt<__half>(mq, mk, mv, a, static_cast<unsigned>(grid), s);
+  return bf16 ? launch_prompt<__nv_bfloat16>(mq, mk, mv, a, grid, s)
+              : launch_prompt<__half>(mq, mk, mv, a, grid, s);
 }

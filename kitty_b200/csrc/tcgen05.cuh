@@ -17,22 +17,27 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
       : "memory");
 }
 // Bounded wait that sleeps in hardware (up to the hint, in ns, per try) instead of spending issue slots of the warps that
-// share the scheduler.
+// share the scheduler; false when the phase did not complete within WAIT_LIMIT_NS.
+__device__ __forceinline__ bool mbar_try_asleep(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(1000000)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity) {
+  if (mbar_try_asleep(bar, parity)) return true;
+  const unsigned long long t0 = global_ns();
+  for (;;) {
 #pragma unroll 1
-  for (int i = 0; i < (1 << 20); ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity), "r"(2000000)
-        : "memory");
-    if (ok) return true;
-    if (i > 1000 && (i & 1023) == 0) __nanosleep(1000);
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_asleep(bar, parity)) return true;
+    if (global_ns() - t0 > WAIT_LIMIT_NS) return false;
   }
-  return false;
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
