@@ -200,6 +200,35 @@ def dtype_code(dtype) -> int:
         raise TypeError(f"kitty_b200 supports float16, bfloat16 and float32 tensors, got {dtype}") from None
 
 
+def head_rows(x, repeated: bool = True):
+    """x [B, H, T, 128], or [T, H, 128] for a packed batch, as the kernels read it, and its (batch, head, token) strides
+    (0 where a dimension has size one: views may carry any number there).  That is x itself when its channels are
+    consecutive and every row starts on a 16-byte boundary (and, without `repeated`, no dimension is expanded), otherwise
+    a copy."""
+    for _ in range(2):
+        st, shape = x.stride(), x.shape
+        if len(st) == 4:
+            a, b, c, d = st
+            n, m, t, _w = shape
+        else:
+            a, n = 0, 1
+            c, b, d = st
+            t, m, _w = shape
+        if n < 2:
+            a = 0
+        if m < 2:
+            b = 0
+        if t < 2:
+            c = 0
+        if d == 1 and not (a | b | c) & (15 // x.element_size()) and not x.data_ptr() & 15 \
+                and (repeated or (a or n < 2) and (b or m < 2) and (c or t < 2)):
+            break
+        import torch
+
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x, (a, b, c)
+
+
 def empty(shape, dtype, device):
     """torch.empty for a contiguous tensor by the way that costs least on the host."""
     import torch

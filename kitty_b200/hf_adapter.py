@@ -14,6 +14,7 @@ import torch
 import torch.nn.functional as F
 
 from .attention import kitty_attention_forward
+from .prompt import prompt_attention
 
 
 def _rotate_half(x):
@@ -98,7 +99,10 @@ def kitty_attention_module_forward(self, hidden_states, position_embeddings=None
         return self.o_proj(out.reshape(*input_shape, -1)), None
     is_prefill = past_key_values.update(k, v, self.layer_idx)
     if is_prefill:
-        out = _prefill_attention(q, k, v, attention_mask, self.scaling).transpose(1, 2)
+        if getattr(self, "kitty_prompt_kernel", False) and attention_mask is None and q.dtype != torch.float32:
+            out = prompt_attention(q, k, v, self.scaling)
+        else:
+            out = _prefill_attention(q, k, v, attention_mask, self.scaling).transpose(1, 2)
         past_key_values.quantize_prefill(self.layer_idx)
     else:
         out, _ = kitty_attention_forward(self, q.contiguous(), past_key_values.kv_cache[self.layer_idx], self.scaling)
@@ -121,14 +125,16 @@ def _fused_step_ok(cache, layer_idx: int, q, k, v) -> bool:
     return cache._step_host is not None           # a step planned at layer 0 is under way
 
 
-def patch_model(model) -> int:
-    """Install the Kitty call sequence on every self-attention module of `model`.  Returns how many were patched."""
+def patch_model(model, prompt_kernel: bool = False) -> int:
+    """Install the Kitty call sequence on every self-attention module of `model`.  Returns how many were patched.
+    prompt_kernel: 16-bit prompts without a mask go through `prompt_attention` instead of torch's attention."""
     n = 0
     cfg = model.config.get_text_config() if hasattr(model.config, "get_text_config") else model.config
     for mod in model.modules():
         if all(hasattr(mod, a) for a in ("q_proj", "k_proj", "v_proj", "o_proj", "layer_idx")):
             mod.num_attention_heads = cfg.num_attention_heads
             mod.num_key_value_heads = cfg.num_key_value_heads
+            mod.kitty_prompt_kernel = prompt_kernel
             mod.forward = types.MethodType(kitty_attention_module_forward, mod)
             n += 1
     return n

@@ -17,7 +17,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .rotary import RotaryEmbedding, _head_strides
+from .rotary import RotaryEmbedding
 
 PAGE_SIZE = 128
 BLOCK = _lib.KV8_BLOCK
@@ -118,7 +118,7 @@ def _row_tensor(x: torch.Tensor, what: str, B: int, layer: KV8Layer) -> torch.Te
     return x if x.is_contiguous() else x.contiguous()
 
 
-def _tokens(x: torch.Tensor, what: str, heads: int, layer: KV8Layer) -> torch.Tensor:
+def _tokens(x: torch.Tensor, what: str, heads: int, layer: KV8Layer):
     shape = x.shape
     if len(shape) != 4 or shape[1] != heads or shape[3] != layer.D:
         raise ValueError(f"expected {what} [B, {heads}, T, {layer.D}], got {tuple(shape)}")
@@ -126,7 +126,7 @@ def _tokens(x: torch.Tensor, what: str, heads: int, layer: KV8Layer) -> torch.Te
         if not x.is_cuda:
             raise ValueError(f"kitty_b200 has no CPU path: the {what} must be on a CUDA device")
         raise ValueError(f"the {what} must be {layer.dtype} on {layer.device}, got {x.dtype} on {x.device}")
-    return x if x.stride(3) == 1 else x.contiguous()
+    return _lib.head_rows(x)
 
 
 def kv8_append(layer: KV8Layer, key: torch.Tensor, value: torch.Tensor, start: torch.Tensor, *,
@@ -138,7 +138,7 @@ def kv8_append(layer: KV8Layer, key: torch.Tensor, value: torch.Tensor, start: t
     (default all).  rotary: the keys are turned on the way, token i of row b by position start[b] + i.  query
     [B, H_Q, T, 128] is then turned by the same positions and returned, [B, H_Q, T, 128] contiguous (all T tokens);
     without it the call returns None."""
-    k, v = _tokens(key, "key", layer.H_KV, layer), _tokens(value, "value", layer.H_KV, layer)
+    (k, k_st), (v, v_st) = _tokens(key, "key", layer.H_KV, layer), _tokens(value, "value", layer.H_KV, layer)
     B, _, T, _ = k.shape
     if v.shape != k.shape:
         raise ValueError(f"key and value differ in shape: {tuple(k.shape)} and {tuple(v.shape)}")
@@ -149,22 +149,19 @@ def kv8_append(layer: KV8Layer, key: torch.Tensor, value: torch.Tensor, start: t
     start = _row_tensor(start, "start", B, layer)
     if lengths is not None:
         lengths = _row_tensor(lengths, "lengths", B, layer)
-    out, h_q, strides = None, 0, _head_strides(k) + _head_strides(v)
+    out, h_q, q_st = None, 0, (0, 0, 0)
     if query is not None:
         if rotary is None:
             raise ValueError("the query goes along to be turned: pass rotary")
         if query.dim() != 4 or query.shape[0] != B or query.shape[2] != T:
             raise ValueError(f"expected query [{B}, H_Q, {T}, {layer.D}], got {tuple(query.shape)}")
         h_q = query.shape[1]
-        query = _tokens(query, "query", h_q, layer)
+        query, q_st = _tokens(query, "query", h_q, layer)
         out = _lib.empty((B, h_q, T, layer.D), layer.dtype, layer.device)
-        strides += _head_strides(query)
-    else:
-        strides += (0, 0, 0)
     if rotary is not None and rotary.device != layer.device:
         raise ValueError(f"the angles are on {rotary.device}, the cache on {layer.device}")
     _lib.call_on(layer.device, _lib.lib().kitty_kv8_append, "kitty_kv8_append", layer.c_layer(), k.data_ptr(),
-                 v.data_ptr(), _lib.i64_array(strides), start.data_ptr(), None if lengths is None else lengths.data_ptr(),
+                 v.data_ptr(), _lib.i64_array(k_st + v_st + q_st), start.data_ptr(), None if lengths is None else lengths.data_ptr(),
                  B, T, None if rotary is None else rotary.c_plan(), query.data_ptr() if h_q else None,
                  out.data_ptr() if h_q else None, h_q)
     return out
@@ -197,7 +194,7 @@ def kv8_attention(query: torch.Tensor, layer: KV8Layer, lengths: torch.Tensor, s
     if query.dim() != 4 or query.shape[2] != 1:
         raise ValueError(f"expected query [B, H_Q, 1, {layer.D}], got {tuple(query.shape)}")
     B, h_q, _, D = query.shape
-    q = _tokens(query, "query", h_q, layer)
+    q, _ = _tokens(query, "query", h_q, layer)
     if h_q == 0 or h_q % layer.H_KV:
         raise ValueError(f"{h_q} query heads over {layer.H_KV} key heads")
     if B > layer.MAX_BS:

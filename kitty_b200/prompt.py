@@ -17,11 +17,15 @@ HEAD_DIM = 128
 _status: dict = {}
 
 
-def _status_word(device: torch.device) -> torch.Tensor:
+def _status_word(device: torch.device) -> Optional[int]:
+    """Address of the device's status word; none during a capture that comes before the device's first call (memory of
+    a graph's own pool must not outlive it)."""
     st = _status.get(device)
     if st is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None
         st = _status[device] = torch.zeros(1, dtype=torch.int32, device=device)
-    return st
+    return st.data_ptr()
 
 
 @functools.lru_cache(maxsize=4096)
@@ -49,8 +53,7 @@ def _lengths(x, what: str, n: int, device) -> Optional[torch.Tensor]:
 
 
 def _source(x: torch.Tensor, what: str, like: torch.Tensor, packed: bool):
-    """The tensor, in place where the copies can read it (consecutive channels, no repeated dimension), and its (batch,
-    head, token) strides."""
+    """The tensor as the copies can read it, and its strides."""
     shape, dev = x.shape, x.device
     if len(shape) != (3 if packed else 4) or shape[-1] != HEAD_DIM:
         raise ValueError(f"expected {what} {'[T, H, 128]' if packed else '[B, H, T, 128]'}, got {tuple(shape)}")
@@ -60,17 +63,7 @@ def _source(x: torch.Tensor, what: str, like: torch.Tensor, packed: bool):
         raise TypeError(f"prompt_attention takes float16 or bfloat16 tensors, got {x.dtype}")
     if x is not like and (x.dtype != like.dtype or dev != like.device):
         raise ValueError("query, key and value must agree in type and device")
-    for again in (False, True):
-        if packed:
-            t, h, d = x.stride()
-            st = (0, h if shape[1] > 1 else 0, t if shape[0] > 1 else 0)
-        else:
-            b, h, t, d = x.stride()
-            st = (b if shape[0] > 1 else 0, h if shape[1] > 1 else 0, t if shape[2] > 1 else 0)
-        if d == 1 and (shape[0] < 2 or packed or b > 0) and (shape[1] < 2 or h > 0) and (shape[-3 if packed else 2] < 2 or t > 0):
-            break
-        x = x.contiguous()
-    return x, st
+    return _lib.head_rows(x, repeated=False)
 
 
 def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, scaling: float, *, causal: bool = True,
@@ -132,5 +125,5 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     _lib.call_on(dev, _lib.lib().kitty_prompt_attn, "kitty_prompt_attn", q.data_ptr(), k.data_ptr(), v.data_ptr(),
                  _lib.dtype_code(q.dtype), _lib.i64_array(q_st + k_st + v_st), B, Lq, Lk, h_q, h_kv, float(scaling),
                  int(causal), *(None if x is None else x.data_ptr() for x in (q_len, k_len, cu_q, cu_k)), out.data_ptr(),
-                 int(zero_rest), _status_word(dev).data_ptr(), None if ws is None else ws.data_ptr(), need)
+                 int(zero_rest), _status_word(dev), None if ws is None else ws.data_ptr(), need)
     return out

@@ -111,32 +111,26 @@ class RotaryEmbedding:
         return self._c_plan
 
 
-def _head_strides(x: torch.Tensor):
-    """(batch, head, token) strides; a dimension of size one has none (views may carry any number there)."""
-    a, b, c, _ = x.stride()
-    n, m, t, _ = x.shape
-    return (a if n > 1 else 0, b if m > 1 else 0, c if t > 1 else 0)
-
-
-def _rotary_input(x: torch.Tensor, what: str, device) -> torch.Tensor:
+def _rotary_input(x: torch.Tensor, what: str, device):
     if x.dim() != 4 or x.shape[3] != HEAD_DIM:
         raise ValueError(f"expected {what} [B, H, T, 128], got {tuple(x.shape)}")
     if x.device != device:
         if not x.is_cuda:
             raise ValueError(f"kitty_b200 has no CPU path: the {what} must be on a CUDA device")
         raise ValueError(f"the angles are on {device}, the {what} on {x.device}")
-    return x if x.stride(3) == 1 else x.contiguous()
+    return _lib.head_rows(x)
 
 
-def _rotary_output(out: torch.Tensor, x: torch.Tensor, what: str) -> torch.Tensor:
-    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(3) != 1:
-        raise ValueError(f"{what}_out must have the {what}'s shape, type and device, with consecutive channels")
-    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
-        raise ValueError(f"{what}_out is an expanded view: several heads would be written to one place")
+def _rotary_output(out: torch.Tensor, x: torch.Tensor, what: str):
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise ValueError(f"{what}_out must have the {what}'s shape, type and device")
+    rows, strides = _lib.head_rows(out, repeated=False)
+    if rows is not out:
+        raise ValueError(f"{what}_out needs consecutive channels, rows on 16-byte boundaries and no expanded dimension")
     same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
     if not same and _spans_overlap(out, x):
         raise ValueError(f"{what}_out overlaps the {what} without being the same view")
-    return out
+    return out, strides
 
 
 def _span(x: torch.Tensor):
@@ -158,7 +152,7 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
     or in query_out / key_out, which may be query and key themselves (in place); other overlaps of outputs and inputs
     are the caller's error and refused where the views' spans show them."""
     dev = rotary.device
-    q, k = _rotary_input(query, "query", dev), _rotary_input(key, "key", dev)
+    (q, q_st), (k, k_st) = _rotary_input(query, "query", dev), _rotary_input(key, "key", dev)
     B, h_q, T, _ = q.shape
     Bk, h_kv, Tk, _ = k.shape
     if Bk != B or Tk != T or k.dtype != q.dtype:
@@ -177,9 +171,15 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
         raise ValueError("positions must be int64 on the query's device")
     if T > 1 and positions.stride(-1) != 1:
         positions = positions.contiguous()
-    qo = torch.empty_like(q) if query_out is None else _rotary_output(query_out, q, "query")
-    ko = torch.empty_like(k) if key_out is None else _rotary_output(key_out, k, "key")
-    strides = _lib.i64_array(_head_strides(q) + _head_strides(k) + _head_strides(qo) + _head_strides(ko))
+    if query_out is None:
+        qo, qo_st = _lib.head_rows(torch.empty_like(q))
+    else:
+        qo, qo_st = _rotary_output(query_out, query, "query")
+    if key_out is None:
+        ko, ko_st = _lib.head_rows(torch.empty_like(k))
+    else:
+        ko, ko_st = _rotary_output(key_out, key, "key")
+    strides = _lib.i64_array(q_st + k_st + qo_st + ko_st)
     _lib.call_on(dev, _lib.lib().kitty_rotary, "kitty_rotary", rotary.c_plan(), q.data_ptr(), k.data_ptr(),
                  positions.data_ptr(), positions.stride(0) if rows > 1 else 0, qo.data_ptr(), ko.data_ptr(), code, B, T,
                  h_q, h_kv, strides)

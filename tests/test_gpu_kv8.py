@@ -354,3 +354,26 @@ def test_prompt_then_tokens_then_a_further_piece(kb):
     assert torch.isfinite(prompt).all() and (prompt[1, 77:] == 0).all()
     layer.check()
     assert kb.prompt_attention_status(DEV) == 0
+
+
+def test_rows_off_their_boundaries(kb):
+    k, v = _kv(1, 2, 40, torch.float16, 4)
+    wide = torch.zeros(1, 2, 40, 130, dtype=torch.float16, device=DEV)
+    wide[..., 1:129] = k
+    a, b = (kb.KV8Layer(1, 128, 2, dtype=torch.float16, device=DEV) for _ in range(2))
+    kb.kv8_append(a, k, v, _i32([0]))
+    kb.kv8_append(b, wide[..., 1:129], v, _i32([0]))
+    assert torch.equal(a.pages, b.pages) and torch.equal(a.tail_k, b.tail_k)
+
+
+def test_a_replaced_page_table_is_used_and_checked(kb):
+    k, v = _kv(1, 1, 128, torch.bfloat16, 5)
+    layer = kb.KV8Layer(1, 256, 1, device=DEV)
+    kb.kv8_append(layer, k, v, _i32([0]))
+    first = layer.pages[0].clone()
+    layer.page_table = torch.tensor([[1, 0]], device=DEV)
+    kb.kv8_append(layer, k, v, _i32([0]))
+    assert torch.equal(layer.pages[1], first)
+    layer.page_table = torch.zeros(1, 3, dtype=torch.int64, device=DEV)
+    with pytest.raises(ValueError, match="page_table"):
+        kb.kv8_append(layer, k, v, _i32([0]))

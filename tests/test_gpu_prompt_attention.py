@@ -243,3 +243,55 @@ def test_agrees_with_decode_attention(kb):
             bound = attention_bound(want, mag, torch.float16, HALF[torch.float16], logit_error(qx, kx, SC))
             assert ((got[b, :, x].double() - want).abs() <= bound).all()
     assert (dec.float() - got.float()).abs().max() <= 1e-2 * got.float().abs().max()
+
+
+def test_rows_off_their_boundaries_and_other_orders(kb):
+    """Views whose rows start anywhere, channels apart, heads expanded: read through a copy, the same result."""
+    q, k, v = _inputs((1, 4, 90, 128), (1, 2, 90, 128), torch.bfloat16, 9)
+    want = kb.prompt_attention(q, k, v, SC)
+
+    def off(x, pad):
+        wide = torch.zeros(*x.shape[:-1], 128 + pad, dtype=x.dtype, device=DEV)
+        wide[..., pad:] = x
+        return wide[..., pad:]
+
+    assert torch.equal(kb.prompt_attention(off(q, 1), off(k, 3), off(v, 4), SC), want)
+    apart = torch.stack((q, q), -1)[..., 0]
+    assert apart.stride(-1) == 2 and torch.equal(kb.prompt_attention(apart, k, v, SC), want)
+    cu = torch.tensor([0, 90], dtype=torch.int32, device=DEV)
+    packed = [off(x[0].transpose(0, 1).contiguous(), 2) for x in (q, k, v)]
+    assert torch.equal(kb.prompt_attention(*packed, SC, cu_seqlens=cu), want[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_patched_model_takes_the_prompt_kernel(kb, dtype, monkeypatch):
+    """patch_model(prompt_kernel=True): every layer's prompt goes through the operator, whose results meet the formula;
+    float32 models and masked batches keep torch's attention."""
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    from kitty_b200 import hf_adapter
+
+    torch.manual_seed(0)
+    cfg = LlamaConfig(hidden_size=512, intermediate_size=1024, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                      head_dim=128, vocab_size=1000, max_position_embeddings=4096)
+    model = LlamaForCausalLM(cfg).eval().to(dtype).to(DEV)
+    assert hf_adapter.patch_model(model, prompt_kernel=True) == 2
+    calls = []
+
+    def recorded(q, k, v, scaling):
+        out = kb.prompt_attention(q, k, v, scaling)
+        calls.append((q, k, v, scaling, out))
+        return out
+
+    monkeypatch.setattr(hf_adapter, "prompt_attention", recorded)
+    ids = torch.randint(0, 1000, (2, 150), device=DEV)
+    cache = kb.get_kvcache_kitty(cfg, 2, 512, device=DEV)
+    toks = hf_adapter.greedy_decode(model, ids, 4, cache)
+    assert toks.shape == (2, 4) and len(calls) == 2 and cache.get_seq_length() == 153
+    for q, k, v, scaling, out in calls:
+        for b in range(2):
+            _check_rows(out[b], *(x[b].transpose(0, 1) for x in (q, k, v)), scaling, True)
+    single = LlamaForCausalLM(cfg).eval().to(DEV)
+    hf_adapter.patch_model(single, prompt_kernel=True)
+    hf_adapter.greedy_decode(single, ids, 2, kb.get_kvcache_kitty(cfg, 2, 512, device=DEV))
+    assert len(calls) == 2

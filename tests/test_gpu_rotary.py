@@ -110,3 +110,23 @@ def test_agrees_with_the_decode_token_path(kb):
         s = src.transpose(1, 2).float().abs()
         bound = 6 * 2.0 ** -8 * (s + torch.roll(s, 64, -1))
         assert ((x.float() - y.float()).abs() <= bound + 1e-6).all()
+
+
+def test_rows_off_their_boundaries(kb):
+    rot = kb.RotaryEmbedding(device=DEV)
+    wide = torch.randn(2, 3, 5, 129, device=DEV).half()
+    q, k = wide[..., 1:], torch.randn(2, 1, 5, 128, device=DEV).half()
+    pos = torch.arange(5, device=DEV)
+    a, _ = kb.apply_rotary(q, k, pos, rot)
+    b, _ = kb.apply_rotary(q.contiguous(), k, pos, rot)
+    assert torch.equal(a, b)
+    e, _ = kb.apply_rotary(k.expand(2, 4, 5, 128), k, pos, rot)             # one head read four times
+    assert torch.equal(e, kb.apply_rotary(k, k, pos, rot)[0].expand(2, 4, 5, 128))
+    before = wide.clone()
+    for bad in (q, k.expand(2, 3, 5, 128)):
+        with pytest.raises(ValueError):
+            kb.apply_rotary(q, k, pos, rot, query_out=bad)
+    buf = torch.randn(2, 3, 6, 128, device=DEV).half()
+    with pytest.raises(ValueError, match="overlaps"):
+        kb.apply_rotary(buf[:, :, :5], k, pos, rot, query_out=buf[:, :, 1:])
+    assert torch.equal(wide, before)
