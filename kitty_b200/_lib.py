@@ -59,7 +59,7 @@ class KittyStepState(C.Structure):
 
 class KittyRotaryPlan(C.Structure):
     """struct kitty_rotary_plan"""
-    _fields_ = [("turns", C.c_void_p), ("factor", C.c_float), ("rotary_dim", C.c_int32), ("layout", C.c_int32),
+    _fields_ = [("turns", C.c_void_p), ("steps", C.c_void_p), ("factor", C.c_float), ("rotary_dim", C.c_int32), ("layout", C.c_int32),
                 ("reserved", C.c_int32)]
 
 

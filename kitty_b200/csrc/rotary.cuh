@@ -5,8 +5,10 @@
 // with channels (p, p + rotary_dim/2) ("half") or (2p, 2p + 1) ("interleaved"); channels from rotary_dim on keep
 // their value.  The plan holds w_p in TURNS per position (w_p / 2 pi, 64 bits): position * turns loses its whole part
 // exactly in 64 bits, and the remaining fraction of a turn goes through sincospif, so an angle at position 2^31 is as
-// good as one at position 1 (a 32-bit product is off by 0.004 rad at position 100000).  The rotation itself is two
-// fused multiply-adds in 32 bits, rounded once to the data type.
+// good as one at position 1 (a 32-bit product is off by 0.004 rad at position 100000).  That is done for the position's
+// multiple of 32; the rest is turned on by the plan's 32-bit table of small steps (four multiplications instead of some
+// hundred instructions: a block of 32 tokens needs one sine and cosine per pair).  The rotation itself is two fused
+// multiply-adds in 32 bits, rounded once to the data type.
 #pragma once
 
 #include "common.cuh"
@@ -45,12 +47,23 @@ struct RotTable {
   __device__ __forceinline__ float2 one(int p) const { return tab[p]; }
 };
 
-__device__ __forceinline__ float2 rot_angle(const kitty_rotary_plan &pl, int64_t pos, int p) {
+constexpr int ROT_STEPS = 32;
+
+// Cosine and sine of pair p at a multiple of 32, and with the remaining steps and the factor turned on.
+__device__ __forceinline__ float2 rot_base(const kitty_rotary_plan &pl, int64_t pos, int p) {
   double t = static_cast<double>(pos) * pl.turns[p];
   t -= rint(t);
   float s, c;
   sincospif(static_cast<float>(t + t), &s, &c);
-  return make_float2(c * pl.factor, s * pl.factor);
+  return make_float2(c, s);
+}
+__device__ __forceinline__ float2 rot_step(const kitty_rotary_plan &pl, float2 base, int step, int p) {
+  const float2 z = reinterpret_cast<const float2 *>(pl.steps)[step * (pl.rotary_dim / 2) + p];
+  return make_float2(fmaf(base.x, z.x, -base.y * z.y) * pl.factor, fmaf(base.y, z.x, base.x * z.y) * pl.factor);
+}
+__device__ __forceinline__ float2 rot_angle(const kitty_rotary_plan &pl, int64_t pos, int p) {
+  const int step = static_cast<int>(pos & (ROT_STEPS - 1));
+  return rot_step(pl, rot_base(pl, pos - step, p), step, p);
 }
 
 template <typename T>
@@ -165,7 +178,8 @@ inline int rot_mode(const kitty_rotary_plan &p, int esize) {
 }
 
 inline int check_rotary_plan(const kitty_rotary_plan *p) {
-  if (p == nullptr || p->turns == nullptr) return KITTY_E_BADARG;
+  if (p == nullptr || p->turns == nullptr || p->steps == nullptr) return KITTY_E_BADARG;
+  if (reinterpret_cast<uintptr_t>(p->steps) & 7) return KITTY_E_BADARG;
   if (p->rotary_dim < 2 || p->rotary_dim > HD || p->rotary_dim % 2 != 0) return KITTY_E_BADSHAPE;
   if (p->layout != KITTY_ROPE_HALF && p->layout != KITTY_ROPE_INTERLEAVED) return KITTY_E_BADARG;
   return KITTY_OK;

@@ -22,8 +22,9 @@ def rotate(x, positions, inv, factor, r, layout):
 
 
 def rotate_bound(x, y, factor, r, layout):
-    """Half a step of the output plus the 32-bit work: sine and cosine to 2 steps (2^-22), their factor, the two products
-    and the sum half a step each (4 * 2^-24), so at most 2^-21 of |x1| + |x2|, times the factor."""
+    """Half a step of the output plus the 32-bit work.  In units of 2^-24: the sine and cosine of the position's multiple
+    of 32 to one, of the rest to a half, their four products and two sums (1.41 + 0.71 + 1), the factor (1), a product
+    and a sum of the rotation itself (2): at most 6.2, within 2^-21 of |x1| + |x2|, times the factor."""
     pair = x.double().abs().clone()
     if layout == "half":
         s = pair[..., : r // 2] + pair[..., r // 2: r]

@@ -16,7 +16,7 @@ def L():
 
 
 def _plan(L, r=128, layout=0, turns=P):
-    return L.KittyRotaryPlan(turns, 1.0, r, layout, 0)
+    return L.KittyRotaryPlan(turns, P, 1.0, r, layout, 0)
 
 
 def _layer(L, **over):
@@ -104,7 +104,7 @@ def test_kv8_entry_points(L):
 
 
 def test_struct_sizes(L):
-    assert C.sizeof(L.KittyRotaryPlan) == 24 and C.sizeof(L.KittyKV8Layer) == 6 * 4 + 5 * 8
+    assert C.sizeof(L.KittyRotaryPlan) == 32 and C.sizeof(L.KittyKV8Layer) == 6 * 4 + 5 * 8
 
 
 def test_python_refusals_without_a_gpu():
