@@ -343,7 +343,7 @@ int kitty_lse_exchange_merge(const float *local_partial, int64_t rows, void *con
 /* ---- Rotary positions of prompts and tokens ------------------------------------------------
  * (No counterpart in the reference, whose models call the element-wise sequence of
  * models/qwen3/modeling_qwen3.py:222-232.)  Pair p of a head is turned by angle position * w_p and multiplied by
- * `factor`; channels from rotary_dim on keep their value.  Angles are formed in 64 bits, the rotation in 32 bits with
+ * `factor`; channels from rotary_dim on keep their value.  Angles, sines and cosines are formed in 64 bits, the rotation in 32 bits with
  * one rounding to the data type at the end (kitty_rope_qk rounds every product, as its models do). */
 typedef enum {
   KITTY_ROPE_HALF = 0,       /* pair p = channels p and p + rotary_dim/2 */
@@ -352,7 +352,7 @@ typedef enum {
 
 typedef struct {
   const double *turns;   /* DEVICE array [rotary_dim / 2]: w_p / (2 pi), the turns per position of each pair */
-  const float *steps;    /* DEVICE array [32][rotary_dim / 2][2], 8-byte aligned: cos(i w_p), sin(i w_p) for i = 0 .. 31 */
+  const double *steps;   /* DEVICE array [32][rotary_dim / 2][2], 16-byte aligned: cos(i w_p), sin(i w_p), i = 0 .. 31 */
   float factor;          /* on cosine and sine (1 unless the scaling asks for more)                        */
   int32_t rotary_dim;    /* even, 2 .. 128                                                                  */
   int32_t layout;        /* kitty_rope_layout                                                               */

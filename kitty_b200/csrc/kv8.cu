@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256, APPEND_BLOCKS<MODE>) kv8_append_kernel(co
   __shared__ __align__(16) uint8_t vt[KV8_OFF_V];
   __shared__ __align__(16) T stage[HALF ? KV8_BLOCK : 1][HD + 8];
   __shared__ uint32_t red[2][8];
-  __shared__ float2 base[MODE == ROT_NONE ? 1 : HD / 2];
+  __shared__ double2 base[MODE == ROT_NONE ? 1 : HD / 2];
   const kitty_kv8_layer &L = a.L;
   const int b = blockIdx.z, cap = L.max_page * PAGE;
   int n = a.counts != nullptr ? a.counts[b] : a.T;

@@ -844,7 +844,7 @@ extern "C" int kitty_prompt_attn(const void *q, const void *k, const void *v, in
                                  int64_t workspace_bytes, void *stream) {
   if (!strides || B < 0 || Lq < 0 || Lk < 0 || h_q <= 0 || h_kv <= 0 || h_q % h_kv != 0) return KITTY_E_BADARG;
   if (dtype != KITTY_F16 && dtype != KITTY_BF16) return KITTY_E_BADARG;
-  if (!(scaling > 0.0f) || !(scaling < INFINITY)) return KITTY_E_BADARG;
+  if (!(scaling > 0.0f) || !(scaling * 1.4426950408889634f < INFINITY)) return KITTY_E_BADARG;
   if (Lq > (1 << 30) || Lk > (1 << 30)) return KITTY_E_BADSHAPE;
   const bool packed = cu_q != nullptr;
   if (Lq == 0 || (B == 0 && !packed)) return KITTY_OK;

@@ -4,11 +4,12 @@
 //   (x1, x2) -> factor * (x1 cos - x2 sin, x2 cos + x1 sin)
 // with channels (p, p + rotary_dim/2) ("half") or (2p, 2p + 1) ("interleaved"); channels from rotary_dim on keep
 // their value.  The plan holds w_p in TURNS per position (w_p / 2 pi, 64 bits): position * turns loses its whole part
-// exactly in 64 bits, and the remaining fraction of a turn goes through sincospif, so an angle at position 2^31 is as
-// good as one at position 1 (a 32-bit product is off by 0.004 rad at position 100000).  That is done for the position's
-// multiple of 32; the rest is turned on by the plan's 32-bit table of small steps (four multiplications instead of some
-// hundred instructions: a block of 32 tokens needs one sine and cosine per pair).  The rotation itself is two fused
-// multiply-adds in 32 bits, rounded once to the data type.
+// exactly in 64 bits, and an angle is off by 2^-51 of the position times w at most (a 32-bit product is off by 0.004 rad
+// at position 100000).  Sine and cosine are 64-bit too: those of the position's multiple of 32 are computed, those of the
+// rest come from the plan's table of small steps and are turned on with four multiplications; a block of 32 tokens so
+// needs one sine and cosine per pair.  Both round to 32 bits once, to half a step.  (With 32-bit sines the turned keys
+// were off by up to 2^-22, and four times as many of them fell on the other side of a rounding to 16 bits as with exact
+// ones.)  The rotation itself is two fused multiply-adds in 32 bits, rounded once to the data type.
 #pragma once
 
 #include "common.cuh"
@@ -49,17 +50,17 @@ struct RotTable {
 
 constexpr int ROT_STEPS = 32;
 
-// Cosine and sine of pair p at a multiple of 32, and with the remaining steps and the factor turned on.
-__device__ __forceinline__ float2 rot_base(const kitty_rotary_plan &pl, int64_t pos, int p) {
+// Factor times cosine and sine of pair p at a multiple of 32, and with the remaining steps turned on.
+__device__ __forceinline__ double2 rot_base(const kitty_rotary_plan &pl, int64_t pos, int p) {
   double t = static_cast<double>(pos) * pl.turns[p];
   t -= rint(t);
-  float s, c;
-  sincospif(static_cast<float>(t + t), &s, &c);
-  return make_float2(c, s);
+  double s, c;
+  sincospi(t + t, &s, &c);
+  return make_double2(c * pl.factor, s * pl.factor);
 }
-__device__ __forceinline__ float2 rot_step(const kitty_rotary_plan &pl, float2 base, int step, int p) {
-  const float2 z = reinterpret_cast<const float2 *>(pl.steps)[step * (pl.rotary_dim / 2) + p];
-  return make_float2(fmaf(base.x, z.x, -base.y * z.y) * pl.factor, fmaf(base.y, z.x, base.x * z.y) * pl.factor);
+__device__ __forceinline__ float2 rot_step(const kitty_rotary_plan &pl, double2 base, int step, int p) {
+  const double2 z = reinterpret_cast<const double2 *>(pl.steps)[step * (pl.rotary_dim / 2) + p];
+  return make_float2(static_cast<float>(fma(base.x, z.x, -base.y * z.y)), static_cast<float>(fma(base.y, z.x, base.x * z.y)));
 }
 __device__ __forceinline__ float2 rot_angle(const kitty_rotary_plan &pl, int64_t pos, int p) {
   const int step = static_cast<int>(pos & (ROT_STEPS - 1));
@@ -179,7 +180,7 @@ inline int rot_mode(const kitty_rotary_plan &p, int esize) {
 
 inline int check_rotary_plan(const kitty_rotary_plan *p) {
   if (p == nullptr || p->turns == nullptr || p->steps == nullptr) return KITTY_E_BADARG;
-  if (reinterpret_cast<uintptr_t>(p->steps) & 7) return KITTY_E_BADARG;
+  if (reinterpret_cast<uintptr_t>(p->steps) & 15) return KITTY_E_BADARG;
   if (p->rotary_dim < 2 || p->rotary_dim > HD || p->rotary_dim % 2 != 0) return KITTY_E_BADSHAPE;
   if (p->layout != KITTY_ROPE_HALF && p->layout != KITTY_ROPE_INTERLEAVED) return KITTY_E_BADARG;
   return KITTY_OK;

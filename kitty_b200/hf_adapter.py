@@ -99,7 +99,8 @@ def kitty_attention_module_forward(self, hidden_states, position_embeddings=None
         return self.o_proj(out.reshape(*input_shape, -1)), None
     is_prefill = past_key_values.update(k, v, self.layer_idx)
     if is_prefill:
-        if getattr(self, "kitty_prompt_kernel", False) and attention_mask is None and q.dtype != torch.float32:
+        if (getattr(self, "kitty_prompt_kernel", False) and attention_mask is None and q.is_cuda and q.shape[-1] == 128
+                and q.dtype in (torch.float16, torch.bfloat16)):
             out = prompt_attention(q, k, v, self.scaling)
         else:
             out = _prefill_attention(q, k, v, attention_mask, self.scaling).transpose(1, 2)

@@ -134,7 +134,8 @@ def kv8_append(layer: KV8Layer, key: torch.Tensor, value: torch.Tensor, start: t
                query: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Append tokens key / value [B, H, T, 128] (any strides with consecutive channels) to rows 0 .. B-1.
 
-    start: int32 [B], the tokens each row holds already.  lengths: int32 [B], how many of the T tokens are the row's
+    start: int32 [B], the tokens each row holds already (a row may be cut back to any length within its open block;
+    further back, give the tokens again from that block's first one).  lengths: int32 [B], how many of the T tokens are the row's
     (default all).  rotary: the keys are turned on the way, token i of row b by position start[b] + i.  query
     [B, H_Q, T, 128] is then turned by the same positions and returned, [B, H_Q, T, 128] contiguous (all T tokens);
     without it the call returns None."""

@@ -3,8 +3,8 @@
 `RotaryEmbedding` holds what a model's configuration says about its angles (base, how much of the head turns, pair
 layout, scaling for long contexts); `apply_rotary` turns the query and key heads of any number of tokens in one launch.
 The reference leaves this to its models' element-wise sequence (models/qwen3/modeling_qwen3.py:222-232), whose roundings
-`hf_adapter.rope_decode_token` reproduces for a decode token; here angles are formed in 64 bits and every output is
-rounded once.
+`hf_adapter.rope_decode_token` reproduces for a decode token; here angles, sines and cosines are formed in 64 bits and every
+output is rounded once.
 """
 from __future__ import annotations
 
@@ -106,7 +106,7 @@ class RotaryEmbedding:
         self._turns = torch.tensor([w / (2 * math.pi) for w in inv], dtype=torch.float64, device=dev)
         self.device = self._turns.device
         step = torch.arange(32, dtype=torch.float64)[:, None] * self.inv_freq
-        self._steps = torch.stack((torch.cos(step), torch.sin(step)), -1).float().to(dev).contiguous()
+        self._steps = torch.stack((torch.cos(step), torch.sin(step)), -1).to(dev).contiguous()
         self._c_plan = _lib.KittyRotaryPlan(self._turns.data_ptr(), self._steps.data_ptr(), self.factor, rotary_dim, ROPE_LAYOUTS[layout], 0)
 
     def c_plan(self) -> "_lib.KittyRotaryPlan":

@@ -21,19 +21,22 @@ def rotate(x, positions, inv, factor, r, layout):
     return y
 
 
-def rotate_bound(x, y, factor, r, layout):
-    """Half a step of the output plus the 32-bit work.  In units of 2^-24: the sine and cosine of the position's multiple
-    of 32 to one, of the rest to a half, their four products and two sums (1.41 + 0.71 + 1), the factor (1), a product
-    and a sum of the rotation itself (2): at most 6.2, within 2^-21 of |x1| + |x2|, times the factor."""
+def rotate_bound(x, y, factor, r, layout, positions, inv):
+    """Half a step of the output plus the 32-bit work: sine and cosine (times the factor) to half a step, 2^-25 of the
+    factor and a little; a product rounded to half a step and the sum of the two: in all at most 1.6 * 2^-24, within
+    2^-23 of |x1| + |x2|, times the factor.  The angles themselves are 64-bit products: the formula's is rounded once
+    (2^-53 of its size), the kernel's three times (the pair's turns, their table entry, the product): together within
+    2^-51 of position * frequency, which counts from position 2^20 on."""
     pair = x.double().abs().clone()
+    far = 2.0 ** -51 * positions.double().abs()[:, None, :, None] * inv
     if layout == "half":
-        s = pair[..., : r // 2] + pair[..., r // 2: r]
+        s = (pair[..., : r // 2] + pair[..., r // 2: r]) * (2.0 ** -23 + far)
         pair[..., : r // 2], pair[..., r // 2: r] = s, s
     else:
-        s = pair[..., 0:r:2] + pair[..., 1:r:2]
+        s = (pair[..., 0:r:2] + pair[..., 1:r:2]) * (2.0 ** -23 + far)
         pair[..., 0:r:2], pair[..., 1:r:2] = s, s
     pair[..., r:] = 0.0
-    return HALF[x.dtype] * y.abs() + 2.0 ** -21 * factor * pair + TINY[x.dtype]
+    return HALF[x.dtype] * y.abs() + factor * pair + TINY[x.dtype]
 
 
 def attend(q, k, v, scaling, limits):

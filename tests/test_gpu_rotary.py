@@ -22,7 +22,7 @@ def kb():
 
 def _check(got, x, pos, rot, layout):
     want = rotate(x, pos, rot.inv_freq.to(DEV), rot.factor, rot.rotary_dim, layout)
-    bound = rotate_bound(x, want, abs(rot.factor), rot.rotary_dim, layout)
+    bound = rotate_bound(x, want, abs(rot.factor), rot.rotary_dim, layout, pos, rot.inv_freq.to(DEV))
     off = (got.double() - want).abs()
     assert (off <= bound).all(), ((off - bound).max().item(), off.max().item())
 
