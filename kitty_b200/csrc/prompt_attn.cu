@@ -129,6 +129,30 @@ __device__ __forceinline__ uint64_t weights64(const float *v, uint64_t c2, uint6
   return add2(sum[0], sum[1]);
 }
 
+// Four 16-byte words of a thread's row, the same of its three neighbours: after the exchange a thread holds one word of
+// each of the four rows, and a store covers 64 consecutive bytes of eight rows (16 of 32 rows it would be otherwise: four
+// times the passes through the memory pipe, 5000 clocks an item).  dst: the thread's own row, `stride` elements to the next.
+template <typename E>
+__device__ __forceinline__ void store_quad(uint4 (&w)[4], E *dst, int64_t stride, int row, int rows) {
+  const int q = threadIdx.x & 3;
+#pragma unroll
+  for (int bit = 1; bit <= 2; bit <<= 1)
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int lo = bit == 1 ? 2 * n : n, hi = lo + bit;
+      uint4 x = q & bit ? w[lo] : w[hi];
+      x.x = __shfl_xor_sync(0xffffffffu, x.x, bit);
+      x.y = __shfl_xor_sync(0xffffffffu, x.y, bit);
+      x.z = __shfl_xor_sync(0xffffffffu, x.z, bit);
+      x.w = __shfl_xor_sync(0xffffffffu, x.w, bit);
+      if (q & bit) w[lo] = x;
+      else w[hi] = x;
+    }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (row - q + k < rows) *reinterpret_cast<uint4 *>(dst + (k - q) * stride + q * (16 / static_cast<int>(sizeof(E)))) = w[k];
+}
+
 struct Seq {
   int b;              // batch coordinate
   int q0, nq, k0, nk; // first row and rows of its queries and keys
@@ -630,7 +654,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         tc_fence_after();
         const bool mine = row < s.rows;
         const int64_t at_out = (s.out0 + row) * static_cast<int64_t>(a.G) * a.h_kv + head;
-        bool odd = false;
+        const int64_t stride = static_cast<int64_t>(a.G) * a.h_kv * HD;      // from a row of the output to the next
+        float bad = 0.0f;                      // NaN as soon as a value is not finite
         if (a.splits == 1) {
           const float inv = limit > 0 ? 1.0f / l : 0.0f;
           T *dst = static_cast<T *>(a.out) + at_out * HD;
@@ -646,13 +671,10 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
               const float y = limit > 0 ? o[e] * inv : 0.0f;
-              odd |= !(fabsf(y) < INFINITY);
+              bad = fmaf(y, 0.0f, bad);
               t[e] = from_f32<T>(y);
             }
-            if (mine) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) reinterpret_cast<uint4 *>(dst + 32 * i)[e] = w[e];
-            }
+            store_quad(w, dst + 32 * i, stride, row, s.rows);
           }
         } else if (mine) {
           // a part of the keys: the accumulator as it is, the maximum and the sum; no accumulator without a sum
@@ -668,14 +690,17 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             tmem_ld32(to + 32 * i, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) odd |= limit > 0 && !(fabsf(o[e]) < INFINITY);
-            if (mine && limit > j0 * PT) {
+            for (int e = 0; e < 32; ++e) bad = fmaf(o[e], 0.0f, bad);
 #pragma unroll
-              for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(dst + 32 * i + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            for (int y = 0; y < 2; ++y) {
+              uint4 w[4];
+              memcpy(w, o + 16 * y, 64);
+              store_quad(w, dst + 32 * i + 16 * y, stride, row, s.rows);
             }
           }
         }
-        unsigned again = __ballot_sync(0xffffffffu, odd && mine);
+        __syncwarp();
+        unsigned again = __ballot_sync(0xffffffffu, !(bad == 0.0f) && mine && limit > j0 * PT);
         while (again) {
           const int r = __ffs(again) - 1;
           again &= again - 1;
