@@ -439,10 +439,10 @@ int kitty_kv8_expand(const kitty_kv8_layer *layer, const int32_t *lengths, const
 
 /* One query token per row over the tokens the row holds (lengths: device int32 [B]; 0 gives zeros).  query
  * [B, h_q, 1, 128] and out [B, 1, h_q, 128], contiguous, of the layer's type; up to 16 query heads per key head,
- * B <= KITTY_KV8_MAX_BATCH.  workspace: kitty_kv8_workspace_bytes, 16-byte aligned, no initial contents; calls that
- * share one must not overlap. */
+ * B <= KITTY_KV8_MAX_BATCH.  workspace: kitty_kv8_workspace_bytes (0 for caches of short rows: null will do),
+ * 16-byte aligned, no initial contents; calls that share one must not overlap. */
 #define KITTY_KV8_MAX_BATCH 2048
-int64_t kitty_kv8_workspace_bytes(int32_t B, int32_t h_kv, int32_t h_q);
+int64_t kitty_kv8_workspace_bytes(int32_t B, int32_t h_kv, int32_t h_q, int32_t max_page);
 int kitty_kv8_attn(const kitty_kv8_layer *layer, const int32_t *lengths, const void *query, int32_t B, int32_t h_q,
                    float scaling, void *out, void *workspace, int64_t workspace_bytes, void *stream);
 

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libkitty_b200.so")
@@ -69,13 +70,12 @@ class KittyKV8Layer(C.Structure):
                [(n, C.c_void_p) for n in ("pages", "tail_k", "tail_v", "page_table", "status")]
 
 
-_I64 = {n: C.c_int64 * n for n in (9, 12)}
+_I64 = {n: struct.Struct(f"{n}q").pack for n in (9, 12)}
 
 
-def i64_array(values):
+def i64_array(values) -> bytes:
     """HOST array of int64 for the entry points that take strides that way."""
-    n = len(values)
-    return (_I64.get(n) or C.c_int64 * n)(*values)
+    return _I64[len(values)](*values)
 
 
 class KittyError(RuntimeError):
@@ -162,7 +162,7 @@ def lib() -> C.CDLL:
     L.kitty_lse_exchange_merge.argtypes = [vp, i64, vp, i32, i32, i32, vp, C.c_int, vp, i64, vp]
     L.kitty_lse_merge.restype = C.c_int
     L.kitty_lse_merge.argtypes = [vp, i32, i64, vp, C.c_int, vp]
-    rot, kv8, strides = C.POINTER(KittyRotaryPlan), C.POINTER(KittyKV8Layer), C.POINTER(i64)
+    rot, kv8, strides = C.POINTER(KittyRotaryPlan), C.POINTER(KittyKV8Layer), C.c_char_p
     L.kitty_rotary.restype = C.c_int
     L.kitty_rotary.argtypes = [rot, vp, vp, vp, i64, vp, vp, C.c_int, i32, i32, i32, i32, strides, vp]
     L.kitty_prompt_attn.restype = C.c_int
@@ -175,7 +175,7 @@ def lib() -> C.CDLL:
     L.kitty_kv8_expand.restype = C.c_int
     L.kitty_kv8_expand.argtypes = [kv8, vp, vp, vp, vp, i32, i32, vp]
     L.kitty_kv8_workspace_bytes.restype = i64
-    L.kitty_kv8_workspace_bytes.argtypes = [i32, i32, i32]
+    L.kitty_kv8_workspace_bytes.argtypes = [i32, i32, i32, i32]
     L.kitty_kv8_attn.restype = C.c_int
     L.kitty_kv8_attn.argtypes = [kv8, vp, vp, i32, i32, C.c_float, vp, vp, i64, vp]
     _lib = L

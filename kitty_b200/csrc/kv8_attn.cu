@@ -22,10 +22,8 @@
 
 namespace kitty {
 
-#ifndef KV8_WARPS
 constexpr int KV8_WARPS = 12;           // per block of threads, one block per multiprocessor
 constexpr int KV8_STAGES = 2;
-#endif
 constexpr int KV8_MAX_SMS = 160;        // the workspace is sized for this many
 constexpr int KV8_WORKERS_MAX = KV8_MAX_SMS * KV8_WARPS;
 constexpr float KV8_FIX = 32512.0f;     // 127 * 256: both bytes of a fixed-point number stay in -128 .. 127
@@ -116,8 +114,10 @@ struct Kv8Cursor {
     blk = rest - h * nblk;
   }
   // true when the next unit belongs to another row
+  template <bool ROW>
   __device__ __forceinline__ bool next(const Kv8AttnArgs &a, const int32_t *prefix) {
     if (++blk < nblk) return false;
+    if (ROW) return true;
     blk = 0;
     if (++h == a.L.h_kv) {
       h = 0;
@@ -131,13 +131,17 @@ struct Kv8Cursor {
 };
 
 // MT: 1 for groups of up to 8 query heads, 2 for up to 16 (two matrix tiles).
-template <typename T, int MT>
-__global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
+// ROW 0: the even split over the machine described above, W = KV8_WARPS.  ROW 1 (see kv8_by_row): a block
+// of threads per row, whose W warps share the row's blocks and join their parts in shared memory: no line of units to
+// find one's place in, no second kernel.
+template <typename T, int MT, int W, bool ROW>
+__global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) kv8_attn_kernel(const __grid_constant__ Kv8AttnArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t bars[KV8_WARPS][KV8_STAGES];
-  __shared__ int32_t scan[KV8_WARPS];
-  __shared__ int32_t skipped[KV8_WARPS][KV8_STAGES];      // stages without a record
-  int32_t *prefix = reinterpret_cast<int32_t *>(smem + KV8_WARPS * KV8_STAGES * KV8_REC);
+  __shared__ __align__(8) uint64_t bars[W][KV8_STAGES];
+  __shared__ int32_t scan[W];
+  __shared__ int32_t skipped[W][KV8_STAGES];      // stages without a record
+  __shared__ float2 parts[ROW ? W : 1][MAX_GROUP];        // maximum and sum of each warp's part
+  int32_t *prefix = reinterpret_cast<int32_t *>(smem + W * KV8_STAGES * KV8_REC);
   const kitty_kv8_layer &L = a.L;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int H = L.h_kv, B = a.B, G = a.G;
@@ -146,9 +150,20 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __gri
     for (int s = 0; s < KV8_STAGES; ++s) mbar_init(smem_u32(&bars[warp][s]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  // units before each sequence: every block of threads scans the lengths
-  {
-    const int per = (B + KV8_WARPS * 32 - 1) / (KV8_WARPS * 32), i0 = min(B, per * static_cast<int>(threadIdx.x));
+  Kv8Cursor cur;
+  int u0, u1, worker = 0;
+  if constexpr (ROW) {
+    cur.b = blockIdx.x / H;
+    cur.h = blockIdx.x % H;
+    cur.len = kv8_clamp_len(L, a.lengths[cur.b]);
+    cur.nblk = (cur.len + KV8_BLOCK - 1) / KV8_BLOCK;
+    u0 = cur.nblk * warp / W;
+    u1 = cur.nblk * (warp + 1) / W;
+    cur.blk = u0;
+    __syncwarp();
+  } else {
+    // units before each sequence: every block of threads scans the lengths
+    const int per = (B + W * 32 - 1) / (W * 32), i0 = min(B, per * static_cast<int>(threadIdx.x));
     const int i1 = min(B, i0 + per);
     int sum = 0;
     for (int i = i0; i < i1; ++i) {
@@ -170,21 +185,21 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __gri
     if (threadIdx.x == 0) prefix[0] = 0;
     __syncthreads();
     if (blockIdx.x == 0)
-      for (int i = threadIdx.x; i <= B; i += KV8_WARPS * 32) a.prefix[i] = prefix[i];
+      for (int i = threadIdx.x; i <= B; i += W * 32) a.prefix[i] = prefix[i];
+    dep_release();
+    const int units = prefix[B] * H;
+    // neighbouring workers sit on different multiprocessors, so that a few units spread over all of them
+    worker = warp * gridDim.x + blockIdx.x;
+    if (units == 0) return;
+    u0 = kv8_first_unit(worker, units, a.workers);
+    u1 = kv8_first_unit(worker + 1, units, a.workers);
+    if (u0 >= u1) return;
+    cur.seek(u0, a, prefix);
   }
-  dep_release();
-  const int units = prefix[B] * H;
-  // neighbouring workers sit on different multiprocessors, so that a few units spread over all of them
-  const int worker = warp * gridDim.x + blockIdx.x;
-  if (units == 0) return;
-  const int u0 = kv8_first_unit(worker, units, a.workers), u1 = kv8_first_unit(worker + 1, units, a.workers);
-  if (u0 >= u1) return;
 
   const uint8_t *ring_p = smem + warp * KV8_STAGES * KV8_REC;
   const uint32_t ring = smem_u32(ring_p);
-  Kv8Cursor cur, ahead;
-  cur.seek(u0, a, prefix);
-  ahead = cur;
+  Kv8Cursor ahead = cur;
   int ua = u0;
   int64_t page = 0;                        // page row of the unit that is requested next, looked up a unit early
   auto look_up = [&] {
@@ -208,7 +223,7 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __gri
         mbar_expect_tx(bar, 0);
       }
     }
-    ahead.next(a, prefix);
+    ahead.template next<ROW>(a, prefix);
     ++ua;
     look_up();
   };
@@ -278,6 +293,7 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __gri
         mbar_wait(smem_u32(&bars[warp][stage]), phase);
         if (++stage == KV8_STAGES) stage = 0, phase ^= 1;
       }
+      if (ROW) break;                          // the block's barrier is still to come
       return;
     }
     const uint8_t *rec = ring_p + stage * KV8_REC;
@@ -436,8 +452,8 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __gri
     if (ua < u1) request(stage);
     if (++stage == KV8_STAGES) stage = 0, phase ^= 1;
     const int b = cur.b, h = cur.h;
-    const bool ends = cur.next(a, prefix);
-    if (ends || u + 1 == u1) {
+    const bool ends = cur.template next<ROW>(a, prefix);
+    if (!ROW && (ends || u + 1 == u1)) {
       fresh = true;
       const bool all = from_start && ends;          // the whole row: no one else has a part of it
       const int64_t row = static_cast<int64_t>(b) * H + h;
@@ -461,6 +477,46 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 1) kv8_attn_kernel(const __gri
           if (t == 0) *reinterpret_cast<float2 *>(o + HD) = make_float2(mx[m], s);
         }
       }
+    }
+  }
+  if constexpr (ROW) {
+    // the warps' parts, each in its own ring (all its copies are done): accumulators [head][128], (maximum, sum) beside
+    float *mine = reinterpret_cast<float *>(smem + warp * KV8_STAGES * KV8_REC);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int head = g + 8 * m;
+      float s = u0 < u1 ? sum[m] : 0.0f;
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      if (head < G) {
+        if (t == 0) parts[warp][head] = make_float2(u0 < u1 ? mx[m] : -INFINITY, s);
+        if (u0 < u1) {
+#pragma unroll
+          for (int n = 0; n < 16; ++n)
+            *reinterpret_cast<float2 *>(mine + head * HD + 8 * n + 2 * t) = make_float2(acc[n][2 * m], acc[n][2 * m + 1]);
+        }
+      }
+    }
+    __syncthreads();
+    T *out = static_cast<T *>(a.out) + static_cast<int64_t>(blockIdx.x) * G * HD;
+    for (int i = threadIdx.x; i < G * HD / 2; i += W * 32) {
+      const int head = i / (HD / 2);
+      float top = -INFINITY, l = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) top = fmaxf(top, parts[w][head].x);
+      if (top == -INFINITY) top = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if (cur.nblk * w / W == cur.nblk * (w + 1) / W) continue;      // a warp without blocks
+        const float2 p = parts[w][head];
+        const float wgt = ex2(p.x - top);
+        const float2 v = *reinterpret_cast<const float2 *>(smem + w * KV8_STAGES * KV8_REC + i * sizeof(float2));
+        l = fmaf(p.y, wgt, l);
+        x = fmaf(v.x, wgt, x);
+        y = fmaf(v.y, wgt, y);
+      }
+      const float inv = cur.nblk > 0 ? 1.0f / l : 0.0f;
+      *reinterpret_cast<uint32_t *>(out + 2 * i) = pack_t<T>(x * inv, y * inv);
     }
   }
 }
@@ -600,24 +656,46 @@ __global__ void __launch_bounds__(HD * KV8_JOIN_GROUPS) kv8_join_kernel(const __
   static_cast<T *>(a.out)[static_cast<int64_t>(blockIdx.x) * HD + c] = from_f32<T>(nblk > 0 ? tot / l : 0.0f);
 }
 
-template <typename T, int MT>
-int launch_kv8_attn(const Kv8AttnArgs &a, int blocks, int smem, cudaStream_t s) {
+template <typename T, int MT, int W, bool ROW>
+int start_kv8_attn(const Kv8AttnArgs &a, int blocks, cudaStream_t s) {
   static PerDeviceOnce once;
+  constexpr int RING = W * KV8_STAGES * KV8_REC;
   const int rc = per_device_once(once, [] {
-    return cudaFuncSetAttribute(kv8_attn_kernel<T, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                KV8_WARPS * KV8_STAGES * KV8_REC + (KITTY_KV8_MAX_BATCH + 1) * 4) == cudaSuccess
+    return cudaFuncSetAttribute(kv8_attn_kernel<T, MT, W, ROW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                RING + (ROW ? 0 : (KITTY_KV8_MAX_BATCH + 1) * 4)) == cudaSuccess
                ? KITTY_OK
                : KITTY_E_CUDA;
   });
   if (rc != KITTY_OK) return rc;
-  kv8_attn_kernel<T, MT><<<blocks, KV8_WARPS * 32, smem, s>>>(a);
-  if (cudaGetLastError() != cudaSuccess) return KITTY_E_CUDA;
+  kv8_attn_kernel<T, MT, W, ROW><<<blocks, W * 32, RING + (ROW ? 0 : (a.B + 1) * 4), s>>>(a);
+  return cudaGetLastError() == cudaSuccess ? KITTY_OK : KITTY_E_CUDA;
+}
+
+// Whether a call gives every row a block of threads (lengths are on the device: the rule goes by what a row can hold).
+// Up to 1024 tokens a row, while there are at most four rows per multiprocessor: 8 rows of 640 tokens 8.2 us (11.0 evenly
+// split and joined), 256 rows of 1024 16.5 (20.1), but 1024 rows of 640 46.9 (44.5).  Up to 4096, from a row per
+// multiprocessor or nearly on: 128 rows of 4096 26 us (39), 1024 rows of 4096 174 (186), but 8 rows of 4096 20 (12).
+bool kv8_by_row(int64_t rows, int max_page) {
+  const int sms = sm_count();
+  return max_page <= 8 ? rows <= 4 * sms : max_page <= 32 && rows >= sms - sms / 8;
+}
+
+template <typename T, int MT>
+int launch_kv8_attn(const Kv8AttnArgs &a, int blocks, cudaStream_t s) {
+  const int rows = a.B * a.L.h_kv;
+  // Eight warps a row; four (three blocks to a multiprocessor) for short rows when there are more than multiprocessors:
+  // 256 rows of 640 tokens 12.4 us, 14.7 with eight; 256 rows of 2048 32.6, 30.7 with eight.
+  if (kv8_by_row(rows, a.L.max_page))
+    return a.L.max_page > 8 || rows <= blocks ? start_kv8_attn<T, MT, 8, true>(a, rows, s)
+                                              : start_kv8_attn<T, MT, 4, true>(a, rows, s);
+  const int rc = start_kv8_attn<T, MT, KV8_WARPS, false>(a, blocks, s);
+  if (rc != KITTY_OK) return rc;
   // From 256 rows on a row has nine partials or fewer (1776 workers): folded by a warp each (1024 rows: 5 us, 25 us as
   // blocks).  Below, a block each: 1024 threads for a few rows of hundreds of partials (8 rows of 222: 9 us, 16 us with
   // 512 threads), 512 threads when there are more blocks than multiprocessors (64 rows of 28: 7 us, 11 us with 1024).
-  const int heads = a.B * a.L.h_kv * a.G;
+  const int heads = rows * a.G;
   cudaError_t e;
-  if (a.B * a.L.h_kv >= 256) e = launch_after(kv8_join_rows_kernel<T>, dim3((heads + 7) / 8), dim3(256), 0, s, a);
+  if (rows >= 256) e = launch_after(kv8_join_rows_kernel<T>, dim3((heads + 7) / 8), dim3(256), 0, s, a);
   else if (heads > blocks) e = launch_after(kv8_join_kernel<T, 4>, dim3(heads), dim3(HD * 4), 0, s, a);
   else e = launch_after(kv8_join_kernel<T, 8>, dim3(heads), dim3(HD * 8), 0, s, a);
   return (e == cudaSuccess && cudaGetLastError() == cudaSuccess) ? KITTY_OK : KITTY_E_CUDA;
@@ -629,9 +707,10 @@ int64_t kv8_prefix_bytes(int B) { return (static_cast<int64_t>(B) + 1 + 3) / 4 *
 
 using namespace kitty;
 
-extern "C" int64_t kitty_kv8_workspace_bytes(int32_t B, int32_t h_kv, int32_t h_q) {
-  if (B < 0 || h_kv <= 0 || h_q <= 0 || h_q % h_kv != 0) return KITTY_E_BADARG;
+extern "C" int64_t kitty_kv8_workspace_bytes(int32_t B, int32_t h_kv, int32_t h_q, int32_t max_page) {
+  if (B < 0 || h_kv <= 0 || h_q <= 0 || max_page <= 0 || h_q % h_kv != 0) return KITTY_E_BADARG;
   if (h_q / h_kv > MAX_GROUP || B > KITTY_KV8_MAX_BATCH) return KITTY_E_BADSHAPE;
+  if (kv8_by_row(static_cast<int64_t>(B) * h_kv, max_page)) return 0;
   return kv8_prefix_bytes(B) + (KV8_WORKERS_MAX + static_cast<int64_t>(B) * h_kv) * (h_q / h_kv) * PART * 4;
 }
 
@@ -640,11 +719,11 @@ extern "C" int kitty_kv8_attn(const kitty_kv8_layer *layer, const int32_t *lengt
                               void *stream) {
   const int rc = check_kv8_layer(layer);
   if (rc != KITTY_OK) return rc;
-  const int64_t need = kitty_kv8_workspace_bytes(B, layer->h_kv, h_q);
+  const int64_t need = kitty_kv8_workspace_bytes(B, layer->h_kv, h_q, layer->max_page);
   if (need < 0) return static_cast<int>(need);
   if (B > layer->max_bs) return KITTY_E_BADARG;
   if (B == 0) return KITTY_OK;
-  if (!lengths || !query || !out || !workspace) return KITTY_E_BADARG;
+  if (!lengths || !query || !out || (need > 0 && !workspace)) return KITTY_E_BADARG;
   if ((reinterpret_cast<uintptr_t>(query) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return KITTY_E_BADARG;
   if (workspace_bytes < need) return KITTY_E_WORKSPACE;
@@ -656,15 +735,16 @@ extern "C" int kitty_kv8_attn(const kitty_kv8_layer *layer, const int32_t *lengt
   a.lengths = lengths;
   a.q = query;
   a.out = out;
-  a.prefix = static_cast<int32_t *>(workspace);
-  a.partials = reinterpret_cast<float *>(static_cast<char *>(workspace) + kv8_prefix_bytes(B));
+  if (need > 0) {
+    a.prefix = static_cast<int32_t *>(workspace);
+    a.partials = reinterpret_cast<float *>(static_cast<char *>(workspace) + kv8_prefix_bytes(B));
+  }
   a.scale_log2 = scaling * 1.4426950408889634f;
   a.B = B;
   a.G = h_q / layer->h_kv;
   a.workers = sms * KV8_WARPS;
-  const int smem = KV8_WARPS * KV8_STAGES * KV8_REC + (B + 1) * 4;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (layer->dtype == KITTY_F16)
-    return a.G > 8 ? launch_kv8_attn<__half, 2>(a, sms, smem, s) : launch_kv8_attn<__half, 1>(a, sms, smem, s);
-  return a.G > 8 ? launch_kv8_attn<__nv_bfloat16, 2>(a, sms, smem, s) : launch_kv8_attn<__nv_bfloat16, 1>(a, sms, smem, s);
+    return a.G > 8 ? launch_kv8_attn<__half, 2>(a, sms, s) : launch_kv8_attn<__half, 1>(a, sms, s);
+  return a.G > 8 ? launch_kv8_attn<__nv_bfloat16, 2>(a, sms, s) : launch_kv8_attn<__nv_bfloat16, 1>(a, sms, s);
 }

@@ -105,7 +105,7 @@ class KV8Layer:
     def workspace_bytes(self, batch: int, h_q: int) -> int:
         need = self._workspace_need.get((batch, h_q))
         if need is None:
-            need = int(_lib.lib().kitty_kv8_workspace_bytes(batch, self.H_KV, h_q))
+            need = int(_lib.lib().kitty_kv8_workspace_bytes(batch, self.H_KV, h_q, self.MAX_PAGE))
             if need < 0:
                 _lib.check(need, "kitty_kv8_workspace_bytes")
             self._workspace_need[(batch, h_q)] = need
@@ -208,7 +208,7 @@ def kv8_attention(query: torch.Tensor, layer: KV8Layer, lengths: torch.Tensor, s
     elif tuple(out.shape) != (B, 1, h_q, D) or out.dtype != layer.dtype or out.device != layer.device \
             or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {layer.dtype} [{B}, 1, {h_q}, {D}] on {layer.device}")
-    ws = _lib.empty((need,), torch.uint8, layer.device)
+    ws = _lib.empty((need,), torch.uint8, layer.device) if need else None
     _lib.call_on(layer.device, _lib.lib().kitty_kv8_attn, "kitty_kv8_attn", layer.c_layer(), lengths.data_ptr(),
-                 q.data_ptr(), B, h_q, float(scaling), out.data_ptr(), ws.data_ptr(), need)
+                 q.data_ptr(), B, h_q, float(scaling), out.data_ptr(), None if ws is None else ws.data_ptr(), need)
     return out

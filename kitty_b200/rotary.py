@@ -174,11 +174,13 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
     if T > 1 and positions.stride(-1) != 1:
         positions = positions.contiguous()
     if query_out is None:
-        qo, qo_st = _lib.head_rows(torch.empty_like(q))
+        qo = torch.empty_like(q)
+        qo_st = q_st if qo.stride() == q.stride() else _lib.head_rows(qo)[1]
     else:
         qo, qo_st = _rotary_output(query_out, query, "query")
     if key_out is None:
-        ko, ko_st = _lib.head_rows(torch.empty_like(k))
+        ko = torch.empty_like(k)
+        ko_st = k_st if ko.stride() == k.stride() else _lib.head_rows(ko)[1]
     else:
         ko, ko_st = _rotary_output(key_out, key, "key")
     strides = _lib.i64_array(q_st + k_st + qo_st + ko_st)

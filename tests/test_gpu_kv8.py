@@ -168,10 +168,12 @@ def _attention_check(got, q, layer, lengths, tails, scaling):
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("H,hq", [(1, 1), (2, 8), (1, 7), (1, 8), (2, 18), (1, 16)])
-@pytest.mark.parametrize("lengths", [[1], [31, 32, 33], [0, 517, 64, 0, 130], [1700]])
-def test_attention(kb, dtype, H, hq, lengths):
-    B, L = len(lengths), max(lengths)
-    k, v = _kv(B, H, L, dtype, L + hq)
+@pytest.mark.parametrize("room", [0, 4100])
+@pytest.mark.parametrize("lengths", [[1], [31, 32, 33], [0, 517, 64, 0, 130], [1700], [1024, 992]])
+def test_attention(kb, dtype, H, hq, lengths, room):
+    """room: caches with place for short rows only and for long ones go different ways."""
+    B, L = len(lengths), max(lengths) + room
+    k, v = _kv(B, H, max(lengths), dtype, max(lengths) + hq)
     q = (0.7 * torch.randn(B, hq, 1, 128, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV)).to(dtype)
     layer = kb.KV8Layer(B, L, H, dtype=dtype, device=DEV, page_table=_scattered(B, -(-L // 128)))
     n = _i32(lengths)
@@ -183,6 +185,20 @@ def test_attention(kb, dtype, H, hq, lengths):
     _attention_check(got, q, layer, lengths, (k, v), SC)
     out = torch.empty_like(got)
     assert kb.kv8_attention(q, layer, n, SC, out=out) is out and torch.equal(out, got)       # the same bits again
+    layer.check()
+
+
+@pytest.mark.parametrize("cap", [256, 1280, 4224])
+def test_attention_many_short_rows(kb, cap):
+    """More rows than multiprocessors, in caches with place for a little and for more."""
+    dtype, B = torch.float16, 90
+    lengths = [(53 * i) % 257 for i in range(B)]
+    layer = kb.KV8Layer(B, cap, 2, dtype=dtype, device=DEV, page_table=_scattered(B, cap // 128))
+    k, v = _kv(B, 2, 256, dtype, 3)
+    n = _i32(lengths)
+    kb.kv8_append(layer, k, v, torch.zeros_like(n), lengths=n)
+    q = torch.randn(B, 14, 1, 128, device=DEV).to(dtype)
+    _attention_check(kb.kv8_attention(q, layer, n, SC), q, layer, lengths, (k, v), SC)
     layer.check()
 
 

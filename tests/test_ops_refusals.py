@@ -93,14 +93,16 @@ def test_kv8_entry_points(L):
     for kw in (dict(lens=None), dict(k=None), dict(v=P + 8), dict(B=5), dict(n=-1)):
         assert expand(good, **kw) == L.KITTY_E_BADARG, kw
     assert expand(good, n=0) == L.KITTY_OK
-    for kw in (dict(lens=None), dict(q=None), dict(q=P + 4), dict(out=None), dict(ws=None), dict(B=5), dict(hq=3), dict(hq=0)):
+    for kw in (dict(lens=None), dict(q=None), dict(q=P + 4), dict(out=None), dict(B=5), dict(hq=3), dict(hq=0)):
         assert attn(good, **kw) == L.KITTY_E_BADARG, kw
     assert attn(good, hq=34) == L.KITTY_E_BADSHAPE
-    assert attn(good, nbytes=100) == L.KITTY_E_WORKSPACE
+    assert attn(_layer(L, max_page=64), nbytes=100) == L.KITTY_E_WORKSPACE
+    assert attn(_layer(L, max_page=64), ws=None) == L.KITTY_E_BADARG
     assert attn(good, B=0) == L.KITTY_OK
-    assert lib.kitty_kv8_workspace_bytes(1, 2, 3) == L.KITTY_E_BADARG
-    assert lib.kitty_kv8_workspace_bytes(L.KV8_MAX_BATCH + 1, 2, 4) == L.KITTY_E_BADSHAPE
-    assert lib.kitty_kv8_workspace_bytes(128, 8, 32) > lib.kitty_kv8_workspace_bytes(1, 8, 32) > 0
+    need = lib.kitty_kv8_workspace_bytes
+    assert need(1, 2, 3, 64) == need(1, 2, 4, 0) == L.KITTY_E_BADARG
+    assert need(L.KV8_MAX_BATCH + 1, 2, 4, 64) == L.KITTY_E_BADSHAPE
+    assert need(128, 8, 32, 64) > need(1, 8, 32, 64) > 0 and need(128, 8, 32, 8) == 0
 
 
 def test_struct_sizes(L):
