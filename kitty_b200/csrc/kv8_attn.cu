@@ -677,7 +677,7 @@ int start_kv8_attn(const Kv8AttnArgs &a, int blocks, cudaStream_t s) {
 // multiprocessor or nearly on: 128 rows of 4096 26 us (39), 1024 rows of 4096 174 (186), but 8 rows of 4096 20 (12).
 bool kv8_by_row(int64_t rows, int max_page) {
   const int sms = sm_count();
-  return max_page <= 8 ? rows <= 4 * sms : max_page <= 32 && rows >= sms - sms / 8;
+  return max_page <= 8 ? rows <= 4 * sms : max_page <= 32 && rows >= sms - sms / 4;
 }
 
 template <typename T, int MT>

@@ -102,7 +102,7 @@ def test_kv8_entry_points(L):
     need = lib.kitty_kv8_workspace_bytes
     assert need(1, 2, 3, 64) == need(1, 2, 4, 0) == L.KITTY_E_BADARG
     assert need(L.KV8_MAX_BATCH + 1, 2, 4, 64) == L.KITTY_E_BADSHAPE
-    assert need(128, 8, 32, 64) > need(1, 8, 32, 64) > 0 and need(128, 8, 32, 8) == 0
+    assert need(128, 8, 32, 64) > need(1, 8, 32, 64) > 0 and need(1, 8, 32, 8) == need(32, 8, 32, 32) == 0
 
 
 def test_struct_sizes(L):
