@@ -9,6 +9,8 @@ import ctypes as C
 import os
 import struct
 
+import torch
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libkitty_b200.so")
 
@@ -191,11 +193,12 @@ def check(status: int, where: str) -> None:
         raise KittyError(int(status), where)
 
 
-def dtype_code(dtype) -> int:
-    import torch
+_DTYPES = {torch.float16: KITTY_F16, torch.bfloat16: KITTY_BF16, torch.float32: KITTY_F32}
 
+
+def dtype_code(dtype) -> int:
     try:
-        return {torch.float16: KITTY_F16, torch.bfloat16: KITTY_BF16, torch.float32: KITTY_F32}[dtype]
+        return _DTYPES[dtype]
     except KeyError:
         raise TypeError(f"kitty_b200 supports float16, bfloat16 and float32 tensors, got {dtype}") from None
 
@@ -223,29 +226,26 @@ def head_rows(x, repeated: bool = True):
         if d == 1 and not (a | b | c) & (15 // x.element_size()) and not x.data_ptr() & 15 \
                 and (repeated or (a or n < 2) and (b or m < 2) and (c or t < 2)):
             break
-        import torch
-
         x = x.clone(memory_format=torch.contiguous_format)
     return x, (a, b, c)
 
 
 def empty(shape, dtype, device):
     """torch.empty for a contiguous tensor by the way that costs least on the host."""
-    import torch
-
-    strides, n = [], 1
-    for d in reversed(shape):
-        strides.append(n)
-        n *= d if d > 1 else 1
-    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=device)
+    if len(shape) == 4:
+        _n, h, t, d = shape
+        strides = (h * t * d, t * d, d, 1)
+    elif len(shape) == 3:
+        strides = (shape[1] * shape[2], shape[2], 1)
+    else:
+        strides = (1,)
+    return torch.empty_strided(shape, strides, dtype=dtype, device=device)
 
 
 def call_on(device, fn, where: str, *args) -> None:
     """Call an entry point with the current stream of `device` (a CUDA device with an index) as its last argument and
     that device current, and raise if it refuses.  A small call costs more on the host than on the device, so the device
     is switched only where it has to be."""
-    import torch
-
     index = device.index
     stream = torch._C._cuda_getCurrentRawStream(index)
     if torch._C._cuda_getDevice() == index:
@@ -258,6 +258,4 @@ def call_on(device, fn, where: str, *args) -> None:
 
 
 def stream_ptr(device) -> int:
-    import torch
-
     return torch.cuda.current_stream(device).cuda_stream
