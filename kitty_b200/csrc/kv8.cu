@@ -127,9 +127,17 @@ __global__ void __launch_bounds__(256, APPEND_BLOCKS<MODE>) kv8_append_kernel(co
     // keys: thread t of token tk holds chunks of eight channels, chunk c from 16t + 8 (c & 1) + 64 (c >> 1)
     const int tk = tid >> 2, t = tid & 3, ik = t0 + tk;
     const bool fresh = ik >= 0 && ik < n, kept = ik < 0 && full;
+    const bool whole = t0 >= 0 && t0 + KV8_BLOCK <= n;  // all tokens of the block come with the call
     auto channel = [&](int c) { return (c >> 1) * 64 + 16 * t + (c & 1) * 8; };
     T *tail_k = static_cast<T *>(L.tail_k) + tail_row + tk * HD;
+    const T *in_k = static_cast<const T *>(a.k) + b * a.ks[0] + ik * a.ks[2] + 16 * t;
     auto fetch_k = [&](int h, uint4 (&w)[4]) {
+      if (whole) {
+        const T *src = in_k + h * a.ks[1];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w[c] = *reinterpret_cast<const uint4 *>(src + (c >> 1) * 64 + (c & 1) * 8);
+        return;
+      }
       const T *src = fresh ? static_cast<const T *>(a.k) + b * a.ks[0] + h * a.ks[1] + ik * a.ks[2]
                            : tail_k + static_cast<int64_t>(h) * KV8_BLOCK * HD;
 #pragma unroll
@@ -138,15 +146,21 @@ __global__ void __launch_bounds__(256, APPEND_BLOCKS<MODE>) kv8_append_kernel(co
     // values: a warp's lane holds four channels of eight tokens
     const int iv = t0 + 8 * warp;
     T *tail_v = static_cast<T *>(L.tail_v) + tail_row + 8 * warp * HD + 4 * lane;
+    const T *in_v = static_cast<const T *>(a.v) + b * a.vs[0] + iv * a.vs[2] + 4 * lane;
     auto fetch_v = [&](int h, uint4 (&w)[4]) {
-      const T *in = static_cast<const T *>(a.v) + b * a.vs[0] + h * a.vs[1] + 4 * lane;
+      const T *in = in_v + h * a.vs[1];
       uint2 z[8];
+      if (whole) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = iv + j;
-        z[j] = make_uint2(0, 0);
-        if (i >= 0 && i < n) z[j] = *reinterpret_cast<const uint2 *>(in + i * a.vs[2]);
-        else if (i < 0 && full) z[j] = *reinterpret_cast<const uint2 *>(tail_v + (static_cast<int64_t>(h) * KV8_BLOCK + j) * HD);
+        for (int j = 0; j < 8; ++j) z[j] = *reinterpret_cast<const uint2 *>(in + j * a.vs[2]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int i = iv + j;
+          z[j] = make_uint2(0, 0);
+          if (i >= 0 && i < n) z[j] = *reinterpret_cast<const uint2 *>(in + j * a.vs[2]);
+          else if (i < 0 && full) z[j] = *reinterpret_cast<const uint2 *>(tail_v + (static_cast<int64_t>(h) * KV8_BLOCK + j) * HD);
+        }
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) w[c] = make_uint4(z[2 * c].x, z[2 * c].y, z[2 * c + 1].x, z[2 * c + 1].y);
@@ -335,19 +349,22 @@ __global__ void __launch_bounds__(256, APPEND_BLOCKS<MODE>) kv8_append_kernel(co
             }
             transpose4(code, out[y]);
           }
-          // channel c: piece c / 16, half (c / 8) % 2, lane 4 (c % 8) + the tokens' eight (the warp)
+          // channel c: piece row c / 16, half (c / 8) % 2, lane 4 (c % 8) + the tokens' eight (the warp); the lane's place in
+          // its row is turned by the row, so that the eight rows a warp writes to fall on different banks
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int c = 4 * lane + j;
-            *reinterpret_cast<uint2 *>(vt + (c >> 4) * 512 + (4 * (c & 7) + warp) * 16 + ((c >> 3) & 1) * 8) = make_uint2(out[0][j], out[1][j]);
+            *reinterpret_cast<uint2 *>(vt + (c >> 4) * 512 + ((4 * (c & 7) + warp) ^ (c >> 4)) * 16 + ((c >> 3) & 1) * 8) = make_uint2(out[0][j], out[1][j]);
           }
           half_barrier(1);
           if (page >= 0) {
             uint8_t *rec = kv8_record(L, page, h, blk & 3);
             if (tid == 0) *reinterpret_cast<float *>(rec + KV8_OFF_SCALE + 4) = scale;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-              *reinterpret_cast<uint4 *>(rec + KV8_OFF_V + (tid + 128 * j) * 16) = *reinterpret_cast<const uint4 *>(vt + (tid + 128 * j) * 16);
+            for (int j = 0; j < 2; ++j) {
+              const int p = tid + 128 * j;
+              *reinterpret_cast<uint4 *>(rec + KV8_OFF_V + p * 16) = *reinterpret_cast<const uint4 *>(vt + (p ^ (p >> 5)) * 16);
+            }
           }
         }
 #pragma unroll
