@@ -89,7 +89,7 @@ __device__ __forceinline__ float kv8_scale(uint32_t m, float &inv, float &pre) {
 __device__ __forceinline__ uint32_t max_abs16(uint32_t m, uint32_t w) { return __vmaxu2(m, w & 0x7fff7fffu); }
 
 // Blocks of threads per multiprocessor: four (64 registers) hide more of the memory's latency than three without spills
-// (4 x 4096 rotated tokens, 8 heads: 26.0 against 28.6 us); the scalar forms have more state and take two.
+// (4 x 4096 rotated tokens, 8 heads: 24 against 28 us); the scalar forms have more state and take two.
 template <int MODE>
 constexpr int APPEND_BLOCKS = MODE == ROT_NONE || MODE == ROT_HALF || MODE == ROT_INTER ? 4 : 2;
 
@@ -545,9 +545,14 @@ extern "C" int kitty_kv8_append(const kitty_kv8_layer *layer, const void *key, c
   a.h_q = h_q;
   const int64_t blocks = (static_cast<int64_t>(T) + 2 * KV8_BLOCK - 2) / KV8_BLOCK;   // that T tokens can touch
   if (B > 65535 || T > (1 << 30)) return KITTY_E_BADSHAPE;
-  // Heads are spread over blocks of threads until there are four per multiprocessor; the rest share an angle table
-  // (4 x 4096 tokens: 26 us; with 14 per multiprocessor, a head or two each, 32 us).
-  int64_t split = (4 * static_cast<int64_t>(sm_count()) + blocks * B - 1) / (blocks * B);
+  // Heads are spread over blocks of threads until there are three per multiprocessor; the rest share an angle table.
+  // From a cold L2, in us, by the blocks asked for per multiprocessor (8 heads; q: with 32 query heads):
+  //                    1     2     3     4
+  //   4 x 4096        27.8  27.9  27.9  29.8
+  //   3 x 2000        26.0  20.8  19.5  22.4
+  //   16 x 512, q     56.0  47.2  47.3  60.5
+  //   1 x 4096, q     33.5  32.4  30.0  30.0
+  int64_t split = (3 * static_cast<int64_t>(sm_count()) + blocks * B - 1) / (blocks * B);
   if (split > layer->h_kv) split = layer->h_kv;
   a.heads = static_cast<int32_t>((layer->h_kv + split - 1) / split);
   split = (layer->h_kv + a.heads - 1) / a.heads;
