@@ -352,7 +352,7 @@ typedef enum {
 
 typedef struct {
   const double *turns;   /* DEVICE array [rotary_dim / 2]: w_p / (2 pi), the turns per position of each pair */
-  const double *steps;   /* DEVICE array [32][rotary_dim / 2][2], 16-byte aligned: cos(i w_p), sin(i w_p), i = 0 .. 31 */
+  const double *steps;   /* DEVICE array [8][rotary_dim / 2][2], 16-byte aligned: cos(i w_p), sin(i w_p), i = 0 .. 7 */
   float factor;          /* on cosine and sine (1 unless the scaling asks for more)                        */
   int32_t rotary_dim;    /* even, 2 .. 128                                                                  */
   int32_t layout;        /* kitty_rope_layout                                                               */

@@ -105,7 +105,6 @@ __global__ void __launch_bounds__(256, APPEND_BLOCKS<MODE>) kv8_append_kernel(co
   __shared__ __align__(16) uint8_t vt[KV8_OFF_V];
   __shared__ __align__(16) T stage[HALF ? KV8_BLOCK : 1][HD + 8];
   __shared__ uint32_t red[2][8];
-  __shared__ double2 base[MODE == ROT_NONE ? 1 : HD / 2];
   const kitty_kv8_layer &L = a.L;
   const int b = blockIdx.z, cap = L.max_page * PAGE;
   int n = a.counts != nullptr ? a.counts[b] : a.T;
@@ -171,15 +170,15 @@ __global__ void __launch_bounds__(256, APPEND_BLOCKS<MODE>) kv8_append_kernel(co
       else fetch_v(h0, w);
     }
     if constexpr (MODE != ROT_NONE) {
-      // a block starts at a multiple of 32: its angles are one sine and cosine per pair and the table of steps
-      static_assert(KV8_BLOCK == ROT_STEPS);
-      const int last = rows_q ? a.T : n;
-      if (threadIdx.x < np) base[threadIdx.x] = rot_base(a.pl, static_cast<int64_t>(blk) * KV8_BLOCK, threadIdx.x);
-      __syncthreads();
-      for (int i = threadIdx.x; i < KV8_BLOCK * (HD / 2); i += 256) {
-        const int tk = i / (HD / 2), p = i % (HD / 2);
-        if (p < np && t0 + tk >= 0 && t0 + tk < last)
-          reinterpret_cast<float2 *>(tab)[2 * BlockTable<T, MODE>::word(p, tk) + (p & 1)] = rot_step(a.pl, base[p], tk, p);
+      // a thread makes the angles of one pair and eight tokens: one sine and cosine at a multiple of eight, and the steps
+      static_assert(256 * ROT_STEPS == KV8_BLOCK * (HD / 2) && KV8_BLOCK % ROT_STEPS == 0);
+      const int last = rows_q ? a.T : n, p = threadIdx.x % (HD / 2), tk = threadIdx.x / (HD / 2) * ROT_STEPS;
+      if (p < np) {
+        const double2 base = rot_base(a.pl, static_cast<int64_t>(blk) * KV8_BLOCK + tk, p);
+#pragma unroll
+        for (int i = 0; i < ROT_STEPS; ++i)
+          if (t0 + tk + i >= 0 && t0 + tk + i < last)
+            reinterpret_cast<float2 *>(tab)[2 * BlockTable<T, MODE>::word(p, tk + i) + (p & 1)] = rot_step(a.pl, base, i, p);
       }
       __syncthreads();
     }
@@ -552,6 +551,7 @@ extern "C" int kitty_kv8_append(const kitty_kv8_layer *layer, const void *key, c
   //   3 x 2000        26.0  20.8  19.5  22.4
   //   16 x 512, q     56.0  47.2  47.3  60.5
   //   1 x 4096, q     33.5  32.4  30.0  30.0
+  // (taken with a slower way to the angles, 26.9 in place of 27.9 since.)
   int64_t split = (3 * static_cast<int64_t>(sm_count()) + blocks * B - 1) / (blocks * B);
   if (split > layer->h_kv) split = layer->h_kv;
   a.heads = static_cast<int32_t>((layer->h_kv + split - 1) / split);

@@ -5,9 +5,10 @@
 // with channels (p, p + rotary_dim/2) ("half") or (2p, 2p + 1) ("interleaved"); channels from rotary_dim on keep
 // their value.  The plan holds w_p in TURNS per position (w_p / 2 pi, 64 bits): position * turns loses its whole part
 // exactly in 64 bits, and an angle is off by 2^-51 of the position times w at most (a 32-bit product is off by 0.004 rad
-// at position 100000).  Sine and cosine are 64-bit too: those of the position's multiple of 32 are computed, those of the
-// rest come from the plan's table of small steps and are turned on with four multiplications; a block of 32 tokens so
-// needs one sine and cosine per pair.  Both round to 32 bits once, to half a step.  (With 32-bit sines the turned keys
+// at position 100000).  Sine and cosine are 64-bit too: those of the position's multiple of eight are computed, those of
+// the rest come from the plan's table of eight small steps and are turned on with four multiplications.  (A table of 32
+// steps has a block of 32 tokens compute a quarter of the sines, but in a quarter of its threads and with four times the
+// loads: 4 x 4096 tokens appended in 27.8 us against 26.9 from a cold L2.)  Both round to 32 bits once, to half a step.  (With 32-bit sines the turned keys
 // were off by up to 2^-22, and four times as many of them fell on the other side of a rounding to 16 bits as with exact
 // ones.)  The rotation itself is two fused multiply-adds in 32 bits, rounded once to the data type.
 #pragma once
@@ -48,9 +49,9 @@ struct RotTable {
   __device__ __forceinline__ float2 one(int p) const { return tab[p]; }
 };
 
-constexpr int ROT_STEPS = 32;
+constexpr int ROT_STEPS = 8;
 
-// Factor times cosine and sine of pair p at a multiple of 32, and with the remaining steps turned on.
+// Factor times cosine and sine of pair p at a multiple of eight, and with the remaining steps turned on.
 __device__ __forceinline__ double2 rot_base(const kitty_rotary_plan &pl, int64_t pos, int p) {
   double t = static_cast<double>(pos) * pl.turns[p];
   t -= rint(t);

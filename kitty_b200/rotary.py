@@ -105,7 +105,7 @@ class RotaryEmbedding:
         self.inv_freq = torch.tensor(inv, dtype=torch.float64)                  # radians per position, on the host
         self._turns = torch.tensor([w / (2 * math.pi) for w in inv], dtype=torch.float64, device=dev)
         self.device = self._turns.device
-        step = torch.arange(32, dtype=torch.float64)[:, None] * self.inv_freq
+        step = torch.arange(8, dtype=torch.float64)[:, None] * self.inv_freq
         self._steps = torch.stack((torch.cos(step), torch.sin(step)), -1).to(dev).contiguous()
         self._c_plan = _lib.KittyRotaryPlan(self._turns.data_ptr(), self._steps.data_ptr(), self.factor, rotary_dim, ROPE_LAYOUTS[layout], 0)
 
