@@ -203,6 +203,14 @@ def dtype_code(dtype) -> int:
         raise TypeError(f"kitty_b200 supports float16, bfloat16 and float32 tensors, got {dtype}") from None
 
 
+def refuse_gradients(where: str, *tensors) -> None:
+    """The operators are for serving: a result without a gradient where one is expected would be a silent mistake."""
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x.requires_grad:
+                raise ValueError(f"{where} has no backward pass: call it under torch.no_grad() or with detached tensors")
+
+
 def head_rows(x, repeated: bool = True):
     """x [B, H, T, 128], or [T, H, 128] for a packed batch, as the kernels read it, and its (batch, head, token) strides
     (0 where a dimension has size one: views may carry any number there).  That is x itself when its channels are

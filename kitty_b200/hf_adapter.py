@@ -100,7 +100,8 @@ def kitty_attention_module_forward(self, hidden_states, position_embeddings=None
     is_prefill = past_key_values.update(k, v, self.layer_idx)
     if is_prefill:
         if (getattr(self, "kitty_prompt_kernel", False) and attention_mask is None and q.is_cuda and q.shape[-1] == 128
-                and q.dtype in (torch.float16, torch.bfloat16)):
+                and q.dtype in (torch.float16, torch.bfloat16)
+                and not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad))):
             out = prompt_attention(q, k, v, self.scaling)
         else:
             out = _prefill_attention(q, k, v, attention_mask, self.scaling).transpose(1, 2)
@@ -128,7 +129,8 @@ def _fused_step_ok(cache, layer_idx: int, q, k, v) -> bool:
 
 def patch_model(model, prompt_kernel: bool = False) -> int:
     """Install the Kitty call sequence on every self-attention module of `model`.  Returns how many were patched.
-    prompt_kernel: 16-bit prompts without a mask go through `prompt_attention` instead of torch's attention."""
+    prompt_kernel: 16-bit prompts without a mask, and without gradients, go through `prompt_attention` instead of torch's
+    attention."""
     n = 0
     cfg = model.config.get_text_config() if hasattr(model.config, "get_text_config") else model.config
     for mod in model.modules():

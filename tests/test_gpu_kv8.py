@@ -154,7 +154,7 @@ def _attention_check(got, q, layer, lengths, tails, scaling):
             qx, kx, vx = q[b, x].double(), kk[x // G], vv[x // G]
             want, mag = attend_fast(qx, kx, vx, scaling, torch.tensor([n], device=DEV))
             # query elements are within half of (largest of the head) / 32512 of their value, 2^-15.98 of the largest
-            delta = logit_error(qx, kx, scaling) + 2.0 ** -15.9 * (qx.abs().max() * kx.abs().sum(1).max()).item() * scaling
+            delta = logit_error(qx, kx, scaling) + 2.0 ** -15.9 * (qx.abs().max() * kx.abs().sum(1).max()).item() * abs(scaling)
             # weights within the same part of their block's largest; those of the open block are sums of two 16-bit numbers
             # (2^-16 of their own size)
             bound = attention_bound(want, mag, q.dtype, 2.0 ** -16, delta)
@@ -393,3 +393,33 @@ def test_a_replaced_page_table_is_used_and_checked(kb):
     layer.page_table = torch.zeros(1, 3, dtype=torch.int64, device=DEV)
     with pytest.raises(ValueError, match="page_table"):
         kb.kv8_append(layer, k, v, _i32([0]))
+
+
+def test_tensors_that_want_a_gradient_are_refused(kb):
+    lay = kb.KV8Layer(1, 128, 1, device=DEV)
+    rot, z = kb.RotaryEmbedding(device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    x, g = (torch.randn(1, 1, 1, 128, device=DEV).bfloat16().requires_grad_(want) for want in (False, True))
+    pos = torch.zeros(1, dtype=torch.int64, device=DEV)
+    calls = [lambda: kb.kv8_append(lay, g, x, z), lambda: kb.kv8_append(lay, x, g, z),
+             lambda: kb.kv8_append(lay, x, x, z, rotary=rot, query=g), lambda: kb.kv8_attention(g, lay, z, 1.0),
+             lambda: kb.apply_rotary(g, x, pos, rot), lambda: kb.apply_rotary(x, g, pos, rot)]
+    for call in calls:
+        with pytest.raises(ValueError, match="no backward pass"):
+            call()
+        with torch.no_grad():
+            call()
+    lay.check()
+
+
+@pytest.mark.parametrize("room", [0, 4100])
+@pytest.mark.parametrize("scaling", [0.0, -0.3, 1e-30, 3.0])
+def test_scalings_of_any_sign_and_size(kb, scaling, room):
+    """Zero is the mean of the values, a negative one turns the order around, a large one picks a few tokens."""
+    lengths = [333, 0, 45]
+    layer = kb.KV8Layer(3, 333 + room, 2, device=DEV)
+    k, v = _kv(3, 2, 333, torch.bfloat16, 9)
+    n = _i32(lengths)
+    kb.kv8_append(layer, k, v, torch.zeros_like(n), lengths=n)
+    q = torch.randn(3, 6, 1, 128, generator=torch.Generator(device=DEV).manual_seed(2), device=DEV).bfloat16()
+    _attention_check(kb.kv8_attention(q, layer, n, scaling), q, layer, lengths, (k, v), scaling)
+    layer.check()

@@ -157,3 +157,18 @@ def test_scaled_frequencies_match_transformers():
             inv, f = _scaled_frequencies(128, base, scaling)
             got = torch.tensor(inv, dtype=torch.float64)
             assert ((got - want.double()).abs() <= 2.0 ** -20 * got).all() and abs(f - factor) < 1e-12
+
+
+def test_gradients_are_refused(L):
+    import kitty_b200 as kb
+
+    x = torch.zeros(1, 1, 2, 128, dtype=torch.bfloat16)
+    for i in range(3):
+        a = [x.clone().requires_grad_(j == i) for j in range(3)]
+        with pytest.raises(ValueError, match="no backward pass"):
+            kb.prompt_attention(*a, 1.0)
+        with torch.no_grad(), pytest.raises(ValueError, match="no CPU path"):
+            kb.prompt_attention(*a, 1.0)
+    L.refuse_gradients("it", x)
+    with pytest.raises(ValueError, match="it has no backward pass"):
+        L.refuse_gradients("it", x, x.clone().requires_grad_())
