@@ -13,6 +13,7 @@
 //                    same columns as 16-bit numbers, as the left operand of the second product.
 //   warp 8           tiled bulk copies: both query tiles, then key and value tiles through a ring of 32 KB stages
 //   warp 9           issues the products; tensor memory: logits A, B and accumulators A, B, 128 columns each
+//   warps 10, 11     take what is not finite out of value tiles that some row does not see all of, half a tile each
 //
 // The running maximum is kept in the logits' own units and allowed to lag: the accumulator is rescaled only when a row's
 // maximum has grown by more than 2^8, by the softmax threads themselves (the product before is complete by then: the
@@ -21,8 +22,13 @@
 // large as the rounding of the output itself).
 //
 // Keys that a row does not see: their logits are replaced before the maximum is taken, so keys may hold anything.  Their
-// values enter the product with weight zero, and zero times infinity or NaN is NaN: a row that ends up with a value that
-// is not finite is looked at again, and computed without the matrix units if one of its unseen values is the cause.
+// values enter the product with weight zero, and zero times infinity or NaN is NaN.  So in the value tiles that some row
+// of the two query tiles does not see all of (three at most: the diagonal, or the last one), infinities and NaN become
+// zeros in shared memory before the product, and the keys that held one are noted.  A row that sees such a key has them
+// added to its accumulator at the end: what is not finite stays so under any weight, so the sum of the numbers
+// themselves is the result.  Padding, the next sequence of a packed batch and later tokens cost no more for what they hold.  The
+// two warps look at a tile while the step before it runs: 4 x 4096 tokens take 468 us with them, 469 without (asked for
+// only when the tile's own step began, and with a test per word instead of a multiply-add, 487).
 #include <cuda.h>
 
 #include "decode.cuh"
@@ -34,7 +40,8 @@ constexpr int PT = 128;                        // rows of a query tile, keys of 
 constexpr int TILE_BYTES = PT * HD * 2;        // 32 KB
 constexpr int KV_STAGES = 5;
 constexpr int PROMPT_SMEM = (2 + KV_STAGES) * TILE_BYTES + 1024;
-constexpr int PROMPT_THREADS = 384;            // three groups of four warps; warps 10 and 11 only hand over registers
+constexpr int PROMPT_THREADS = 384;            // three groups of four warps
+constexpr int CLEAN_TILES = 3;                 // value tiles of an item that some row does not see all of, at most
 constexpr float LAG = 8.0f;                    // log2 of how far a maximum may lag
 
 struct PromptArgs {
@@ -168,55 +175,89 @@ __device__ __forceinline__ int key_limit(const Seq &s, int i, int causal) {
   return causal ? clampi(i + 1 + s.nk - s.nq, 0, s.nk) : s.nk;
 }
 
-// One row again, by one warp, without the matrix units: only keys that the row sees are touched.  Keys lo .. hi - 1 were
-// multiplied; the row sees those below limit.
+// What an item's value tiles held that is not finite.
+struct Odd {
+  uint32_t rows[2][4 * CLEAN_TILES];   // by half of the channels: bits of the keys, from key tile0 * 128 on
+  const void *v;                       // the first of the sequence's value rows
+  int tile0, nk;
+};
+
+// x * 0 + acc on two 16-bit numbers: NaN from the first x on that is not finite.
 template <typename T>
-__device__ __noinline__ void repair_row(const PromptArgs &a, const Seq &s, int row, int head, int limit, int lo, int hi, int z) {
-  const int lane = threadIdx.x & 31;
-  const int hk = head / a.G;
-  const T *k = static_cast<const T *>(a.k) + s.b * a.ks[0] + hk * a.ks[1] + s.k0 * a.ks[2] + 4 * lane;
-  const T *v = static_cast<const T *>(a.v) + s.b * a.vs[0] + hk * a.vs[1] + s.k0 * a.vs[2] + 4 * lane;
-  auto load4 = [](const T *p, float (&x)[4]) {
-    T t[4];
-    *reinterpret_cast<uint2 *>(t) = *reinterpret_cast<const uint2 *>(p);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = to_f32<T>(t[e]);
+__device__ __forceinline__ uint32_t stain2(uint32_t x, uint32_t acc) {
+  if constexpr (__is_same(T, __half)) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(x), "r"(0));
+  else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(x), "r"(0));
+  return acc;
+}
+
+// Half a value tile (128 rows of 128 bytes) in shared memory, by one warp: numbers that are not finite become zero, and
+// the bits of their rows are set in `rows`.
+template <typename T>
+__device__ __forceinline__ void clear_odd_values(uint32_t half, uint32_t *rows) {
+  constexpr uint32_t EXP = __is_same(T, __half) ? 0x7c007c00u : 0x7f807f80u, ONE = __is_same(T, __half) ? 0x04000400u : 0x00800080u;
+  // an exponent of all ones, and only that, carries into the sign's place
+  auto odd = [](uint32_t x) { return ((x & EXP) + ONE) & 0x80008000u; };
+  auto load = [](uint32_t at, uint32_t (&w)[4]) {
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
   };
-  bool cause = false;
-  float x[4];
-  for (int j = max(limit, lo); j < hi; ++j) {
-    load4(v + j * a.vs[2], x);
+  const int lane = threadIdx.x & 31;
+  const uint32_t at = half + lane * 16;
+  uint32_t acc[4] = {};
+#pragma unroll 1
+  for (int i = 0; i < 32; i += 8) {
+    uint32_t w[8][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) cause |= !(fabsf(x[e]) < INFINITY);
+    for (int y = 0; y < 8; ++y) load(at + (i + y) * 512, w[y]);
+#pragma unroll
+    for (int y = 0; y < 8; ++y)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = stain2<T>(w[y][e], acc[e]);
   }
-  if (!__any_sync(0xffffffffu, cause)) return;
-  float q[4], acc[4] = {}, m = -INFINITY, l = 0.0f;
-  load4(static_cast<const T *>(a.q) + s.b * a.qs[0] + head * a.qs[1] + (static_cast<int64_t>(s.q0) + row) * a.qs[2] + 4 * lane, q);
-  for (int j = lo; j < min(limit, hi); ++j) {
-    load4(k + j * a.ks[2], x);
-    float d = q[0] * x[0] + q[1] * x[1] + q[2] * x[2] + q[3] * x[3];
+  if (!__any_sync(0xffffffffu, (odd(acc[0]) | odd(acc[1]) | odd(acc[2]) | odd(acc[3])) != 0)) return;
+#pragma unroll 1
+  for (int i = 0; i < 32; ++i) {
+    uint32_t w[4];
+    load(at + i * 512, w);
+    if (odd(w[0]) | odd(w[1]) | odd(w[2]) | odd(w[3])) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    d *= a.c;
-    const float mn = fmaxf(m, d), ref = mn == -INFINITY ? 0.0f : mn;
-    const float f = ex2(m - ref), p = ex2(d - ref);
-    load4(v + j * a.vs[2], x);
-    l = l * f + p;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = acc[e] * f + p * x[e];
-    m = mn;
+      for (int e = 0; e < 4; ++e) w[e] &= ~((odd(w[e]) >> 15) * 0xffffu);
+      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * 512), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+      const int row = 4 * i + (lane >> 3);
+      atomicOr(rows + (row >> 5), 1u << (row & 31));
+    }
   }
-  const int64_t at = (s.out0 + row) * static_cast<int64_t>(a.G) * a.h_kv + head;
-  if (a.splits > 1) {
-    const int64_t pa = z * a.rows * a.G * a.h_kv + at;
-    *reinterpret_cast<float4 *>(a.part + pa * HD + 4 * lane) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-    if (lane == 0) a.part_ml[pa] = make_float2(m, l);
-    return;
-  }
-  T o[4];
+}
+
+// Adds what clear_odd_values() took out, as far as the thread's row sees it, to the row's accumulator.  The keys are the
+// same for all rows of a warp, which read them together.
+template <typename T>
+__device__ __noinline__ void add_odd_values(const Odd &odd, int64_t stride, uint32_t acc, int limit) {
+#pragma unroll 1
+  for (int i = 0; i < 4; ++i) {
+    float o[32];
+    tmem_ld32(acc + 32 * i, o);
+    tmem_wait_ld();
+#pragma unroll 1
+    for (int y = 0; y < 4 * CLEAN_TILES; ++y) {
+      uint32_t m = odd.rows[0][y] | odd.rows[1][y];
+      while (m) {
+        const int key = odd.tile0 * PT + 32 * y + __ffs(m) - 1;
+        m &= m - 1;
+        if (key >= odd.nk) break;
+        const T *row = static_cast<const T *>(odd.v) + key * stride + 32 * i;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) o[e] = from_f32<T>(acc[e] / l);
-  *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + at * HD + 4 * lane) = *reinterpret_cast<const uint2 *>(o);
+        for (int c = 0; c < 4; ++c) {
+          float x[8];
+          Vec8<T>::load(row + 8 * c, x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (key < limit && !(fabsf(x[e]) < INFINITY)) o[8 * c + e] += x[e];
+        }
+      }
+    }
+    tmem_st32(acc + 32 * i, reinterpret_cast<const uint32_t *>(o));
+  }
+  tmem_wait_st();
 }
 
 // One piece of work of a block: a pair of query tiles of one key head against its key tiles (or the z-th part of them).
@@ -225,6 +266,7 @@ struct Item {
   int h, pair, z;
   int j0, n;          // first key tile and their number
   int nb[2];          // how many of them each tile sees
+  int clean;          // the first of them that some row does not see all of (n: none)
   int more;           // 0: there is no further item
 };
 
@@ -327,6 +369,13 @@ __device__ __forceinline__ bool find_item(const PromptArgs &a, int id, Item &w) 
   w.n = static_cast<int>(static_cast<int64_t>(most) * (w.z + 1) / a.splits) - w.j0;
   w.nb[0] = min(max(all0 - w.j0, 0), w.n);
   w.nb[1] = min(max(all1 - w.j0, 0), w.n);
+  // rows of the two tiles see 255 keys more than their first row at most, which are in CLEAN_TILES tiles
+  w.clean = w.n;
+  for (int x = 0; x < 2; ++x)
+    if (w.nb[x] > 0) {
+      tile_of(a, s, w.h, w.pair, x, row0, head);
+      w.clean = min(w.clean, max(key_limit(s, row0, a.causal) / PT - w.j0, 0));
+    }
   w.more = 1;
   return true;
 }
@@ -338,9 +387,10 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
   constexpr bool BF16 = __is_same(T, __nv_bfloat16);
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar_q, bar_q_free, bar_full[KV_STAGES], bar_empty[KV_STAGES], bar_s[2], bar_p[2][2], bar_o[2],
-      bar_item[2], bar_item_free[2], bar_end;
+      bar_item[2], bar_item_free[2], bar_turn[2], bar_clean[2], bar_odd[2], bar_odd_free[2], bar_end;
   __shared__ uint32_t tmem_base;
   __shared__ Item items[2];
+  __shared__ Odd odd[2];
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
   if (warp == 9) tmem_alloc(smem_u32(&tmem_base), 512);
@@ -354,7 +404,11 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       mbar_init(smem_u32(&bar_p[x][1]), 4);
       mbar_init(smem_u32(&bar_o[x]), 1);
       mbar_init(smem_u32(&bar_item[x]), 1);
-      mbar_init(smem_u32(&bar_item_free[x]), 9);            // the issuing warp and eight softmax warps
+      mbar_init(smem_u32(&bar_item_free[x]), 11);           // all warps but the copying one
+      mbar_init(smem_u32(&bar_turn[x]), 1);
+      mbar_init(smem_u32(&bar_clean[x]), 2);
+      mbar_init(smem_u32(&bar_odd[x]), 2);
+      mbar_init(smem_u32(&bar_odd_free[x]), 8);
     }
     mbar_init(smem_u32(&bar_end), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -449,13 +503,13 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       const uint32_t full = smem_u32(&bar_full[0]), empty = smem_u32(&bar_empty[0]);
       const uint32_t ready = smem_u32(&bar_s[0]), weights = smem_u32(&bar_p[0][0]), done = smem_u32(&bar_o[0]);
       const uint32_t q_lo = umma_lo(q_addr, 16), k_lo = umma_lo(kv_addr, 16), v_lo = umma_lo(kv_addr, TILE_BYTES / 2);
-      uint32_t pos = 0, step0 = 0, step1 = 0;               // tiles read; weights of either query tile taken, so far
+      uint32_t pos = 0, step0 = 0, step1 = 0, cleaned = 0;  // tiles read, weights of either query tile taken, tiles cleaned so far
       int loaded = 0;
       bool ok = true;
       Item w;
       for (int c = 0; ok && next_item(c, w); ++c) {
         if (w.n == 0) continue;
-        const int n = w.n, nb0 = w.nb[0], nb1 = w.nb[1];
+        const int n = w.n, nb0 = w.nb[0], nb1 = w.nb[1], clean = w.clean;
         if (elect_one()) {
           uint32_t st = pos % KV_STAGES, ph = pos / KV_STAGES & 1;      // ring position of the next tile
           auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -479,7 +533,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             }
             umma_commit(ready + 8 * x);
           };
+          // Value tile j is to be cleaned: said a step early, so that it is done when the step's weights are there.  The next
+          // tile may be asked for, and done, before this thread sees that this one is, but not the one after it: two barriers
+          // either way.
+          auto ask = [&](int j) { mbar_arrive(smem_u32(&bar_turn[(cleaned + (j - clean)) & 1])); };
           wait(smem_u32(&bar_q), loaded & 1);
+          if (clean == 0) ask(0);
           if (wait(full + 8 * st, ph)) {
 #pragma unroll 1
             for (int x = 0; x < 2; ++x)
@@ -492,6 +551,11 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
           for (int j = 0; j < n && ok; ++j) {
             const uint32_t sv = st;
             if (!wait(full + 8 * sv, ph)) break;
+            if (j + 1 >= clean && j + 1 < n) ask(j + 1);
+            if (j >= clean) {
+              const uint32_t at = cleaned + (j - clean);
+              if (!wait(smem_u32(&bar_clean[at & 1]), (at >> 1) & 1)) break;
+            }
             advance();
             const bool more = j + 1 < n;
 #pragma unroll 1
@@ -533,6 +597,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         pos += 2 * n;
         step0 += nb0;
         step1 += nb1;
+        cleaned += n - clean;
         ++loaded;
       }
       // every product is complete before the tensor memory is given back
@@ -541,6 +606,38 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         mbar_wait_asleep(smem_u32(&bar_end), 0);
       }
       __syncwarp();
+    } else {
+      // ---- values that are not finite, in the tiles that the issuing warp asks for
+      uint32_t pos = 0, cleaned = 0;
+      bool ok = true;
+      Item w;
+      for (int c = 0; ok && next_item(c, w); ++c) {
+        // the softmax warps are done with the words of the item before last
+        if (c >= 2) ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_odd_free[c & 1]), ((c >> 1) - 1) & 1));
+        if (!ok) break;
+        Odd &o = odd[c & 1];
+        uint32_t *rows = o.rows[warp - 10];
+        if (lane < 4 * CLEAN_TILES) rows[lane] = 0;
+        if (warp == 10 && lane == 0) {
+          o.v = static_cast<const T *>(a.v) + w.s.b * a.vs[0] + w.h * a.vs[1] + w.s.k0 * a.vs[2];
+          o.tile0 = w.j0 + w.clean;
+          o.nk = w.s.nk;
+        }
+        __syncwarp();
+        for (int j = w.clean; j < w.n; ++j, ++cleaned) {
+          const uint32_t at = pos + 2 * j + 1, st = at % KV_STAGES;
+          ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_turn[cleaned & 1]), (cleaned >> 1) & 1) &&
+                                           mbar_wait_asleep(smem_u32(&bar_full[st]), at / KV_STAGES & 1));
+          if (!ok) break;
+          clear_odd_values<T>(kv_addr + st * TILE_BYTES + (warp - 10) * (TILE_BYTES / 2), rows + 4 * (j - w.clean));
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // the product reads what was written here
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&bar_clean[cleaned & 1]));
+        }
+        if (ok && lane == 0) mbar_arrive(smem_u32(&bar_odd[c & 1]));
+        pos += 2 * w.n;
+      }
+      if (!ok) give_up();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
@@ -650,12 +747,19 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       if (nb > 0 && ok) ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_o[x]), outs & 1));
       step += nb;
       outs += nb > 0;
+      tc_fence_after();
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_odd[count & 1]), (count >> 1) & 1));
+      if (ok) {
+        const Odd &o = odd[count & 1];
+        const bool some = lane < 4 * CLEAN_TILES && (o.rows[0][lane] | o.rows[1][lane]) != 0;
+        if (__any_sync(0xffffffffu, some) && nb > 0) add_odd_values<T>(o, a.vs[2], to, limit);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&bar_odd_free[count & 1]));
+      }
       if (live && ok) {
-        tc_fence_after();
         const bool mine = row < s.rows;
         const int64_t at_out = (s.out0 + row) * static_cast<int64_t>(a.G) * a.h_kv + head;
         const int64_t stride = static_cast<int64_t>(a.G) * a.h_kv * HD;      // from a row of the output to the next
-        float bad = 0.0f;                      // NaN as soon as a value is not finite
         if (a.splits == 1) {
           const float inv = limit > 0 ? 1.0f / l : 0.0f;
           T *dst = static_cast<T *>(a.out) + at_out * HD;
@@ -670,9 +774,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             T *t = reinterpret_cast<T *>(w);
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
-              const float y = limit > 0 ? o[e] * inv : 0.0f;
-              bad = fmaf(y, 0.0f, bad);
-              t[e] = from_f32<T>(y);
+              t[e] = from_f32<T>(limit > 0 ? o[e] * inv : 0.0f);
             }
             store_quad(w, dst + 32 * i, stride, row, s.rows);
           }
@@ -690,22 +792,12 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
             tmem_ld32(to + 32 * i, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) bad = fmaf(o[e], 0.0f, bad);
-#pragma unroll
             for (int y = 0; y < 2; ++y) {
               uint4 w[4];
               memcpy(w, o + 16 * y, 64);
               store_quad(w, dst + 32 * i + 16 * y, stride, row, s.rows);
             }
           }
-        }
-        __syncwarp();
-        unsigned again = __ballot_sync(0xffffffffu, !(bad == 0.0f) && mine && limit > j0 * PT);
-        while (again) {
-          const int r = __ffs(again) - 1;
-          again &= again - 1;
-          const int hi = min((j0 + nb) * PT, a.Lk - s.k0);
-          repair_row<T>(a, s, __shfl_sync(0xffffffffu, row, r), head, __shfl_sync(0xffffffffu, limit, r), j0 * PT, hi, z);
         }
       }
     }

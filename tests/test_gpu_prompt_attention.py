@@ -295,3 +295,82 @@ def test_patched_model_takes_the_prompt_kernel(kb, dtype, monkeypatch):
     hf_adapter.patch_model(single, prompt_kernel=True)
     hf_adapter.greedy_decode(single, ids, 2, kb.get_kvcache_kitty(cfg, 2, 512, device=DEV))
     assert len(calls) == 2
+
+
+def _best_us(call, n=5):
+    """Shortest of n timed calls (after one that is not)."""
+    call()
+    best = float("inf")
+    for _ in range(n):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        call()
+        b.record()
+        b.synchronize()
+        best = min(best, 1000.0 * a.elapsed_time(b))
+    return best
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [True, False])
+def test_padding_that_is_not_finite_costs_no_more(kb, dtype, causal):
+    """Keys and values behind a row's last one, or of the next sequence: the same bits in about the same time, whatever they
+    hold.  (The limit is wide: a row computed without the tensor cores takes thousands of times as long.)"""
+    q, k, v = _inputs((2, 8, 2500, 128), (2, 2, 2500, 128), dtype, 21)
+    lens = torch.tensor([2450, 1111], dtype=torch.int32, device=DEV)
+    k2, v2 = k.clone(), v.clone()
+    for b in range(2):
+        n = int(lens[b])
+        k[b, :, n:], v[b, :, n:] = 0.0, 0.0
+        k2[b, :, n:], v2[b, :, n:] = float("inf"), float("nan")
+    run = lambda kk, vv: kb.prompt_attention(q, kk, vv, SC, causal=causal, key_lengths=lens)  # noqa: E731
+    assert torch.equal(run(k2, v2), run(k, v))
+    assert _best_us(lambda: run(k2, v2)) <= 3.0 * _best_us(lambda: run(k, v)) + 200.0
+    # packed: the second sequence is not finite, the first does not notice
+    qp, kp, vp = (x[0].transpose(0, 1).contiguous() for x in (q, k, v))
+    cu = torch.tensor([0, 1300, 2500], dtype=torch.int32, device=DEV)
+    packed = lambda vv: kb.prompt_attention(qp, kp, vv, SC, causal=causal, cu_seqlens=cu)  # noqa: E731
+    bad = vp.clone()
+    bad[1300:] = float("-inf")
+    want, got = packed(vp), packed(bad)
+    assert torch.equal(got[:1300], want[:1300]) and not torch.isfinite(got[1300:]).any()
+    assert _best_us(lambda: packed(bad)) <= 3.0 * _best_us(lambda: packed(vp)) + 2000.0
+    assert kb.prompt_attention_status(DEV) == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,h,Lq,Lk", [(1, 1, 700, 700), (6, 2, 300, 333), (3, 1, 40, 3000), (2, 2, 260, 200)])
+def test_values_that_are_not_finite_reach_the_rows_that_see_them(kb, dtype, hq, h, Lq, Lk):
+    """Infinities and NaN at the edges of tiles and within them: a row that sees some gets their sum in their channels, and
+    otherwise every row has the bits that it has with zeros in their place."""
+    inf, nan = float("inf"), float("nan")
+    q, k, v = _inputs((1, hq, Lq, 128), (1, h, Lk, 128), dtype, 22)
+    odd = torch.zeros(h, Lk, 128, device=DEV, dtype=torch.float64)
+    for x in range(h):
+        for i, key in enumerate([0, 63, 127, 128, 129, 255, 256, 300, Lk - 130, Lk - 3, Lk - 2, Lk - 1]):
+            if 0 <= key < Lk:
+                odd[x, key, (7 * i + x) % 128] = (nan, inf, -inf)[i % 3]
+        odd[x, Lk // 2, 3], odd[x, Lk - 5, 3] = inf, -inf                  # opposite ones: NaN from the second on
+        odd[x, Lk - 9] = nan                                             # a whole row
+    hit = odd != 0
+    v = torch.where(hit[None], torch.zeros_like(v), v)
+    want = kb.prompt_attention(q, k, v, SC)
+    got = kb.prompt_attention(q, k, torch.where(hit[None], odd[None].to(dtype), v), SC)
+    lim = _limits(Lq, Lk, True)
+    reach = torch.cat((torch.zeros(h, 1, 128, device=DEV, dtype=torch.float64), odd.cumsum(1)), 1)[:, lim]    # [h, Lq, 128]
+    for x in range(hq):
+        add = reach[x // (hq // h)]
+        w, g = want[0, :, x], got[0, :, x]
+        assert torch.equal(g[add == 0], w[add == 0])
+        assert torch.isnan(g[torch.isnan(add)]).all()
+        assert (g[torch.isinf(add)].double() == add[torch.isinf(add)]).all()
+    assert torch.isfinite(want).all() and kb.prompt_attention_status(DEV) == 0
+
+
+def test_nothing_but_nan(kb):
+    """Values that are all NaN: every row that sees one is NaN, in a bounded time."""
+    q, k, v = _inputs((1, 8, 3000, 128), (1, 2, 3000, 128), torch.bfloat16, 23)
+    clean = _best_us(lambda: kb.prompt_attention(q, k, v, SC), 2)
+    v[:] = float("nan")
+    assert torch.isnan(kb.prompt_attention(q, k, v, SC)).all()
+    assert _best_us(lambda: kb.prompt_attention(q, k, v, SC), 2) <= 20.0 * clean + 5000.0
