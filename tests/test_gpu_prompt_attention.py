@@ -374,3 +374,25 @@ def test_nothing_but_nan(kb):
     v[:] = float("nan")
     assert torch.isnan(kb.prompt_attention(q, k, v, SC)).all()
     assert _best_us(lambda: kb.prompt_attention(q, k, v, SC), 2) <= 20.0 * clean + 5000.0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_blocks_that_take_several_items_of_several_tiles(kb, dtype):
+    """More items than multiprocessors, each of several key tiles, of unequal numbers: what a block carries from item to item."""
+    q, k, v = _inputs((3, 24, 1400, 128), (3, 12, 1400, 128), dtype, 24)
+    ql = torch.tensor([1400, 900, 1400], dtype=torch.int32, device=DEV)
+    kl = torch.tensor([1400, 900, 130], dtype=torch.int32, device=DEV)
+    got = kb.prompt_attention(q, k, v, SC, query_lengths=ql, key_lengths=kl)
+    for b in range(3):
+        n, m = int(ql[b]), int(kl[b])
+        assert (got[b, n:] == 0).all()
+        _check_rows(got[b, :n], q[b, :, :n].transpose(0, 1), k[b, :, :m].transpose(0, 1), v[b, :, :m].transpose(0, 1), SC, True)
+    again = kb.prompt_attention(q, k, v, SC, query_lengths=ql, key_lengths=kl)
+    assert torch.equal(got, again)                                     # and the same bits each time
+    lens = [1400, 3, 700, 129, 1, 1399]
+    cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=DEV)
+    qp, kp, vp = _inputs((sum(lens), 24, 128), (sum(lens), 12, 128), dtype, 25)
+    got = kb.prompt_attention(qp, kp, vp, SC, cu_seqlens=cu, causal=False)
+    for a, b in zip(cu[:-1].tolist(), cu[1:].tolist()):
+        _check_rows(got[a:b], qp[a:b], kp[a:b], vp[a:b], SC, False, (a, b))
+    assert kb.prompt_attention_status(DEV) == 0
