@@ -418,9 +418,9 @@ typedef struct {
   int32_t *status;            /* device int32: bits below are set, never cleared        */
 } kitty_kv8_layer;
 
-#define KITTY_KV8_BAD_PAGE 1   /* a page-table entry out of range: its block was skipped             */
-#define KITTY_KV8_BAD_LENGTH 2 /* a length or start outside 0 .. 128*max_page: it was clamped        */
-#define KITTY_KV8_TIMEOUT 4    /* a bounded device-side wait ran out                                 */
+#define KITTY_KV8_BAD_PAGE 1   /* a page-table entry out of range: its block was skipped: as if not held */
+#define KITTY_KV8_BAD_LENGTH 2 /* a length or start outside 0 .. 128*max_page: it was clamped            */
+#define KITTY_KV8_TIMEOUT 4    /* a bounded device-side wait ran out                                     */
 
 /* Tokens key / value [B, h_kv, T, 128] (element strides (batch, head, token) in the HOST array strides: key, value,
  * query) become tokens start[b], start[b] + 1, ... of row b; counts[b] of them (null: all T).  With a rotary plan the

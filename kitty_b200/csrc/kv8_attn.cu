@@ -345,14 +345,16 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) kv8_attn_kernel(const 
         for (int e = 0; e < 2 * MT; ++e)
           p[i][e] = 8 * t + 2 * i + (e & 1) < cnt ? c[i][e] * a.scale_log2 : -INFINITY;
     }
-    if (skipped[warp][stage]) {
+    const bool skip = skipped[warp][stage] != 0;
+    if (skip) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int e = 0; e < 2 * MT; ++e) p[i][e] = -INFINITY;
       vscale = 0.0f;
     }
-    // the block's own maximum and weights, and the running maximum and sum (base 2)
+    // The block's own maximum and weights, and the running maximum and sum (base 2).  A maximum stays -infinity as long as
+    // nothing but skipped blocks was met; of tokens whose logits are all -infinity it is the lowest number.
     float corr[MT], part[MT];
     bool moved = false;
 #pragma unroll
@@ -361,6 +363,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) kv8_attn_kernel(const 
                         fmaxf(fmaxf(p[2][2 * m], p[2][2 * m + 1]), fmaxf(p[3][2 * m], p[3][2 * m + 1])));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      if (!skip) top = fmaxf(top, -3.402823466e38f);
       const float own = top == -INFINITY ? 0.0f : top;
       const float mn = fmaxf(mx[m], top), ref = mn == -INFINITY ? 0.0f : mn;
       corr[m] = ex2(mx[m] - ref);
@@ -465,7 +468,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) kv8_attn_kernel(const 
         const int head = g + 8 * m;
         if (head < G && all) {
           T *o = static_cast<T *>(a.out) + (row * G + head) * HD + 2 * t;
-          const float inv = 1.0f / s;
+          const float inv = mx[m] == -INFINITY ? 0.0f : 1.0f / s;       // every block skipped: zeros
 #pragma unroll
           for (int n = 0; n < 16; ++n)
             *reinterpret_cast<uint32_t *>(o + 8 * n) = pack_t<T>(acc[n][2 * m] * inv, acc[n][2 * m + 1] * inv);
@@ -504,7 +507,8 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) kv8_attn_kernel(const 
       float top = -INFINITY, l = 0.0f, x = 0.0f, y = 0.0f;
 #pragma unroll
       for (int w = 0; w < W; ++w) top = fmaxf(top, parts[w][head].x);
-      if (top == -INFINITY) top = 0.0f;
+      const bool none = top == -INFINITY;                                // no token, or every block skipped
+      if (none) top = 0.0f;
 #pragma unroll
       for (int w = 0; w < W; ++w) {
         if (cur.nblk * w / W == cur.nblk * (w + 1) / W) continue;      // a warp without blocks
@@ -515,7 +519,7 @@ __global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1) kv8_attn_kernel(const 
         x = fmaf(v.x, wgt, x);
         y = fmaf(v.y, wgt, y);
       }
-      const float inv = cur.nblk > 0 ? 1.0f / l : 0.0f;
+      const float inv = none ? 0.0f : 1.0f / l;
       *reinterpret_cast<uint32_t *>(out + 2 * i) = pack_t<T>(x * inv, y * inv);
     }
   }
@@ -580,7 +584,7 @@ __global__ void __launch_bounds__(256) kv8_join_rows_kernel(const __grid_constan
       }
       m = mn;
     }
-  const float inv = nblk > 0 ? 1.0f / l : 0.0f;
+  const float inv = m == -INFINITY ? 0.0f : 1.0f / l;      // no token, or every block skipped: zeros
   uint2 o;
   o.x = pack_t<T>(acc[0] * inv, acc[1] * inv);
   o.y = pack_t<T>(acc[2] * inv, acc[3] * inv);
@@ -653,7 +657,7 @@ __global__ void __launch_bounds__(HD * KV8_JOIN_GROUPS) kv8_join_kernel(const __
   float tot = 0.0f;
 #pragma unroll
   for (int i = 0; i < KV8_JOIN_GROUPS; ++i) tot += red[i][c];
-  static_cast<T *>(a.out)[static_cast<int64_t>(blockIdx.x) * HD + c] = from_f32<T>(nblk > 0 ? tot / l : 0.0f);
+  static_cast<T *>(a.out)[static_cast<int64_t>(blockIdx.x) * HD + c] = from_f32<T>(m == -INFINITY ? 0.0f : tot / l);
 }
 
 template <typename T, int MT, int W, bool ROW>

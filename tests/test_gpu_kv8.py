@@ -423,3 +423,47 @@ def test_scalings_of_any_sign_and_size(kb, scaling, room):
     q = torch.randn(3, 6, 1, 128, generator=torch.Generator(device=DEV).manual_seed(2), device=DEV).bfloat16()
     _attention_check(kb.kv8_attention(q, layer, n, scaling), q, layer, lengths, (k, v), scaling)
     layer.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,H,cap,lengths", [
+    (3, 1, 640, [128, 512, 600]),                       # a block of threads per row
+    (150, 1, 640, [128, 512, 600] + [96] * 147),        # four warps a row
+    (3, 2, 4096, [128, 2048, 3900]),                    # split over workers, joined by blocks
+    (130, 2, 9000, [128, 2048, 8900] + [96] * 127)])    # joined by warps; short rows that one worker has whole
+@pytest.mark.parametrize("hq_per", [1, 12])
+def test_rows_whose_pages_are_all_bad(kb, dtype, B, H, cap, lengths, hq_per):
+    """Blocks of bad pages count as not held: a row that keeps nothing is zero, one that keeps its open block is that."""
+    pages = -(-cap // 128)
+    layer = kb.KV8Layer(B, cap, H, dtype=dtype, device=DEV, num_pages=200, page_table=torch.full((B, pages), -7, device=DEV))
+    k, v = _kv(B, H, max(lengths) + 5, dtype, 31)
+    g = torch.Generator(device=DEV).manual_seed(32)
+    q = torch.randn(B, H * hq_per, 1, 128, generator=g, device=DEV).to(dtype)
+    n = _i32(lengths)
+    kb.kv8_append(layer, k, v, torch.zeros_like(n), lengths=n)             # open blocks only: the pages are bad
+    got = kb.kv8_attention(q, layer, n, SC)
+    for b, m in enumerate(lengths):
+        full = m // 32 * 32
+        if m == full:
+            assert (got[b] == 0).all(), b
+            continue
+        for x in range(H * hq_per):
+            want, mag = attend_fast(q[b, x].double(), k[b, x // hq_per, full:m].double(), v[b, x // hq_per, full:m].double(), SC,
+                                    torch.tensor([m - full], device=DEV))
+            bound = attention_bound(want, mag, dtype, 2.0 ** -16, logit_error(q[b, x].double(), k[b, x // hq_per, full:m].double(), SC))
+            assert ((got[b, :, x].double() - want).abs() <= bound).all(), (b, x)
+    with pytest.raises(ValueError, match="page-table"):
+        layer.check()
+
+
+@pytest.mark.parametrize("room", [0, 4100])
+def test_logits_that_are_all_minus_infinity(kb, room):
+    """Not the same as a row without tokens: zero over zero."""
+    layer = kb.KV8Layer(1, 100 + room, 1, dtype=torch.float16, device=DEV)
+    k, v = torch.zeros(1, 1, 7, 128, device=DEV).half(), torch.ones(1, 1, 7, 128, device=DEV).half()
+    k[..., 5] = float("-inf")
+    kb.kv8_append(layer, k, v, _i32([0]))
+    q = torch.zeros(1, 2, 1, 128, device=DEV).half()
+    q[..., 5] = 1.0
+    assert torch.isnan(kb.kv8_attention(q, layer, _i32([7]), SC)).all()
+    layer.check()
