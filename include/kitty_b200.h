@@ -34,7 +34,8 @@ typedef enum {
   KITTY_E_WORKSPACE = -3, /* caller's workspace too small                               */
   KITTY_E_CUDA = -4,      /* a CUDA runtime call failed (see cudaGetLastError)          */
   KITTY_E_TIMEOUT = -5,   /* a bounded device-side wait ran out                         */
-  KITTY_E_STATIC_LIMIT = -6 /* problem needs more scratch than kitty_decode_attn_static has */
+  KITTY_E_STATIC_LIMIT = -6, /* problem needs more scratch than kitty_decode_attn_static has */
+  KITTY_E_OVERLAP = -7       /* an output shares memory with another tensor of the call     */
 } kitty_status;
 
 typedef enum { KITTY_F16 = 0, KITTY_BF16 = 1, KITTY_F32 = 2 } kitty_dtype;
@@ -340,6 +341,11 @@ int kitty_lse_exchange_merge(const float *local_partial, int64_t rows, void *con
                              int32_t world, int32_t seq, void *out, int out_dtype, int32_t *status, int64_t wait_ns,
                              void *stream);
 
+/* Whether two sets of rows share memory, as the entry points below ask about their outputs: rows of `run` bytes at
+ * x + sum(i * x_steps), 0 <= i < x_sizes, three dimensions each, steps in bytes (HOST arrays).  1 or 0. */
+int kitty_rows_overlap(const void *x, const int64_t *x_sizes, const int64_t *x_steps, const void *y,
+                       const int64_t *y_sizes, const int64_t *y_steps, int64_t run);
+
 /* ---- Rotary positions of prompts and tokens ------------------------------------------------
  * (No counterpart in the reference, whose models call the element-wise sequence of
  * models/qwen3/modeling_qwen3.py:222-232.)  Pair p of a head is turned by angle position * w_p and multiplied by
@@ -362,7 +368,8 @@ typedef struct {
 /* q [B, h_q, T, 128] and k [B, h_kv, T, 128] of `dtype` (any of the three) turned into q_out / k_out.  positions:
  * device int64, row b at positions + b*pos_stride_b (0: one row for all), T values each.  strides: HOST array of
  * twelve element strides, (batch, head, token) of q, k, q_out and k_out; channels are consecutive and every row starts
- * on a 16-byte boundary.  An output may be its own input (in place); any other overlap is the caller's error.
+ * on a 16-byte boundary.  An output may be its own input (in place); any other memory that it shares with an input or
+ * with the other output is refused (KITTY_E_OVERLAP).
  * h_q or h_kv may be 0. */
 int kitty_rotary(const kitty_rotary_plan *plan, const void *q, const void *k, const int64_t *positions,
                  int64_t pos_stride_b, void *q_out, void *k_out, int dtype, int32_t B, int32_t T, int32_t h_q,
@@ -381,7 +388,8 @@ int kitty_rotary(const kitty_rotary_plan *plan, const void *q, const void *k, co
  * causal: the last query of a sequence sees its last key, query i sees keys 0 .. i + (keys - queries).  A row that
  * sees no key is zero.  Keys and values that a row does not see never reach its result, whatever they hold.
  * strides: HOST array of nine element strides, (batch, head, token) of q, k and v (batch ignored when packed).
- * out: contiguous [B, Lq, h_q, 128] or [Lq, h_q, 128] of the same type.  scaling: positive and finite.
+ * out: contiguous [B, Lq, h_q, 128] or [Lq, h_q, 128] of the same type, no part of q, k or v (KITTY_E_OVERLAP).
+ * scaling: positive and finite.
  * status: device int32 or null, set to 1 when a bounded device-side wait ran out.
  * workspace: null, or kitty_prompt_workspace_bytes of scratch (0 for most calls; 16-byte aligned, no initial contents,
  * not shared by calls that overlap).  With it, calls with few query rows cut the keys in parts that run side by side
@@ -426,20 +434,21 @@ typedef struct {
  * query) become tokens start[b], start[b] + 1, ... of row b; counts[b] of them (null: all T).  With a rotary plan the
  * keys are turned on the way by their position in the row, and rounded to the data type before they are stored; the
  * query rows [B, h_q, T, 128] (or null, h_q = 0) are turned by the same positions into q_out [B, h_q, T, 128]
- * (contiguous), all T of them.  Tokens that end up in an open block go to the tails, others into their pages: a
+ * (contiguous; no part of key, value or query: KITTY_E_OVERLAP), all T of them.  Tokens that end up in an open block go to the tails, others into their pages: a
  * token-by-token caller and one that gives the whole prompt leave the same bytes. */
 int kitty_kv8_append(const kitty_kv8_layer *layer, const void *key, const void *value, const int64_t *strides,
                      const int32_t *start, const int32_t *counts, int32_t B, int32_t T,
                      const kitty_rotary_plan *rotary, const void *query, void *q_out, int32_t h_q, void *stream);
 
 /* Tokens start[b] .. start[b] + n - 1 of every row (start null: from 0) as values of the layer's type, k_out / v_out
- * [B, h_kv, n, 128] contiguous.  lengths: device int32 [B], what the rows hold; tokens behind it are zeros. */
+ * [B, h_kv, n, 128] contiguous and apart (KITTY_E_OVERLAP).  lengths: device int32 [B], what the rows hold; tokens behind it are zeros. */
 int kitty_kv8_expand(const kitty_kv8_layer *layer, const int32_t *lengths, const int32_t *start, void *k_out,
                      void *v_out, int32_t B, int32_t n, void *stream);
 
 /* One query token per row over the tokens the row holds (lengths: device int32 [B]; 0 gives zeros).  query
  * [B, h_q, 1, 128] and out [B, 1, h_q, 128], contiguous, of the layer's type; up to 16 query heads per key head,
- * B <= KITTY_KV8_MAX_BATCH.  workspace: kitty_kv8_workspace_bytes (0 for caches of short rows: null will do),
+ * B <= KITTY_KV8_MAX_BATCH.  out may be the query's own memory, row for row; any other overlap is refused
+ * (KITTY_E_OVERLAP).  workspace: kitty_kv8_workspace_bytes (0 for caches of short rows: null will do),
  * 16-byte aligned, no initial contents; calls that share one must not overlap. */
 #define KITTY_KV8_MAX_BATCH 2048
 int64_t kitty_kv8_workspace_bytes(int32_t B, int32_t h_kv, int32_t h_q, int32_t max_page);

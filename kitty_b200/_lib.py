@@ -15,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libkitty_b200.so")
 
 KITTY_OK, KITTY_E_BADARG, KITTY_E_BADSHAPE, KITTY_E_WORKSPACE, KITTY_E_CUDA, KITTY_E_TIMEOUT = 0, -1, -2, -3, -4, -5
-KITTY_E_STATIC_LIMIT = -6
+KITTY_E_STATIC_LIMIT, KITTY_E_OVERLAP = -6, -7
 STATIC_SCRATCH_BYTES = 8 << 20
 KITTY_F16, KITTY_BF16, KITTY_F32 = 0, 1, 2
 SELECT_FUSED, SELECT_SUPPLIED = 0, 1
@@ -32,7 +32,7 @@ EXPORTS = [
     "kitty_lse_exchange_bytes", "kitty_lse_exchange_merge", "kitty_decode_attn_exchange", "kitty_rope_qk",
     "kitty_plan_step_split", "kitty_decode_step_exchange", "kitty_append_rows", "kitty_flush_rows",
     "kitty_decode_attn_rows", "kitty_rotary", "kitty_prompt_workspace_bytes", "kitty_prompt_attn", "kitty_kv8_append", "kitty_kv8_expand",
-    "kitty_kv8_workspace_bytes", "kitty_kv8_attn",
+    "kitty_kv8_workspace_bytes", "kitty_kv8_attn", "kitty_rows_overlap",
 ]
 
 
@@ -72,7 +72,7 @@ class KittyKV8Layer(C.Structure):
                [(n, C.c_void_p) for n in ("pages", "tail_k", "tail_v", "page_table", "status")]
 
 
-_I64 = {n: struct.Struct(f"{n}q").pack for n in (9, 12)}
+_I64 = {n: struct.Struct(f"{n}q").pack for n in (3, 9, 12)}
 
 
 def i64_array(values) -> bytes:
@@ -165,6 +165,8 @@ def lib() -> C.CDLL:
     L.kitty_lse_merge.restype = C.c_int
     L.kitty_lse_merge.argtypes = [vp, i32, i64, vp, C.c_int, vp]
     rot, kv8, strides = C.POINTER(KittyRotaryPlan), C.POINTER(KittyKV8Layer), C.c_char_p
+    L.kitty_rows_overlap.restype = C.c_int
+    L.kitty_rows_overlap.argtypes = [vp, strides, strides, vp, strides, strides, i64]
     L.kitty_rotary.restype = C.c_int
     L.kitty_rotary.argtypes = [rot, vp, vp, vp, i64, vp, vp, C.c_int, i32, i32, i32, i32, strides, vp]
     L.kitty_prompt_attn.restype = C.c_int
@@ -261,6 +263,8 @@ def call_on(device, fn, where: str, *args) -> None:
     else:
         with torch.cuda.device(index):
             rc = fn(*args, stream)
+    if rc == KITTY_E_OVERLAP:
+        raise ValueError(f"{where}: {strerror(rc)}")
     if rc != KITTY_OK:
         raise KittyError(int(rc), where)
 

@@ -506,6 +506,7 @@ extern "C" const char *kitty_strerror(int status) {
     case KITTY_E_STATIC_LIMIT:
       return "the problem needs more scratch than the built-in array of kitty_decode_attn_static "
              "(KITTY_STATIC_SCRATCH_BYTES); use kitty_decode_attn with a caller-owned workspace";
+    case KITTY_E_OVERLAP: return "an output overlaps another tensor of the call";
     default: return "unknown status";
   }
 }

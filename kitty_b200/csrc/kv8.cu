@@ -12,6 +12,7 @@
 // is the second byte of the number.
 #include "decode.cuh"
 #include "kv8.cuh"
+#include "overlap.cuh"
 #include "rotary.cuh"
 
 namespace kitty {
@@ -538,6 +539,15 @@ extern "C" int kitty_kv8_append(const kitty_kv8_layer *layer, const void *key, c
     a.qs[i] = strides[6 + i];
     if (a.ks[i] % 8 != 0 || a.vs[i] % 8 != 0 || (h_q > 0 && a.qs[i] % 8 != 0)) return KITTY_E_BADARG;
   }
+  if (h_q > 0) {
+    constexpr int64_t ROW = HD * 2;
+    const Rows turned{q_out, {B, h_q, T}, {h_q * T * ROW, T * ROW, ROW}, ROW};
+    const void *in[3] = {key, value, query};
+    for (int x = 0; x < 3; ++x) {
+      const int64_t *st = strides + 3 * x;
+      if (rows_meet(turned, {in[x], {B, x < 2 ? layer->h_kv : h_q, T}, {st[0] * 2, st[1] * 2, st[2] * 2}, ROW})) return KITTY_E_OVERLAP;
+    }
+  }
   a.start = start;
   a.counts = counts;
   a.T = T;
@@ -572,6 +582,8 @@ extern "C" int kitty_kv8_expand(const kitty_kv8_layer *layer, const int32_t *len
   if (!lengths || !k_out || !v_out) return KITTY_E_BADARG;
   if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) return KITTY_E_BADARG;
   if (B > 65535 || layer->h_kv > 65535 || n > (1 << 30)) return KITTY_E_BADSHAPE;
+  const int64_t bytes = static_cast<int64_t>(B) * layer->h_kv * n * HD * 2;
+  if (rows_meet({k_out, {1, 1, 1}, {}, bytes}, {v_out, {1, 1, 1}, {}, bytes})) return KITTY_E_OVERLAP;
   ExpandArgs a{*layer, lengths, start, k_out, v_out, n};
   const int64_t blocks = (static_cast<int64_t>(n) + 2 * KV8_BLOCK - 2) / KV8_BLOCK;
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(layer->h_kv), static_cast<unsigned>(B));

@@ -18,6 +18,7 @@
 // fp16 product needs, cost twice the instructions in all and held the kernel at 79 % of the copy bandwidth.
 // tcgen05 has no use here: 16 of 128 tile rows would be filled.
 #include "kv8.cuh"
+#include "overlap.cuh"
 #include "paged_core.cuh"
 
 namespace kitty {
@@ -731,6 +732,8 @@ extern "C" int kitty_kv8_attn(const kitty_kv8_layer *layer, const int32_t *lengt
   if ((reinterpret_cast<uintptr_t>(query) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return KITTY_E_BADARG;
   if (workspace_bytes < need) return KITTY_E_WORKSPACE;
+  const int64_t bytes = static_cast<int64_t>(B) * h_q * HD * 2;
+  if (out != query && rows_meet({out, {1, 1, 1}, {}, bytes}, {query, {1, 1, 1}, {}, bytes})) return KITTY_E_OVERLAP;
   // units are counted in 32 bits
   if (static_cast<int64_t>(B) * layer->max_page * 4 > 0x7fffffff / layer->h_kv) return KITTY_E_BADSHAPE;
   const int sms = sm_count() < KV8_MAX_SMS ? sm_count() : KV8_MAX_SMS;

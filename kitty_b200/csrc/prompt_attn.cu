@@ -32,6 +32,7 @@
 #include <cuda.h>
 
 #include "decode.cuh"
+#include "overlap.cuh"
 #include "tcgen05.cuh"
 
 namespace kitty {
@@ -1007,6 +1008,12 @@ extern "C" int kitty_prompt_attn(const void *q, const void *k, const void *v, in
       a.part_ml = reinterpret_cast<float2 *>(a.part + a.splits * a.rows * h_q * HD);
     }
   }
+  const int64_t row = static_cast<int64_t>(h_q) * HD * 2;
+  const Rows written{out, {packed ? 1 : B, Lq, h_q}, {Lq * row, row, HD * 2}, HD * 2};
+  const void *in[3] = {q, k, v};
+  for (int x = 0; x < 3; ++x)
+    if (rows_meet(written, {in[x], {size[x][0], size[x][1], size[x][2]}, {st[x][0] * 2, st[x][1] * 2, st[x][2] * 2}, HD * 2}))
+      return KITTY_E_OVERLAP;
   const int64_t pairs = prompt_pairs(packed, B, Lq, a.G, a.zero_rest);
   if (!packed) a.pairs = static_cast<int32_t>(B > 0 ? pairs / B : 0);
   const int64_t items = pairs * h_kv * a.splits;

@@ -6,6 +6,7 @@
 #include "rotary.cuh"
 
 #include "decode.cuh"
+#include "overlap.cuh"
 
 namespace kitty {
 
@@ -94,6 +95,12 @@ int launch_rotary(const RotArgs &a, dim3 grid, cudaStream_t s) {
 
 using namespace kitty;
 
+extern "C" int kitty_rows_overlap(const void *x, const int64_t *x_sizes, const int64_t *x_steps, const void *y,
+                                  const int64_t *y_sizes, const int64_t *y_steps, int64_t run) {
+  return rows_meet({x, {x_sizes[0], x_sizes[1], x_sizes[2]}, {x_steps[0], x_steps[1], x_steps[2]}, run},
+                   {y, {y_sizes[0], y_sizes[1], y_sizes[2]}, {y_steps[0], y_steps[1], y_steps[2]}, run});
+}
+
 extern "C" int kitty_rotary(const kitty_rotary_plan *plan, const void *q, const void *k, const int64_t *positions,
                             int64_t pos_stride_b, void *q_out, void *k_out, int dtype, int32_t B, int32_t T,
                             int32_t h_q, int32_t h_kv, const int64_t *strides, void *stream) {
@@ -118,6 +125,18 @@ extern "C" int kitty_rotary(const kitty_rotary_plan *plan, const void *q, const 
       if ((s ? h_kv : h_q) != 0 && ((a.is[s][i] * esize) % 16 != 0 || (a.os[s][i] * esize) % 16 != 0)) return KITTY_E_BADARG;
     }
   }
+  Rows rows[2][2];                 // [query, key][in, out]
+  for (int s = 0; s < 2; ++s) {
+    const int64_t h = s ? h_kv : h_q;
+    for (int o = 0; o < 2; ++o) {
+      const int64_t *st = strides + 3 * s + 6 * o;
+      rows[s][o] = {o ? a.out[s] : a.in[s], {B, h, T}, {st[0] * esize, st[1] * esize, st[2] * esize}, HD * esize};
+    }
+  }
+  for (int s = 0; s < 2; ++s)
+    if ((!same_rows(rows[s][1], rows[s][0]) && rows_meet(rows[s][1], rows[s][0])) || rows_meet(rows[s][1], rows[1 - s][0]))
+      return KITTY_E_OVERLAP;
+  if (rows_meet(rows[0][1], rows[1][1])) return KITTY_E_OVERLAP;
   a.pos = positions;
   a.pos_b = pos_stride_b;
   a.T = T;

@@ -192,7 +192,8 @@ def kv8_attention(query: torch.Tensor, layer: KV8Layer, lengths: torch.Tensor, s
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one query token per row over the lengths[b] tokens (int32 [B], on the device) that row b holds.
     query [B, H_Q, 1, 128] of the layer's type, up to 16 query heads per key head.  Returns [B, 1, H_Q, 128]; a row
-    without tokens is zero.  The scratch is the caller's stream's (torch's allocator), so calls may run side by side."""
+    without tokens is zero.  `out` may be a view of the query's own memory, row for row; other overlaps are refused.  The
+    scratch is the caller's stream's (torch's allocator), so calls may run side by side."""
     if query.dim() != 4 or query.shape[2] != 1:
         raise ValueError(f"expected query [B, H_Q, 1, {layer.D}], got {tuple(query.shape)}")
     _lib.refuse_gradients("kv8_attention", query)

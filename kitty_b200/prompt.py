@@ -77,7 +77,8 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     for a batch padded on the right.  Returns [B, Lq, H_Q, 128]; padding rows are zeros.
     Packed: query [T, H_Q, 128], key / value [Tk, H, 128], cu_seqlens int32 [N + 1] on the device, 0 first and never
     falling, with sequence s at rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (cu_seqlens_k for the keys where they differ).  Returns [T, H_Q, 128]; rows that
-    belong to no sequence behind the last one are zeros in a new tensor and left as they are in a given `out`.
+    belong to no sequence behind the last one are zeros in a new tensor and left as they are in a given `out`.  An `out`
+    that shares memory with an input is refused.
 
     causal: the last query of a sequence sees its last key, so with more keys than queries the queries are a further
     piece of a prompt.  A row that sees no key is zero.  What a row does not see does not reach it, whatever it holds."""

@@ -129,30 +129,15 @@ def _rotary_output(out: torch.Tensor, x: torch.Tensor, what: str):
     rows, strides = _lib.head_rows(out, repeated=False)
     if rows is not out:
         raise ValueError(f"{what}_out needs consecutive channels, rows on 16-byte boundaries and no expanded dimension")
-    same = out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
-    if not same and _spans_overlap(out, x):
-        raise ValueError(f"{what}_out overlaps the {what} without being the same view")
     return out, strides
-
-
-def _span(x: torch.Tensor):
-    last = sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
-    return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size()
-
-
-def _spans_overlap(x: torch.Tensor, y: torch.Tensor) -> bool:
-    if x.numel() == 0 or y.numel() == 0:
-        return False
-    (a, b), (c, d) = _span(x), _span(y)
-    return a < d and c < b
 
 
 def apply_rotary(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor, rotary: RotaryEmbedding, *,
                  query_out: Optional[torch.Tensor] = None, key_out: Optional[torch.Tensor] = None):
     """Turn query [B, H_Q, T, 128] and key [B, H, T, 128] (any strides with consecutive channels, fp16 / bf16 / fp32) by
     `positions` (int64 [T], [1, T] or [B, T]).  Returns (query, key) turned, in new tensors of the same memory order,
-    or in query_out / key_out, which may be query and key themselves (in place); other overlaps of outputs and inputs
-    are the caller's error and refused where the views' spans show them."""
+    or in query_out / key_out, which may be query and key themselves (in place).  An output that shares any other memory
+    with an input or with the other output is refused."""
     dev = rotary.device
     _lib.refuse_gradients("apply_rotary", query, key)
     (q, q_st), (k, k_st) = _rotary_input(query, "query", dev), _rotary_input(key, "key", dev)

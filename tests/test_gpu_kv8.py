@@ -467,3 +467,23 @@ def test_logits_that_are_all_minus_infinity(kb, room):
     q[..., 5] = 1.0
     assert torch.isnan(kb.kv8_attention(q, layer, _i32([7]), SC)).all()
     layer.check()
+
+
+@pytest.mark.parametrize("B,cap,lengths", [(2, 640, [600, 77]), (150, 640, [33, 600] + [96] * 148), (2, 4096, [3900, 100]),
+                                           (300, 9000, [600, 40] + [96] * 298)])
+def test_output_in_the_query_s_own_place(kb, B, cap, lengths):
+    """Row for row over the query, on each of the ways a call can take."""
+    layer = kb.KV8Layer(B, cap, 1, device=DEV, num_pages=1000,
+                        page_table=(torch.arange(B * -(-cap // 128), device=DEV) % 1000).view(B, -1))
+    k, v = _kv(B, 1, 600, torch.bfloat16, 41)
+    n = _i32(lengths)
+    kb.kv8_append(layer, k, v, torch.zeros_like(n), lengths=n.clamp(max=600))
+    q = torch.randn(B, 6, 1, 128, generator=torch.Generator(device=DEV).manual_seed(42), device=DEV).bfloat16()
+    want = kb.kv8_attention(q, layer, n, SC)
+    for _ in range(5):
+        mine = q.clone()
+        got = kb.kv8_attention(mine, layer, n, SC, out=mine.view(B, 1, 6, 128))
+        assert got.data_ptr() == mine.data_ptr() and torch.equal(got, want)
+    buf = torch.zeros(B + 1, 6, 128, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="overlaps"):
+        kb.kv8_attention(buf[:B].view(B, 6, 1, 128), layer, n, SC, out=buf[1:].view(B, 1, 6, 128))

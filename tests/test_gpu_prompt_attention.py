@@ -396,3 +396,29 @@ def test_blocks_that_take_several_items_of_several_tiles(kb, dtype):
     for a, b in zip(cu[:-1].tolist(), cu[1:].tolist()):
         _check_rows(got[a:b], qp[a:b], kp[a:b], vp[a:b], SC, False, (a, b))
     assert kb.prompt_attention_status(DEV) == 0
+
+
+def test_outputs_over_the_inputs_are_refused(kb):
+    """Other rows still read what an output would overwrite; slices of one buffer that only lie between each other are fine."""
+    q, k, v = _inputs((2, 4, 300, 128), (2, 4, 300, 128), torch.float16, 26)
+    want = kb.prompt_attention(q, k, v, SC)
+    wide = torch.zeros(2, 300, 12, 128, dtype=torch.float16, device=DEV)
+    for i, x in enumerate((q, k, v)):
+        wide[:, :, 4 * i:4 * i + 4] = x.transpose(1, 2)
+    a, b, c = (wide[:, :, 4 * i:4 * i + 4].transpose(1, 2) for i in range(3))
+    assert torch.equal(kb.prompt_attention(a, b, c, SC), want)
+    for i in range(3):
+        args = [q, k, v]
+        out = args[i].clone()                                           # [B, H, T, 128] in memory, taken as [B, T, H, 128]
+        args[i] = out
+        with pytest.raises(ValueError, match="overlaps"):
+            kb.prompt_attention(*args, SC, out=out.view(2, 300, 4, 128))
+        assert torch.equal(args[i], (q, k, v)[i])
+    cu = torch.tensor([0, 300], dtype=torch.int32, device=DEV)
+    kp, vp = k[0].transpose(0, 1), v[0].transpose(0, 1)
+    pool = torch.empty(600, 4, 128, dtype=torch.float16, device=DEV)
+    pool[:300] = q[0].transpose(0, 1)
+    with pytest.raises(ValueError, match="overlaps"):
+        kb.prompt_attention(pool[:300], kp, vp, SC, cu_seqlens=cu, out=pool[299:599])
+    got = kb.prompt_attention(pool[:300], kp, vp, SC, cu_seqlens=cu, out=pool[300:])
+    assert torch.equal(got, want[0])

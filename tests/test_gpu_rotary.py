@@ -130,3 +130,19 @@ def test_rows_off_their_boundaries(kb):
     with pytest.raises(ValueError, match="overlaps"):
         kb.apply_rotary(buf[:, :, :5], k, pos, rot, query_out=buf[:, :, 1:])
     assert torch.equal(wide, before)
+
+
+def test_outputs_beside_the_inputs_in_one_buffer(kb):
+    """Slices of one fused projection, turned in place and into other slices of the same buffer."""
+    rot = kb.RotaryEmbedding(device=DEV)
+    fused = torch.randn(2, 40, 24, 128, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV).bfloat16()
+    cut = lambda x, a, b: x[:, :, a:b].transpose(1, 2)                  # noqa: E731
+    pos = torch.arange(40, device=DEV)
+    want = kb.apply_rotary(cut(fused, 0, 8), cut(fused, 8, 12), pos, rot)
+    got = kb.apply_rotary(cut(fused, 0, 8), cut(fused, 8, 12), pos, rot, query_out=cut(fused, 12, 20), key_out=cut(fused, 20, 24))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    a, b = cut(fused, 0, 8), cut(fused, 8, 16)
+    before = fused.clone()
+    with pytest.raises(ValueError, match="overlaps"):
+        kb.apply_rotary(a, b, pos, rot, query_out=b, key_out=a)
+    assert torch.equal(fused, before)

@@ -172,3 +172,80 @@ def test_gradients_are_refused(L):
     L.refuse_gradients("it", x)
     with pytest.raises(ValueError, match="it has no backward pass"):
         L.refuse_gradients("it", x, x.clone().requires_grad_())
+
+
+def _meet(L, x, y, run):
+    """x, y: (address, sizes, steps in bytes)."""
+    (a, n, s), (b, m, t) = x, y
+    return bool(L.lib().kitty_rows_overlap(a, L.i64_array(n), L.i64_array(s), b, L.i64_array(m), L.i64_array(t), run))
+
+
+def test_whether_rows_share_memory(L):
+    """Against the sets of bytes themselves: nested and fused layouts, expanded dimensions, steps that do not nest."""
+    import random
+
+    rng = random.Random(5)
+
+    def bytes_of(at, n, s, run):
+        out = {at}
+        for size, step in zip(n, s):
+            out = {x + i * step for x in out for i in range(size)}
+        return {x + i for x in out for i in range(run)}
+
+    met = apart = 0
+    for _ in range(4000):
+        run = rng.choice([2, 4])
+        n = [[rng.choice([1, 1, 2, 3]) for _ in range(3)] for _ in range(2)]
+        if rng.random() < 0.6:                       # both from one buffer, as slices of a fused projection are
+            st, step = [], run
+            for _ in range(3):
+                st.append(step)
+                step *= rng.choice([2, 3, 4])
+            rng.shuffle(st)
+            s = [st, st]
+        else:
+            s = [[run * rng.randrange(-3, 9) for _ in range(3)] for _ in range(2)]
+        at = 1000 + rng.randrange(-12, 13) * rng.choice([1, run])
+        want = bool(bytes_of(1000, n[0], s[0], run) & bytes_of(at, n[1], s[1], run))
+        assert _meet(L, (1000, n[0], s[0]), (at, n[1], s[1]), run) == want, (n, s, at, run)
+        met, apart = met + want, apart + (not want)
+    assert met > 500 and apart > 500
+    assert not _meet(L, (1000, (0, 2, 1), (4, 8, 16)), (1000, (2, 2, 1), (4, 8, 16)), 4)
+    # rows of 256 bytes, [2, T, 40, 128] in 16 bits: 32 query and 8 key heads of one buffer; the same at 2^31 rows
+    for T in (4096, 1 << 30):
+        st = (T * 10240, 256, 10240)
+        q, k = (1 << 20, (2, 32, T), st), ((1 << 20) + 32 * 256, (2, 8, T), st)
+        assert not _meet(L, q, k, 256) and not _meet(L, k, q, 256) and _meet(L, q, (q[0] + 31 * 256, (2, 8, T), st), 256)
+        assert _meet(L, q, (k[0] + 8 * 256, (2, 8, T), st), 256) and not _meet(L, q, (q[0] + 2 * T * 10240, (1, 1, 1), (0, 0, 0)), 256)
+
+
+def test_outputs_that_share_memory_are_refused(L):
+    """Refused before anything is launched, whatever else the call holds."""
+    H = 256                                           # bytes of a 16-bit row
+    fused = (5 * 12 * 128, 128, 12 * 128)             # [B, T, 12 heads, 128]: heads 0-3 query, 4-7 key, 8-11 others
+    rot = lambda qo, ko: _rotary(L, _plan(L), q=P, k=P + 4 * H, qo=P + qo * H, ko=P + ko * H, B=2, T=5, hq=4, h=4,  # noqa: E731
+                                 st=fused * 4)
+    for qo, ko in ((4, 0), (4, 8), (8, 0), (8, 8), (1, 8), (8, 5), (0, 0), (8, 9), (0, 3)):
+        assert rot(qo, ko) == L.KITTY_E_OVERLAP, (qo, ko)
+    # the same place, but in another order
+    assert _rotary(L, _plan(L), q=P, k=1 << 30, qo=P, ko=1 << 30, B=1, T=5, hq=4, h=4, st=(0, 128, 512) + (0, 640, 128) * 3) \
+        == L.KITTY_E_OVERLAP
+    heads = (7 * 4 * 128, 128, 4 * 128)
+    far = 1 << 30
+    one = dict(B=2, Lq=7, Lk=7, hq=4, h=4, out=P)
+    for where in "qkv":
+        at = dict(q=far, k=2 * far, v=3 * far)
+        for shift in (0, 3 * H, -2 * 7 * 4 * H + H):
+            assert _prompt(L, **{**at, where: P + far + shift}, **{**one, "out": P + far}, st=heads * 3) == L.KITTY_E_OVERLAP
+    assert _prompt(L, q=P, k=far, v=2 * far, **one, st=(7 * 4 * 128, 7 * 128, 128) + heads * 2) == L.KITTY_E_OVERLAP
+    assert _prompt(L, q=P, k=far, v=2 * far, cu=P, **{**one, "B": 1}, st=(0, 128, 512) * 3) == L.KITTY_E_OVERLAP
+    lib, layer = L.lib(), _layer(L, h_kv=2)
+    for shift in (H, -H, 3 * H):
+        assert lib.kitty_kv8_attn(layer, P, far, 2, 2, 1.0, far + shift, P, 1 << 40, None) == L.KITTY_E_OVERLAP
+    assert lib.kitty_kv8_expand(layer, P, None, far, far + 5 * H, 2, 4, None) == L.KITTY_E_OVERLAP
+    st = L.i64_array((2 * 6 * 128, 6 * 128, 128) * 3)
+    for name in ("key", "value", "query"):
+        at = {"key": far, "value": 2 * far, "query": 3 * far}
+        assert lib.kitty_kv8_append(layer, at["key"], at["value"], st, P, None, 2, 6, _plan(L), at["query"], at[name] + 3 * H, 2,
+                                    None) == L.KITTY_E_OVERLAP
+    assert "overlaps" in L.strerror(L.KITTY_E_OVERLAP)
