@@ -19,6 +19,17 @@ HEAD_DIM = 128
 ROPE_LAYOUTS = {"half": _lib.ROPE_HALF, "interleaved": _lib.ROPE_INTERLEAVED}
 
 
+# Fields of a scaling besides rope_type: those it needs, those that it may have.  (rope_theta and partial_rotary_factor are
+# the embedding's base and rotary_dim; a linear scaling has no use for the original length.)
+_COMMON = {"rope_type", "type", "rope_theta", "partial_rotary_factor"}
+_FIELDS = {
+    "default": (set(), set()),
+    "linear": ({"factor"}, {"original_max_position_embeddings"}),
+    "llama3": ({"factor", "original_max_position_embeddings", "low_freq_factor", "high_freq_factor"}, set()),
+    "yarn": ({"factor", "original_max_position_embeddings"}, {"beta_fast", "beta_slow", "attention_factor", "truncate"}),
+}
+
+
 def _scaled_frequencies(rotary_dim: int, base: float, scaling: Optional[dict]):
     """Radians per position of every pair (Python floats) and the factor on cosine and sine, from the fields of a
     transformers configuration's rope parameters."""
@@ -27,11 +38,17 @@ def _scaled_frequencies(rotary_dim: int, base: float, scaling: Optional[dict]):
     if scaling is None:
         return inv, 1.0
     kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if kind not in _FIELDS:
+        raise ValueError(f"rope scaling {kind!r} is not supported ({', '.join(_FIELDS)})")
+    needed, optional = _FIELDS[kind]
+    missing = sorted(f for f in needed if scaling.get(f) is None)
+    if missing:
+        raise ValueError(f"rope scaling {kind!r} needs {', '.join(missing)}")
+    unknown = sorted(set(scaling) - needed - optional - _COMMON)
+    if unknown:
+        raise ValueError(f"rope scaling {kind!r} with {', '.join(unknown)} is not supported")
     if kind == "default":
         return inv, 1.0
-    known = ("linear", "llama3", "yarn")
-    if kind not in known:
-        raise ValueError(f"rope scaling {kind!r} is not supported (default, {', '.join(known)})")
     factor = float(scaling["factor"])
     if not (factor > 0 and math.isfinite(factor)):
         raise ValueError(f"rope scaling factor must be positive, got {factor}")
@@ -51,10 +68,6 @@ def _scaled_frequencies(rotary_dim: int, base: float, scaling: Optional[dict]):
         return out, 1.0
     # yarn: pairs that make beta_fast turns or more over the original context keep their angle, those with beta_slow or
     # fewer are stretched, a ramp over the pair index in between; all sines and cosines are scaled
-    unknown = set(scaling) - {"rope_type", "type", "factor", "original_max_position_embeddings", "beta_fast", "beta_slow",
-                              "attention_factor", "truncate", "rope_theta", "partial_rotary_factor"}
-    if unknown:
-        raise ValueError(f"yarn fields {sorted(unknown)} are not supported")
     if base == 1.0:
         raise ValueError("yarn scaling needs a base other than 1")
 
@@ -81,26 +94,39 @@ def _scaled_frequencies(rotary_dim: int, base: float, scaling: Optional[dict]):
 class RotaryEmbedding:
     """Angles of a model's rotary positions, kept on a CUDA device.
 
-    head_dim: 128.  rotary_dim: channels that turn (even, default all; the rest keep their value).  layout: 'half' (pair
-    p = channels p and p + rotary_dim/2) or 'interleaved' (channels 2p and 2p + 1).  scaling: None or the rope parameters
-    of a transformers configuration, with `rope_type` 'default', 'linear', 'llama3' or 'yarn'."""
+    head_dim: 128.  base: default 10000.  rotary_dim: channels that turn (even, default all; the rest keep their value).
+    layout: 'half' (pair p = channels p and p + rotary_dim/2) or 'interleaved' (channels 2p and 2p + 1).  scaling: None or
+    the rope parameters of a transformers configuration, with `rope_type` 'default', 'linear', 'llama3' or 'yarn'.  Their
+    `rope_theta` is the base and their `partial_rotary_factor` the part of the head that turns; an argument that says
+    otherwise is refused, and so are fields that are not known here."""
 
-    def __init__(self, head_dim: int = HEAD_DIM, base: float = 10000.0, rotary_dim: Optional[int] = None,
+    def __init__(self, head_dim: int = HEAD_DIM, base: Optional[float] = None, rotary_dim: Optional[int] = None,
                  layout: str = "half", scaling: Optional[dict] = None, device="cuda"):
-        rotary_dim = head_dim if rotary_dim is None else int(rotary_dim)
         if head_dim != HEAD_DIM:
             raise ValueError(f"kitty_b200 kernels are built for head_dim=128, got {head_dim}")
+        theta, part = (None, None) if scaling is None else (scaling.get("rope_theta"), scaling.get("partial_rotary_factor"))
+        if theta is not None:
+            if base is not None and float(base) != float(theta):
+                raise ValueError(f"base is {base}, the rope parameters say rope_theta={theta}")
+            base = theta
+        if part is not None:
+            turned = int(head_dim * float(part))
+            if rotary_dim is not None and int(rotary_dim) != turned:
+                raise ValueError(f"rotary_dim is {rotary_dim}, the rope parameters say partial_rotary_factor={part}, that is {turned}")
+            rotary_dim = turned
+        base = 10000.0 if base is None else float(base)
+        rotary_dim = head_dim if rotary_dim is None else int(rotary_dim)
         if rotary_dim < 2 or rotary_dim > head_dim or rotary_dim % 2:
             raise ValueError(f"rotary_dim must be even and in 2 .. {head_dim}, got {rotary_dim}")
         if layout not in ROPE_LAYOUTS:
             raise ValueError(f"layout must be 'half' or 'interleaved', got {layout!r}")
         if not (base > 0 and math.isfinite(base)):
             raise ValueError(f"base must be positive, got {base}")
+        inv, self.factor = _scaled_frequencies(rotary_dim, base, scaling)
         dev = torch.device(device)
         if dev.type != "cuda":
             raise ValueError("kitty_b200 has no CPU path: the angles live on a CUDA device")
-        inv, self.factor = _scaled_frequencies(rotary_dim, float(base), scaling)
-        self.head_dim, self.rotary_dim, self.layout, self.base = head_dim, rotary_dim, layout, float(base)
+        self.head_dim, self.rotary_dim, self.layout, self.base = head_dim, rotary_dim, layout, base
         self.scaling = dict(scaling) if scaling is not None else None
         self.inv_freq = torch.tensor(inv, dtype=torch.float64)                  # radians per position, on the host
         self._turns = torch.tensor([w / (2 * math.pi) for w in inv], dtype=torch.float64, device=dev)

@@ -249,3 +249,62 @@ def test_outputs_that_share_memory_are_refused(L):
         assert lib.kitty_kv8_append(layer, at["key"], at["value"], st, P, None, 2, 6, _plan(L), at["query"], at[name] + 3 * H, 2,
                                     None) == L.KITTY_E_OVERLAP
     assert "overlaps" in L.strerror(L.KITTY_E_OVERLAP)
+
+
+def _angles(monkeypatch, **kw):
+    """What a RotaryEmbedding makes of its arguments before it goes to a device: (rotary_dim, base, scaling)."""
+    import kitty_b200 as kb
+    from kitty_b200 import rotary
+
+    seen = []
+    real = rotary._scaled_frequencies
+    monkeypatch.setattr(rotary, "_scaled_frequencies", lambda *a: seen.append(a) or real(*a))
+    with pytest.raises(ValueError, match="no CPU path"):
+        kb.RotaryEmbedding(device="cpu", **kw)
+    return seen[0]
+
+
+def test_rope_parameters_are_taken_or_refused(monkeypatch):
+    """rope_theta and partial_rotary_factor come with a configuration's rope parameters: honoured, and refused where an
+    argument says otherwise."""
+    from transformers import LlamaConfig
+
+    import kitty_b200 as kb
+
+    cfg = LlamaConfig(rope_parameters={"rope_type": "llama3", "rope_theta": 500000.0, "factor": 8.0, "low_freq_factor": 1.0,
+                                       "high_freq_factor": 4.0, "original_max_position_embeddings": 8192})
+    assert _angles(monkeypatch, scaling=cfg.rope_parameters)[:2] == (128, 500000.0)
+    assert _angles(monkeypatch, scaling=cfg.rope_parameters, base=500000.0, rotary_dim=64)[:2] == (64, 500000.0)
+    assert _angles(monkeypatch, scaling={"rope_type": "default", "rope_theta": 1000000})[:2] == (128, 1000000.0)
+    half = {"rope_type": "linear", "factor": 2.0, "rope_theta": 10000.0, "partial_rotary_factor": 0.5}
+    assert _angles(monkeypatch, scaling=half)[:2] == (64, 10000.0) and _angles(monkeypatch, scaling=half, rotary_dim=64)[0] == 64
+    assert _angles(monkeypatch)[:2] == (128, 10000.0) and _angles(monkeypatch, base=5.0)[:2] == (128, 5.0)
+    for bad, what in ((dict(base=10000.0, scaling=cfg.rope_parameters), "rope_theta"), (dict(rotary_dim=128, scaling=half), "partial_rotary_factor"),
+                      (dict(scaling={"rope_theta": 0.0}), "base must be"), (dict(scaling={**half, "partial_rotary_factor": 0.4}), "rotary_dim")):
+        with pytest.raises(ValueError, match=what):
+            kb.RotaryEmbedding(device="cpu", **bad)
+
+
+def test_scalings_are_refused_by_name():
+    """Each for its own reason."""
+    from kitty_b200.rotary import _scaled_frequencies
+
+    llama3 = {"rope_type": "llama3", "factor": 2.0, "original_max_position_embeddings": 4096, "low_freq_factor": 1.0, "high_freq_factor": 4.0}
+    yarn = {"rope_type": "yarn", "factor": 2.0, "original_max_position_embeddings": 4096}
+    linear = {"rope_type": "linear", "factor": 2.0}
+    for scaling in (llama3, yarn, linear, {"rope_type": "default"}, {"type": "linear", "factor": 3}, {}):
+        assert len(_scaled_frequencies(128, 10000.0, scaling)[0]) == 64
+    for scaling, what in (({"rope_type": "dynamic", "factor": 2.0}, "'dynamic' is not supported"), ({"rope_type": None}, "None is not supported"),
+                          ({**linear, "factor": -1.0}, "factor must be positive"), ({**linear, "factor": math.inf}, "factor must be positive"),
+                          ({"rope_type": "linear"}, "needs factor"), ({**linear, "low_freq_factor": 1.0}, "with low_freq_factor"),
+                          ({"rope_type": "default", "mrope_section": [1]}, "with mrope_section"),
+                          ({"full_attention": linear}, "with full_attention"),
+                          ({**llama3, "high_freq_factor": 1.0}, "high_freq_factor must be above"), ({**llama3, "beta_fast": 3}, "with beta_fast"),
+                          ({k: v for k, v in llama3.items() if k[:4] != "low_"}, "needs low_freq_factor"),
+                          ({**llama3, "original_max_position_embeddings": None}, "needs original_max"),
+                          ({**yarn, "original_max_position_embeddings": 0}, "original_max_position_embeddings must be positive"),
+                          ({**yarn, "mscale": 1.0}, "with mscale"), ({**yarn, "factor": None}, "needs factor")):
+        with pytest.raises(ValueError, match=what):
+            _scaled_frequencies(128, 10000.0, scaling)
+    with pytest.raises(ValueError, match="base other than 1"):
+        _scaled_frequencies(128, 1.0, yarn)
