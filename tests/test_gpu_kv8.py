@@ -487,3 +487,43 @@ def test_output_in_the_query_s_own_place(kb, B, cap, lengths):
     buf = torch.zeros(B + 1, 6, 128, dtype=torch.bfloat16, device=DEV)
     with pytest.raises(ValueError, match="overlaps"):
         kb.kv8_attention(buf[:B].view(B, 6, 1, 128), layer, n, SC, out=buf[1:].view(B, 1, 6, 128))
+
+
+@pytest.mark.parametrize("rotated", [False, True])
+def test_what_refused_and_clamped_appends_store(kb, rotated):
+    """A count below zero or a start outside stores nothing; too many tokens are stored as far as they go.  Other rows of the
+    call are stored as ever."""
+    T, cap = 40, 256
+    rot = kb.RotaryEmbedding(device=DEV) if rotated else None
+    k, v = _kv(2, 2, T, torch.bfloat16, 51)
+    k0, v0 = _kv(2, 2, 250, torch.bfloat16, 52)
+
+    def held(start, n):
+        layer = kb.KV8Layer(2, cap, 2, device=DEV)
+        kb.kv8_append(layer, k0, v0, _i32([0, 0]))                          # 250 tokens each: 26 in the open block
+        if n is not None:
+            kb.kv8_append(layer, k, v, _i32(start), lengths=None if n == "all" else _i32(n), rotary=rot)
+        return layer
+
+    same = lambda a, b, row: all(torch.equal(getattr(a, x).view(2, -1)[row], getattr(b, x).view(2, -1)[row])  # noqa: E731
+                                 for x in ("pages", "tail_k", "tail_v"))
+    before = held(None, None)
+    for start, n, row in (([250, 250], [-3, 5], 0), ([-1, 250], [5, 5], 0), ([257, 250], [5, 5], 0), ([250, 1 << 30], [5, 5], 1),
+                          ([250, -(1 << 31)], [5, 5], 1), ([250, 250], [5, -(1 << 31)], 1)):
+        got = held(start, n)
+        want = held([250, 250], [0, 5] if row == 0 else [5, 0])
+        assert same(got, before, row) and same(got, want, 1 - row), (start, n)
+        with pytest.raises(ValueError, match="length"):
+            got.check()
+    # six of the tokens fit; more than the call has are what it has
+    fits = held([250, 250], [6, 6])
+    fits.check()
+    for n in ("all", [40, 6], [7, 1 << 30]):
+        got = held([250, 250], n)
+        assert same(got, fits, 0) and same(got, fits, 1)
+        with pytest.raises(ValueError, match="length"):
+            got.check()
+    got, want = held([100, 256], [999, 3]), held([100, 256], [40, 0])       # a full row takes nothing
+    assert same(got, want, 0) and same(got, before, 1)
+    with pytest.raises(ValueError, match="length"):
+        got.check()

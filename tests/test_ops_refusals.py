@@ -308,3 +308,17 @@ def test_scalings_are_refused_by_name():
             _scaled_frequencies(128, 10000.0, scaling)
     with pytest.raises(ValueError, match="base other than 1"):
         _scaled_frequencies(128, 1.0, yarn)
+
+
+def test_constructors_refuse_each_for_its_own_reason():
+    import kitty_b200 as kb
+
+    for bad, what in ((dict(head_dim=64), "head_dim=128"), (dict(rotary_dim=3), "rotary_dim must be even"), (dict(rotary_dim=130), "rotary_dim"),
+                      (dict(rotary_dim=0), "rotary_dim"), (dict(layout="pairs"), "layout must be"), (dict(base=0.0), "base must be positive"),
+                      (dict(base=math.inf), "base must be positive"), (dict(base=math.nan), "base must be positive"), ({}, "no CPU path")):
+        with pytest.raises(ValueError, match=what):
+            kb.RotaryEmbedding(**{"device": "cpu", **bad})
+    for bad, what in ((dict(MAX_BS=0), "must be positive"), (dict(MAX_LEN=0), "must be positive"), (dict(H_KV=-1), "must be positive"),
+                      (dict(D=64), "D=128"), (dict(MAX_LEN=(1 << 30) + 1), "2\\^30"), ({}, "no CPU path")):
+        with pytest.raises(ValueError, match=what):
+            kb.KV8Layer(**{**dict(MAX_BS=1, MAX_LEN=128, H_KV=1, device="cpu"), **bad})
