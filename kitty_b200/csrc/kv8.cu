@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(256, APPEND_BLOCKS<MODE>) kv8_append_kernel(co
 
   auto process = [&](int blk, bool kv, bool rows_q) {
     const int t0 = blk * KV8_BLOCK - s;                 // input index of the block's first token
-    const bool full = (blk + 1) * KV8_BLOCK <= end;
+    const bool full = blk < eb;
     const int64_t tail_row = static_cast<int64_t>(b) * L.h_kv * KV8_BLOCK * HD;
     // keys: thread t of token tk holds chunks of eight channels, chunk c from 16t + 8 (c & 1) + 64 (c >> 1)
     const int tk = tid >> 2, t = tid & 3, ik = t0 + tk;
@@ -401,10 +401,9 @@ __global__ void __launch_bounds__(256, APPEND_BLOCKS<MODE>) kv8_append_kernel(co
     __syncthreads();
   };
 
-  const int blk = fb + blockIdx.x;
-  const bool full = (blk + 1) * KV8_BLOCK <= end;
-  const bool kv = n > 0 && (full || (blockIdx.x == 0 && eb == fb));
-  const bool rows_q = MODE != ROT_NONE && a.h_q > 0 && blk * KV8_BLOCK - s < a.T;
+  const int blk = fb + blockIdx.x;               // start and T may be 2^30 each: the token behind the block can pass 2^31
+  const bool kv = n > 0 && (blk < eb || (blockIdx.x == 0 && eb == fb));
+  const bool rows_q = MODE != ROT_NONE && a.h_q > 0 && static_cast<int>(blockIdx.x) * KV8_BLOCK - s % KV8_BLOCK < a.T;
   if (kv || rows_q) process(blk, kv, rows_q);
   // The open block that the call leaves behind overwrites the tails, which the first block reads: the same threads do
   // both, one after the other.
@@ -448,9 +447,10 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const __grid_constant__
     atomicOr(L.status, KITTY_KV8_BAD_LENGTH);
     s = cap;                                            // nothing held there: zeros
   }
-  const int blk = s / KV8_BLOCK + blockIdx.x, t0 = blk * KV8_BLOCK - s;    // output index of the block's first token
+  const int blk = s / KV8_BLOCK + blockIdx.x;
+  const int t0 = static_cast<int>(blockIdx.x) * KV8_BLOCK - s % KV8_BLOCK;     // output index of the block's first token
   if (t0 >= a.n) return;
-  const bool full = (blk + 1) * KV8_BLOCK <= len;
+  const bool full = blk < len / KV8_BLOCK;
   const int64_t page = full ? kv8_page(L, b, blk) : -1;
   const int64_t bh = static_cast<int64_t>(b) * L.h_kv + h;
   T *ko = static_cast<T *>(a.k_out) + bh * a.n * HD, *vo = static_cast<T *>(a.v_out) + bh * a.n * HD;
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(256) kv8_expand_kernel(const __grid_constant__
     expand16<T>(make_uint4(vw[0], vw[1], vw[2], vw[3]), sc.y, x);
     put(vo, tk, c, x);
   } else {
-    const bool held = !full && blk * KV8_BLOCK + tk < len;      // an open block's token; a skipped page gives zeros
+    const bool held = !full && blk == len / KV8_BLOCK && tk < len % KV8_BLOCK;      // an open block's token; a skipped page gives zeros
     const int64_t at = (bh * KV8_BLOCK + tk) * HD + c;
     for (int side = 0; side < 2; ++side) {
       if (held) {

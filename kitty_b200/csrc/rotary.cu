@@ -143,7 +143,7 @@ extern "C" int kitty_rotary(const kitty_rotary_plan *plan, const void *q, const 
   a.h_q = h_q;
   a.h_all = h_q + h_kv;
   a.tt = T < ROT_TOK ? T : ROT_TOK;
-  a.tiles = (T + a.tt - 1) / a.tt;
+  a.tiles = static_cast<int32_t>((static_cast<int64_t>(T) + a.tt - 1) / a.tt);
   const int64_t blocks = static_cast<int64_t>(B) * a.tiles;
   if (blocks > 0x7fffffff) return KITTY_E_BADSHAPE;
   // Few tokens: spread the heads over blocks too, at least four heads each.

@@ -527,3 +527,28 @@ def test_what_refused_and_clamped_appends_store(kb, rotated):
     assert same(got, want, 0) and same(got, before, 1)
     with pytest.raises(ValueError, match="length"):
         got.check()
+
+
+def test_the_last_tokens_of_the_longest_cache(kb):
+    """Positions up to 2^30, in calls of up to 2^30 tokens: block numbers whose tokens pass 2^31."""
+    cap = 1 << 30
+    layer = kb.KV8Layer(1, cap, 1, device=DEV, num_pages=2, page_table=torch.zeros(1, cap // 128, dtype=torch.int64, device=DEV))
+    layer.page_table[0, -1] = 1
+    k, v = _kv(1, 1, 64, torch.bfloat16, 61)
+    one = kb.KV8Layer(1, 64, 1, device=DEV)
+    kb.kv8_append(one, k, v, _i32([0]))
+    kb.kv8_append(layer, k, v, _i32([cap - 64]))
+    layer.check()
+    assert torch.equal(layer.pages[1, :, 2:], one.pages[0, :, :2]) and (layer.pages[0] == 0).all()
+    # the most tokens that a call may have (all of them the same one): those that still fit are stored
+    many = (x[:, :, :1].expand(1, 1, cap, 128) for x in (k, v))
+    kb.kv8_append(layer, *many, _i32([cap - 32]))
+    with pytest.raises(ValueError, match="length"):
+        layer.check()
+    same = kb.KV8Layer(1, 32, 1, device=DEV)
+    kb.kv8_append(same, k[:, :, :1].expand(1, 1, 32, 128), v[:, :, :1].expand(1, 1, 32, 128), _i32([0]))
+    assert torch.equal(layer.pages[1, :, 3], same.pages[0, :, 0]) and torch.equal(layer.pages[1, :, 2], one.pages[0, :, 0])
+    assert (layer.pages[0] == 0).all() and (layer.pages[1, :, :2] == 0).all()
+    ke, ve = kb.kv8_expand(layer, _i32([cap]), 70, start=_i32([cap - 50]))
+    assert torch.equal(ke[0, :, :18], _held(k[0], 32, torch.bfloat16)[:, 14:]) and (ke[0, :, 50:] == 0).all()
+    assert torch.equal(ve[0, :, 18:50], _held(v[0, :, :1].expand(1, 32, 128), 32, torch.bfloat16))
