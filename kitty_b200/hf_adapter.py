@@ -14,7 +14,7 @@ import torch
 import torch.nn.functional as F
 
 from .attention import kitty_attention_forward
-from .prompt import prompt_attention
+from .prompt import check_prompt_attention, prompt_attention
 
 
 def _rotate_half(x):
@@ -103,6 +103,8 @@ def kitty_attention_module_forward(self, hidden_states, position_embeddings=None
                 and q.dtype in (torch.float16, torch.bfloat16)
                 and not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad))):
             out = prompt_attention(q, k, v, self.scaling)
+            if getattr(self, "kitty_prompt_check", False) and not torch.cuda.is_current_stream_capturing():
+                check_prompt_attention()          # once a prompt, behind the last layer's attention
         else:
             out = _prefill_attention(q, k, v, attention_mask, self.scaling).transpose(1, 2)
         past_key_values.quantize_prefill(self.layer_idx)
@@ -130,16 +132,20 @@ def _fused_step_ok(cache, layer_idx: int, q, k, v) -> bool:
 def patch_model(model, prompt_kernel: bool = False) -> int:
     """Install the Kitty call sequence on every self-attention module of `model`.  Returns how many were patched.
     prompt_kernel: 16-bit prompts without a mask, and without gradients, go through `prompt_attention` instead of torch's
-    attention."""
-    n = 0
+    attention; at the last layer the host waits for the prompt once, to raise if a bounded wait on the device ran out."""
+    n, last = 0, None
     cfg = model.config.get_text_config() if hasattr(model.config, "get_text_config") else model.config
     for mod in model.modules():
         if all(hasattr(mod, a) for a in ("q_proj", "k_proj", "v_proj", "o_proj", "layer_idx")):
             mod.num_attention_heads = cfg.num_attention_heads
             mod.num_key_value_heads = cfg.num_key_value_heads
-            mod.kitty_prompt_kernel = prompt_kernel
+            mod.kitty_prompt_kernel, mod.kitty_prompt_check = prompt_kernel, False
+            if last is None or mod.layer_idx > last.layer_idx:
+                last = mod
             mod.forward = types.MethodType(kitty_attention_module_forward, mod)
             n += 1
+    if last is not None:
+        last.kitty_prompt_check = prompt_kernel
     return n
 
 

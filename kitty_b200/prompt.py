@@ -44,6 +44,13 @@ def prompt_attention_status(device="cuda") -> int:
     return 0 if st is None else int(st.item())
 
 
+def check_prompt_attention() -> None:
+    """Synchronise and raise if a wait has run out in a prompt-attention call of any device (its output is not complete)."""
+    for dev, st in list(_status.items()):
+        if int(st.item()):
+            raise _lib.KittyError(_lib.KITTY_E_TIMEOUT, f"prompt_attention on {dev}")
+
+
 def _lengths(x, what: str, n: int, device) -> Optional[torch.Tensor]:
     if x is None:
         return None

@@ -422,3 +422,33 @@ def test_outputs_over_the_inputs_are_refused(kb):
         kb.prompt_attention(pool[:300], kp, vp, SC, cu_seqlens=cu, out=pool[299:599])
     got = kb.prompt_attention(pool[:300], kp, vp, SC, cu_seqlens=cu, out=pool[300:])
     assert torch.equal(got, want[0])
+
+
+def test_patched_model_reports_a_wait_that_ran_out(kb):
+    """Once per prompt the patched model looks at the status word that the kernels set when they give up."""
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    from kitty_b200 import hf_adapter, prompt
+
+    cfg = LlamaConfig(hidden_size=256, intermediate_size=256, num_hidden_layers=3, num_attention_heads=2, num_key_value_heads=1,
+                      head_dim=128, vocab_size=100, max_position_embeddings=512)
+    model = LlamaForCausalLM(cfg).eval().bfloat16().to(DEV)
+    hf_adapter.patch_model(model, prompt_kernel=True)
+    assert [m.self_attn.kitty_prompt_check for m in model.model.layers] == [False, False, True]
+    ids = torch.randint(0, 100, (1, 70), device=DEV)
+    run = lambda: hf_adapter.greedy_decode(model, ids, 2, kb.get_kvcache_kitty(cfg, 1, 256, device=DEV))  # noqa: E731
+    run()
+    word = prompt._status[torch.device(DEV)]
+    word.fill_(1)
+    try:
+        with pytest.raises(kb.KittyError, match="prompt_attention on cuda:0"):
+            run()
+    finally:
+        word.zero_()
+    run()
+    hf_adapter.patch_model(model)                                     # torch's attention: nothing to look at
+    word.fill_(1)
+    try:
+        run()
+    finally:
+        word.zero_()
