@@ -10,6 +10,7 @@ import os
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libkitty_b200.so")
@@ -206,11 +207,16 @@ def dtype_code(dtype) -> int:
 
 
 def refuse_gradients(where: str, *tensors) -> None:
-    """The operators are for serving: a result without a gradient where one is expected would be a silent mistake."""
+    """The operators are for serving: a result without a gradient, or a tangent, where one is expected would be a silent
+    mistake."""
     if torch.is_grad_enabled():
         for x in tensors:
-            if x.requires_grad:
+            if x is not None and x.requires_grad:
                 raise ValueError(f"{where} has no backward pass: call it under torch.no_grad() or with detached tensors")
+    if forward_ad._current_level >= 0:
+        for x in tensors:
+            if x is not None and forward_ad.unpack_dual(x).tangent is not None:
+                raise ValueError(f"{where} has no forward derivative: call it with the primal of a dual tensor")
 
 
 def head_rows(x, repeated: bool = True):

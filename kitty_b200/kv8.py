@@ -139,7 +139,7 @@ def kv8_append(layer: KV8Layer, key: torch.Tensor, value: torch.Tensor, start: t
     (default all).  rotary: the keys are turned on the way, token i of row b by position start[b] + i.  query
     [B, H_Q, T, 128] is then turned by the same positions and returned, [B, H_Q, T, 128] contiguous (all T tokens);
     without it the call returns None."""
-    _lib.refuse_gradients("kv8_append", key, value, key if query is None else query)
+    _lib.refuse_gradients("kv8_append", key, value, query)
     (k, k_st), (v, v_st) = _tokens(key, "key", layer.H_KV, layer), _tokens(value, "value", layer.H_KV, layer)
     B, _, T, _ = k.shape
     if v.shape != k.shape:
@@ -196,7 +196,7 @@ def kv8_attention(query: torch.Tensor, layer: KV8Layer, lengths: torch.Tensor, s
     scratch is the caller's stream's (torch's allocator), so calls may run side by side."""
     if query.dim() != 4 or query.shape[2] != 1:
         raise ValueError(f"expected query [B, H_Q, 1, {layer.D}], got {tuple(query.shape)}")
-    _lib.refuse_gradients("kv8_attention", query)
+    _lib.refuse_gradients("kv8_attention", query, out)
     B, h_q, _, D = query.shape
     q, _ = _tokens(query, "query", h_q, layer)
     if h_q == 0 or h_q % layer.H_KV:

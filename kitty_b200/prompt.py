@@ -90,7 +90,7 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     causal: the last query of a sequence sees its last key, so with more keys than queries the queries are a further
     piece of a prompt.  A row that sees no key is zero.  What a row does not see does not reach it, whatever it holds."""
     packed = cu_seqlens is not None
-    _lib.refuse_gradients("prompt_attention", query, key, value)
+    _lib.refuse_gradients("prompt_attention", query, key, value, out)
     q, q_st = _source(query, "query", query, packed)
     k, k_st = _source(key, "key", query, packed)
     v, v_st = _source(value, "value", query, packed)

@@ -165,7 +165,7 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
     or in query_out / key_out, which may be query and key themselves (in place).  An output that shares any other memory
     with an input or with the other output is refused."""
     dev = rotary.device
-    _lib.refuse_gradients("apply_rotary", query, key)
+    _lib.refuse_gradients("apply_rotary", query, key, query_out, key_out)
     (q, q_st), (k, k_st) = _rotary_input(query, "query", dev), _rotary_input(key, "key", dev)
     B, h_q, T, _ = q.shape
     Bk, h_kv, Tk, _ = k.shape

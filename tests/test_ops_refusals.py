@@ -322,3 +322,37 @@ def test_constructors_refuse_each_for_its_own_reason():
                       (dict(D=64), "D=128"), (dict(MAX_LEN=(1 << 30) + 1), "2\\^30"), ({}, "no CPU path")):
         with pytest.raises(ValueError, match=what):
             kb.KV8Layer(**{**dict(MAX_BS=1, MAX_LEN=128, H_KV=1, device="cpu"), **bad})
+
+
+def test_tangents_and_outputs_that_want_a_gradient_are_refused(L):
+    """A forward-mode dual would lose its tangent, a lent output that autograd tracks its history."""
+    import types
+
+    import torch.autograd.forward_ad as fwd
+
+    import kitty_b200 as kb
+
+    x = torch.zeros(1, 1, 2, 128, dtype=torch.bfloat16)
+    rot = types.SimpleNamespace(device=torch.device("cpu"))
+    layer = types.SimpleNamespace(device=torch.device("cpu"))
+    n = torch.zeros(1, dtype=torch.int32)
+
+    def calls(a, b):
+        return [lambda: kb.apply_rotary(a, b, torch.arange(2), rot), lambda: kb.apply_rotary(b, a, torch.arange(2), rot),
+                lambda: kb.prompt_attention(a, b, b, 1.0), lambda: kb.prompt_attention(b, a, b, 1.0), lambda: kb.prompt_attention(b, b, a, 1.0),
+                lambda: kb.kv8_append(layer, a, b, n), lambda: kb.kv8_append(layer, b, a, n), lambda: kb.kv8_append(layer, b, b, n, query=a),
+                lambda: kb.kv8_attention(a[:, :, :1], layer, n, 1.0)]
+
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for grad in (torch.enable_grad, torch.no_grad):
+            with grad():
+                for call in calls(dual, x):
+                    with pytest.raises(ValueError, match="no forward derivative"):
+                        call()
+        L.refuse_gradients("it", x, None)
+    want = x.clone().requires_grad_()
+    for call in (lambda: kb.apply_rotary(x, x, torch.arange(2), rot, query_out=want), lambda: kb.apply_rotary(x, x, torch.arange(2), rot, key_out=want),
+                 lambda: kb.prompt_attention(x, x, x, 1.0, out=want), lambda: kb.kv8_attention(x[:, :, :1], layer, n, 1.0, out=want[:, :, :1])):
+        with pytest.raises(ValueError, match="no backward pass"):
+            call()
