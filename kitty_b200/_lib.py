@@ -219,6 +219,10 @@ def refuse_gradients(where: str, *tensors) -> None:
                 raise ValueError(f"{where} has no forward derivative: call it with the primal of a dual tensor")
 
 
+# To be called for a lent output once it is written: a tensor that autograd has saved for a backward pass is missed there.
+written = torch.autograd.graph.increment_version
+
+
 def head_rows(x, repeated: bool = True):
     """x [B, H, T, 128], or [T, H, 128] for a packed batch, as the kernels read it, and its (batch, head, token) strides
     (0 where a dimension has size one: views may carry any number there).  That is x itself when its channels are

@@ -206,6 +206,7 @@ def kv8_attention(query: torch.Tensor, layer: KV8Layer, lengths: torch.Tensor, s
     q = q.contiguous()
     lengths = _row_tensor(lengths, "lengths", B, layer)
     need = layer.workspace_bytes(B, h_q)
+    lent = out is not None
     if out is None:
         out = _lib.empty((B, 1, h_q, D), layer.dtype, layer.device)
     elif tuple(out.shape) != (B, 1, h_q, D) or out.dtype != layer.dtype or out.device != layer.device \
@@ -214,4 +215,6 @@ def kv8_attention(query: torch.Tensor, layer: KV8Layer, lengths: torch.Tensor, s
     ws = _lib.empty((need,), torch.uint8, layer.device) if need else None
     _lib.call_on(layer.device, _lib.lib().kitty_kv8_attn, "kitty_kv8_attn", layer.c_layer(), lengths.data_ptr(),
                  q.data_ptr(), B, h_q, float(scaling), out.data_ptr(), None if ws is None else ws.data_ptr(), need)
+    if lent:
+        _lib.written(out)
     return out

@@ -135,4 +135,6 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
                  _lib.dtype_code(q.dtype), _lib.i64_array(q_st + k_st + v_st), B, Lq, Lk, h_q, h_kv, float(scaling),
                  int(causal), *(None if x is None else x.data_ptr() for x in (q_len, k_len, cu_q, cu_k)), out.data_ptr(),
                  int(zero_rest), _status_word(dev), None if ws is None else ws.data_ptr(), need)
+    if not zero_rest:
+        _lib.written(out)
     return out

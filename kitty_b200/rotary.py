@@ -199,4 +199,7 @@ def apply_rotary(query: torch.Tensor, key: torch.Tensor, positions: torch.Tensor
     _lib.call_on(dev, _lib.lib().kitty_rotary, "kitty_rotary", rotary.c_plan(), q.data_ptr(), k.data_ptr(),
                  positions.data_ptr(), positions.stride(0) if rows > 1 else 0, qo.data_ptr(), ko.data_ptr(), code, B, T,
                  h_q, h_kv, strides)
+    for x in (query_out, key_out):
+        if x is not None:
+            _lib.written(x)
     return qo, ko

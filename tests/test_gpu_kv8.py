@@ -552,3 +552,29 @@ def test_the_last_tokens_of_the_longest_cache(kb):
     ke, ve = kb.kv8_expand(layer, _i32([cap]), 70, start=_i32([cap - 50]))
     assert torch.equal(ke[0, :, :18], _held(k[0], 32, torch.bfloat16)[:, 14:]) and (ke[0, :, 50:] == 0).all()
     assert torch.equal(ve[0, :, 18:50], _held(v[0, :, :1].expand(1, 32, 128), 32, torch.bfloat16))
+
+
+def test_autograd_notices_lent_outputs(kb):
+    """A tensor saved for a backward pass and then lent as an output: that backward pass says so."""
+    x = lambda *s: torch.randn(*s, device=DEV).bfloat16()                   # noqa: E731
+    w = torch.ones(1, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    rot, pos = kb.RotaryEmbedding(device=DEV), torch.arange(3, device=DEV)
+    layer, n = kb.KV8Layer(1, 128, 1, device=DEV), _i32([3])
+    kb.kv8_append(layer, x(1, 1, 3, 128), x(1, 1, 3, 128), _i32([0]))
+    q, k, v, o = x(1, 2, 3, 128), x(1, 1, 3, 128), x(1, 1, 3, 128), x(1, 3, 2, 128)
+    o1 = x(1, 1, 2, 128)
+    for saved, call in ((q, lambda: kb.apply_rotary(q, k, pos, rot, query_out=q, key_out=k)),
+                        (k, lambda: kb.apply_rotary(q, k, pos, rot, key_out=k)),
+                        (o, lambda: kb.prompt_attention(q, k, v, SC, out=o)),
+                        (o1, lambda: kb.kv8_attention(q[:, :, :1], layer, n, SC, out=o1))):
+        y = (w * saved).sum()
+        call()
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward()
+    with torch.inference_mode():                                            # and inference tensors are lent as ever
+        q = x(1, 2, 3, 128)
+        kb.apply_rotary(q, k, pos, rot, query_out=q)
+    kb.apply_rotary(q, k, pos, rot, query_out=q)
+    y = (w * k).sum()
+    kb.apply_rotary(q, k, pos, rot)                                         # nothing lent, nothing written
+    y.backward()
