@@ -105,7 +105,8 @@ class KV8Layer:
     def workspace_bytes(self, batch: int, h_q: int) -> int:
         need = self._workspace_need.get((batch, h_q))
         if need is None:
-            need = int(_lib.lib().kitty_kv8_workspace_bytes(batch, self.H_KV, h_q, self.MAX_PAGE))
+            with torch.cuda.device(self.device):        # the plan depends on the device's multiprocessors
+                need = int(_lib.lib().kitty_kv8_workspace_bytes(batch, self.H_KV, h_q, self.MAX_PAGE))
             if need < 0:
                 _lib.check(need, "kitty_kv8_workspace_bytes")
             self._workspace_need[(batch, h_q)] = need

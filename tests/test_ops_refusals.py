@@ -356,3 +356,34 @@ def test_tangents_and_outputs_that_want_a_gradient_are_refused(L):
                  lambda: kb.prompt_attention(x, x, x, 1.0, out=want), lambda: kb.kv8_attention(x[:, :, :1], layer, n, 1.0, out=want[:, :, :1])):
         with pytest.raises(ValueError, match="no backward pass"):
             call()
+
+
+def test_workspaces_are_planned_on_the_tensors_own_device(L, monkeypatch):
+    """How a call is split depends on the device's multiprocessors: the library is asked with that device current."""
+    import types
+
+    import kitty_b200 as kb
+    from kitty_b200 import prompt
+
+    current = ["cuda:0"]
+
+    class Device:
+        def __init__(self, dev):
+            self.dev = str(dev)
+
+        def __enter__(self):
+            current.append(self.dev)
+
+        def __exit__(self, *exc):
+            current.pop()
+
+    asked = []
+    fake = types.SimpleNamespace(kitty_kv8_workspace_bytes=lambda *a: asked.append((current[-1], a)) or 64,
+                                 kitty_prompt_workspace_bytes=lambda *a: asked.append((current[-1], a)) or 64)
+    monkeypatch.setattr(L, "lib", lambda: fake)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    layer = types.SimpleNamespace(_workspace_need={}, H_KV=2, MAX_PAGE=64, device=torch.device("cuda", 1))
+    assert kb.KV8Layer.workspace_bytes(layer, 3, 8) == kb.KV8Layer.workspace_bytes(layer, 3, 8) == 64
+    assert prompt._workspace_need(torch.device("cuda", 2), 1, 7, 9, 4, 2, True, False) == 64
+    assert asked == [("cuda:1", (3, 2, 8, 64)), ("cuda:2", (1, 7, 9, 4, 2, 1, 0))]
+    prompt._workspace_need.cache_clear()
