@@ -17,7 +17,10 @@
 //
 // The running maximum is kept in the logits' own units and allowed to lag: the accumulator is rescaled only when a row's
 // maximum has grown by more than 2^8, by the softmax threads themselves (the product before is complete by then: the
-// commit that announces new logits also covers it).  Weights up to 256 fit the 16-bit types, sums are 32-bit.
+// commit that announces new logits also covers it).  Weights up to 256 fit the 16-bit types, sums are 32-bit.  fp16 weights
+// are held 2^7 times as large (up to 2^15, of 65504): those below 2^-32 of the largest round to nothing, which costs a
+// million of them together 2^-13, and not those below 2^-25, which counted in the sum but were missing from the product
+// (0.1 % with 32768 keys behind a dominant one).
 // Weights are rounded to the inputs' type for the second product (half a step, 2^-9 for bf16, of independent sign, as
 // large as the rounding of the output itself).
 //
@@ -44,6 +47,8 @@ constexpr int PROMPT_SMEM = (2 + KV_STAGES) * TILE_BYTES + 1024;
 constexpr int PROMPT_THREADS = 384;            // three groups of four warps
 constexpr int CLEAN_TILES = 3;                 // value tiles of an item that some row does not see all of, at most
 constexpr float LAG = 8.0f;                    // log2 of how far a maximum may lag
+template <typename T>
+constexpr float SHIFT = __is_same(T, __half) ? 7.0f : 0.0f;      // log2 of the weight of a maximum
 
 struct PromptArgs {
   const void *q, *k, *v;
@@ -52,7 +57,8 @@ struct PromptArgs {
   const int32_t *q_lens, *k_lens, *cu_q, *cu_k;
   int32_t *status;
   float *part;                                 // splits > 1: [splits][rows][h_q][128] accumulators,
-  float2 *part_ml;                             // [splits][rows][h_q] (maximum in base 2, sum; sum -1: sees nothing)
+  float2 *part_ml;                             // [splits][rows][h_q] (maximum in base 2, sum; sum -1: sees nothing); sums
+                                               // and accumulators are 2^SHIFT times as large, all of them
   int64_t rows;                                // output rows of one head
   int32_t B, Lq, Lk, G, h_kv, pairs, causal, zero_rest, splits, items;
   float c;                                     // scaling * log2 e
@@ -86,7 +92,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// 2^x of two numbers (finite, below 2^7) on the multiply-add pipe: x = whole + f with |f| <= 1/2, 2^f by a polynomial of
+// 2^x of two numbers (finite, below 2^16) on the multiply-add pipe: x = whole + f with |f| <= 1/2, 2^f by a polynomial of
 // degree four fitted for the least largest relative error (2.6e-6 = 2^-18.6), the whole part added to the exponent.
 // Below 2^-126 the result stays there: a weight of 1e-38.
 __device__ __forceinline__ uint64_t ex2_poly2(uint64_t x2) {
@@ -115,7 +121,7 @@ __device__ __forceinline__ uint32_t pack2(uint64_t p) {
   }
 }
 
-// Weights of 64 logits, 2^(v c - mc), as 16-bit pairs; returns their sum.  POLY: every eighth pair goes through the
+// Weights of 64 logits, 2^(v c - mc + SHIFT), as 16-bit pairs; returns their sum.  POLY: every eighth pair goes through the
 // polynomial, which takes some of the load off the 16-a-clock exponential unit (for finite logits only): 1.36 PFLOP/s
 // over long unmasked rows; with none, a quarter or three eighths of them 1.35, 1.30 and 1.28.
 template <typename T, bool POLY>
@@ -694,7 +700,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         if (j > 0 && !masked) {
           // The maximum so far is mostly the one to use: the first weights are taken with it while the tile's own maximum
           // is found, and count if no row has outgrown it (nor met a NaN, which this comparison does not pass).
-          const uint64_t nmc2 = pk2(-m * a.c, -m * a.c);
+          const float nmc = fmaf(-m, a.c, SHIFT<T>);
+          const uint64_t nmc2 = pk2(nmc, nmc);
           sum = weights64<T, true>(v, c2, nmc2, w);
           largest(0);
           tmem_wait_ld();
@@ -735,8 +742,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
               tmem_st32(to + 32 * i, reinterpret_cast<const uint32_t *>(o));
             }
           }
-          const float mc = m == -INFINITY ? 0.0f : m * a.c;
-          const uint64_t nmc2 = pk2(-mc, -mc);
+          const float nmc = m == -INFINITY ? 0.0f : fmaf(-m, a.c, SHIFT<T>);
+          const uint64_t nmc2 = pk2(nmc, nmc);
           sum = weights64<T, false>(v, c2, nmc2, w);
           announce(0);
           sum = add2(sum, weights64<T, false>(v + 64, c2, nmc2, w));

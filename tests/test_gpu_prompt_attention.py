@@ -452,3 +452,25 @@ def test_patched_model_reports_a_wait_that_ran_out(kb):
         run()
     finally:
         word.zero_()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("margin", [4.0, 12.0, 18.0, 20.0])
+def test_many_small_weights_behind_a_large_one(kb, dtype, margin):
+    """One key far above 32767 equal ones, whose values alone are not zero: the result is all theirs,
+    n w / (1 + n w) with w = e^-margin."""
+    from kitty_b200 import _lib
+
+    hq, Lq, n = 16, 4096, 32767
+    assert _lib.lib().kitty_prompt_workspace_bytes(1, Lq, n + 1, hq, 1, 0, 0) == 0      # keys not cut in parts
+    q = torch.zeros(1, hq, Lq, 128, dtype=dtype, device=DEV)
+    q[..., 7] = 1.0
+    k, v = torch.zeros(1, 1, n + 1, 128, dtype=dtype, device=DEV), torch.ones(1, 1, n + 1, 128, dtype=dtype, device=DEV)
+    k[:, :, 0, 7], v[:, :, 0] = margin, 0.0
+    got = kb.prompt_attention(q, k, v, 1.0, causal=False)
+    w = torch.tensor(-margin, dtype=torch.float64).exp().item()
+    want = n * w / (1.0 + n * w)
+    # a weight is rounded to half a step, or to half of 2^-31 of the largest where that is more (fp16's smallest number is
+    # 2^-24, and the largest weight 2^7); logits and exponentials are off by 2^-16 of the weight at most; the output's half step
+    part = max(HALF[dtype], 2.0 ** -32 / w if dtype == torch.float16 else 0.0) + 2.0 ** -16
+    assert (got.double() - want).abs().max().item() <= want * (part + HALF[dtype] * (1.0 + part))
