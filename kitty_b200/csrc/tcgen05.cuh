@@ -91,15 +91,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *u) {
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *u) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(addr),
-      "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]),
-      "r"(u[10]), "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15])
-      : "memory");
-}
-
 // ---- matrix products ------------------------------------------------------------ //
 // Shared-memory operand in the 128-byte swizzle: rows of 128 bytes in groups of eight (1024 bytes).
 //   rows = the operand's M or N index, 64 contraction elements each: next 8 rows at `sbo`; lbo unused.
