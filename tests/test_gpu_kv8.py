@@ -578,3 +578,41 @@ def test_autograd_notices_lent_outputs(kb):
     y = (w * k).sum()
     kb.apply_rotary(q, k, pos, rot)                                         # nothing lent, nothing written
     y.backward()
+
+
+@pytest.mark.parametrize("dtype,hq", [(torch.bfloat16, 4), (torch.float16, 7), (torch.bfloat16, 16)])
+def test_attention_long_rows(kb, dtype, hq):
+    """Rows of up to 70000 tokens beside short ones: many partials of one row, and workers that end within rows."""
+    lengths = [70001, 31, 40000, 0, 517]
+    B, pages = len(lengths), [-(-n // 128) for n in lengths]
+    table = torch.zeros(B, max(pages), dtype=torch.int64)
+    at = 0
+    order = torch.randperm(sum(pages), generator=torch.Generator().manual_seed(71))
+    for b, m in enumerate(pages):
+        table[b, :m] = order[at:at + m]
+        at += m
+    layer = kb.KV8Layer(B, max(lengths), 1, dtype=dtype, device=DEV, num_pages=at, page_table=table.to(DEV))
+    k, v = _kv(B, 1, max(lengths), dtype, 72)
+    n = _i32(lengths)
+    kb.kv8_append(layer, k, v, torch.zeros_like(n), lengths=n)
+    q = torch.randn(B, hq, 1, 128, generator=torch.Generator(device=DEV).manual_seed(73), device=DEV).to(dtype)
+    got = kb.kv8_attention(q, layer, n, SC)
+    _attention_check(got, q, layer, lengths, (k, v), SC)
+    assert torch.equal(kb.kv8_attention(q, layer, n, SC), got)
+    layer.check()
+
+
+@pytest.mark.parametrize("room", [0, 4100])
+@pytest.mark.parametrize("size", [30.0, 1000.0])
+def test_a_query_channel_far_above_the_others(kb, room, size):
+    """The other channels keep 1/65024 of it, as the bound says."""
+    lengths = [700, 90]
+    layer = kb.KV8Layer(2, 700 + room, 2, device=DEV)
+    k, v = _kv(2, 2, 700, torch.bfloat16, 81)
+    n = _i32(lengths)
+    kb.kv8_append(layer, k, v, torch.zeros_like(n), lengths=n)
+    q = torch.randn(2, 6, 1, 128, generator=torch.Generator(device=DEV).manual_seed(82), device=DEV)
+    q[..., 77] *= size
+    q = q.bfloat16()
+    _attention_check(kb.kv8_attention(q, layer, n, SC), q, layer, lengths, (k, v), SC)
+    layer.check()
