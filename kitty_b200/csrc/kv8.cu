@@ -89,8 +89,10 @@ __device__ __forceinline__ float kv8_scale(uint32_t m, float &inv, float &pre) {
 
 __device__ __forceinline__ uint32_t max_abs16(uint32_t m, uint32_t w) { return __vmaxu2(m, w & 0x7fff7fffu); }
 
-// Blocks of threads per multiprocessor: four (64 registers) hide more of the memory's latency than three without spills
-// (4 x 4096 rotated tokens, 8 heads: 24 against 28 us); the scalar forms have more state and take two.
+// Blocks of threads per multiprocessor: four (64 registers, which keeps 212 bytes a thread of the rotating half form in
+// local memory, 12 of the plain one) hide more of the memory's latency than three (80 registers: 60 bytes and none).  Between
+// events, from a cold L2, 8 heads: 4 x 4096 rotated tokens 30.7 against 34.8 us, as they are 26.6 against 30.7, 3 x 2000
+// rotated 20.5 against 22.4.  The scalar forms have more state and take two.
 template <int MODE>
 constexpr int APPEND_BLOCKS = MODE == ROT_NONE || MODE == ROT_HALF || MODE == ROT_INTER ? 4 : 2;
 

@@ -11,8 +11,8 @@
 // bytes as they are; records hold them in operand order, so every shared-memory read is one conflict-free 16-byte word
 // per lane.  The other operand is a 16-bit fixed-point number in two bytes, 256 hi + lo, which are two of the tile's
 // sixteen rows (eight heads):
-//   logits   query elements in units of (largest of the head) / 32512: off by at most 2^-16 of the head's largest
-//   weights  in units of (largest of the block's 32 tokens) / 32512: off by at most 2^-16 of that one, so a far larger
+//   logits   query elements in units of (largest of the head) / 32512: off by at most 1/65024 of the head's largest
+//   weights  in units of (largest of the block's 32 tokens) / 32512: off by at most 1/65024 of that one, so a far larger
 //            weight elsewhere in the sequence costs nothing
 // Scales, exponentials, sums and accumulators are 32-bit floats.  Conversions of the codes to 16-bit floats, which an
 // fp16 product needs, cost twice the instructions in all and held the kernel at 79 % of the copy bandwidth.
@@ -131,7 +131,9 @@ struct Kv8Cursor {
   }
 };
 
-// MT: 1 for groups of up to 8 query heads, 2 for up to 16 (two matrix tiles).
+// MT: 1 for groups of up to 8 query heads, 2 for up to 16 (two matrix tiles).  At 168 registers the even split keeps 80
+// bytes a thread in local memory with MT 1 and 280 with MT 2 (32 x 32768 tokens, 2 key heads: 120 us for groups of 8, 142
+// for groups of 16, 82 at the copy bandwidth).
 // ROW 0: the even split over the machine described above, W = KV8_WARPS.  ROW 1 (see kv8_by_row): a block
 // of threads per row, whose W warps share the row's blocks and join their parts in shared memory: no line of units to
 // find one's place in, no second kernel.
@@ -676,7 +678,9 @@ int start_kv8_attn(const Kv8AttnArgs &a, int blocks, cudaStream_t s) {
   return cudaGetLastError() == cudaSuccess ? KITTY_OK : KITTY_E_CUDA;
 }
 
-// Whether a call gives every row a block of threads (lengths are on the device: the rule goes by what a row can hold).
+// Whether a call gives every row a block of threads.  Lengths are on the device: the rule goes by what a row can hold, so a
+// short row in a cache with room for a long one is split and joined (1 x 517 tokens, 8 heads: 6.8 us on the device with room
+// for 640, 10.5 with room for 32768; 16 x 517: 7.3 and 15.3).
 // Up to 1024 tokens a row, while there are at most four rows per multiprocessor: 8 rows of 640 tokens 8.2 us (11.0 evenly
 // split and joined), 256 rows of 1024 16.5 (20.1), but 1024 rows of 640 46.9 (44.5).  Up to 4096, from a row per
 // multiprocessor or nearly on: 128 rows of 4096 26 us (39), 1024 rows of 4096 174 (186), but 8 rows of 4096 20 (12).
@@ -695,9 +699,12 @@ int launch_kv8_attn(const Kv8AttnArgs &a, int blocks, cudaStream_t s) {
                                               : start_kv8_attn<T, MT, 4, true>(a, rows, s);
   const int rc = start_kv8_attn<T, MT, KV8_WARPS, false>(a, blocks, s);
   if (rc != KITTY_OK) return rc;
-  // From 256 rows on a row has nine partials or fewer (1776 workers): folded by a warp each (1024 rows: 5 us, 25 us as
-  // blocks).  Below, a block each: 1024 threads for a few rows of hundreds of partials (8 rows of 222: 9 us, 16 us with
-  // 512 threads), 512 threads when there are more blocks than multiprocessors (64 rows of 28: 7 us, 11 us with 1024).
+  // From 256 rows of about one length on a row has nine partials or fewer (1776 workers): folded by a warp each (1024 rows:
+  // 5 us, 25 us as blocks).  Below, a block each: 1024 threads for a few rows of hundreds of partials (8 rows of 222: 9 us,
+  // 16 us with 512 threads), 512 threads when there are more blocks than multiprocessors (64 rows of 28: 7 us, 11 us with
+  // 1024).  The rule goes by the number of rows, which the host knows, not by their lengths: a long row among hundreds of
+  // short ones has hundreds of partials that one warp folds (40 sequences, 8 heads, one of 131072 tokens and 39 of 500:
+  // 120 us in all, 81 for as many tokens evenly spread; 256 rows, one of 131072: 157).
   const int heads = rows * a.G;
   cudaError_t e;
   if (rows >= 256) e = launch_after(kv8_join_rows_kernel<T>, dim3((heads + 7) / 8), dim3(256), 0, s, a);

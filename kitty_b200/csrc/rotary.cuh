@@ -8,9 +8,10 @@
 // at position 100000).  Sine and cosine are 64-bit too: those of the position's multiple of eight are computed, those of
 // the rest come from the plan's table of eight small steps and are turned on with four multiplications.  (A table of 32
 // steps has a block of 32 tokens compute a quarter of the sines, but in a quarter of its threads and with four times the
-// loads: 4 x 4096 tokens appended in 27.8 us against 26.9 from a cold L2.)  Both round to 32 bits once, to half a step.  (With 32-bit sines the turned keys
-// were off by up to 2^-22, and four times as many of them fell on the other side of a rounding to 16 bits as with exact
-// ones.)  The rotation itself is two fused multiply-adds in 32 bits, rounded once to the data type.
+// loads: 4 x 4096 tokens appended in 27.8 us against 26.9 from a cold L2.)  Both, times the plan's factor, round to 32 bits
+// once, to half a step; a factor other than 1 is itself a 32-bit number, half a step off at most.  (With 32-bit sines the
+// turned keys were off by up to 2^-22, and four times as many of them fell on the other side of a rounding to 16 bits as
+// with exact ones.)  The rotation itself is two fused multiply-adds in 32 bits, rounded once to the data type.
 #pragma once
 
 #include "common.cuh"

@@ -1,9 +1,9 @@
 """The 8-bit cache: pages of 128 tokens behind a page table, a scale for each block of 32 tokens and head.
 
 For layers or models that two bits per value hurt: keys and values are whole numbers -127..127 times one fp32 scale per
-(block, head), a quarter of a percent away from their 16-bit values at the block's largest and half the size of a 16-bit
-cache.  The tokens of a row's open block stay in 16 bits until it is full, as `KittyCache` keeps its Q-buffers, so what
-is stored does not depend on how the tokens were cut into calls.
+(block, head), off by at most 1/254 (0.39 %) of the block's largest and half the size of a 16-bit cache.  The tokens of a
+row's open block stay in 16 bits until it is full, as `KittyCache` keeps its Q-buffers, so what is stored does not depend
+on how the tokens were cut into calls.
 
 The caller keeps the lengths and passes them as device tensors (`start`, `lengths`: int32, one per row), so every call
 can be captured in a CUDA graph and replayed as the sequences grow; `KV8Layer.check()` reports what the kernels had to
@@ -30,7 +30,8 @@ class KV8Layer:
     MAX_BS rows of up to MAX_LEN tokens, H_KV heads of 128 channels; dtype (fp16 or bf16) is the type of the open blocks,
     of the tokens that come in and of the values that go out.  page_table: int64 [MAX_BS, ceil(MAX_LEN / 128)] page rows
     (default: row b's pages side by side); num_pages: page rows of the cache (default: as many as the table has
-    entries).  The table may be changed between calls; entries of pages that no token has reached are never read."""
+    entries).  The table, `layer.page_table`, may be changed between calls, in place or for another contiguous one (one that
+    is not contiguous is copied when the layer is made); entries of pages that no token has reached are never read."""
 
     def __init__(self, MAX_BS: int, MAX_LEN: int, H_KV: int, D: int = 128, *, dtype: torch.dtype = torch.bfloat16,
                  device="cuda", num_pages: Optional[int] = None, page_table: Optional[torch.Tensor] = None):
