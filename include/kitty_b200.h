@@ -434,7 +434,7 @@ typedef struct {
  * query) become tokens start[b], start[b] + 1, ... of row b; counts[b] of them (null: all T).  With a rotary plan the
  * keys are turned on the way by their position in the row, and rounded to the data type before they are stored; the
  * query rows [B, h_q, T, 128] (or null, h_q = 0) are turned by the same positions into q_out [B, h_q, T, 128]
- * (contiguous; no part of key, value or query: KITTY_E_OVERLAP), all T of them.  Tokens that end up in an open block go to the tails, others into their pages: a
+ * (contiguous; the query itself, or no part of key, value and query: KITTY_E_OVERLAP), all T of them.  Tokens that end up in an open block go to the tails, others into their pages: a
  * token-by-token caller and one that gives the whole prompt leave the same bytes. */
 int kitty_kv8_append(const kitty_kv8_layer *layer, const void *key, const void *value, const int64_t *strides,
                      const int32_t *start, const int32_t *counts, int32_t B, int32_t T,

@@ -547,7 +547,8 @@ extern "C" int kitty_kv8_append(const kitty_kv8_layer *layer, const void *key, c
     const void *in[3] = {key, value, query};
     for (int x = 0; x < 3; ++x) {
       const int64_t *st = strides + 3 * x;
-      if (rows_meet(turned, {in[x], {B, x < 2 ? layer->h_kv : h_q, T}, {st[0] * 2, st[1] * 2, st[2] * 2}, ROW})) return KITTY_E_OVERLAP;
+      const Rows read{in[x], {B, x < 2 ? layer->h_kv : h_q, T}, {st[0] * 2, st[1] * 2, st[2] * 2}, ROW};
+      if (!(x == 2 && same_rows(turned, read)) && rows_meet(turned, read)) return KITTY_E_OVERLAP;
     }
   }
   a.start = start;

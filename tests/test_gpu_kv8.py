@@ -616,3 +616,19 @@ def test_a_query_channel_far_above_the_others(kb, room, size):
     q = q.bfloat16()
     _attention_check(kb.kv8_attention(q, layer, n, SC), q, layer, lengths, (k, v), SC)
     layer.check()
+
+
+def test_append_turns_a_query_in_place(kb):
+    """The entry point's rotated query may be the query itself."""
+    from kitty_b200 import _lib
+
+    rot = kb.RotaryEmbedding(rotary_dim=96, device=DEV)
+    k, v = _kv(2, 2, 70, torch.bfloat16, 91)
+    q = torch.randn(2, 6, 70, 128, generator=torch.Generator(device=DEV).manual_seed(92), device=DEV).bfloat16()
+    a, b = (kb.KV8Layer(2, 128, 2, device=DEV) for _ in range(2))
+    start = _i32([0, 5])
+    want = kb.kv8_append(a, k, v, start, rotary=rot, query=q)
+    st = [_lib.head_rows(x)[1] for x in (k, v, q)]
+    _lib.call_on(b.device, _lib.lib().kitty_kv8_append, "kitty_kv8_append", b.c_layer(), k.data_ptr(), v.data_ptr(),
+                 _lib.i64_array(st[0] + st[1] + st[2]), start.data_ptr(), None, 2, 70, rot.c_plan(), q.data_ptr(), q.data_ptr(), 6)
+    assert torch.equal(q, want) and torch.equal(a.pages, b.pages)

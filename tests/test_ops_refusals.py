@@ -243,6 +243,8 @@ def test_outputs_that_share_memory_are_refused(L):
     for shift in (H, -H, 3 * H):
         assert lib.kitty_kv8_attn(layer, P, far, 2, 2, 1.0, far + shift, P, 1 << 40, None) == L.KITTY_E_OVERLAP
     assert lib.kitty_kv8_expand(layer, P, None, far, far + 5 * H, 2, 4, None) == L.KITTY_E_OVERLAP
+    st = L.i64_array((2 * 6 * 128, 6 * 128, 128) * 2 + (2 * 6 * 128, 128, 2 * 128))
+    assert lib.kitty_kv8_append(layer, far, 2 * far, st, P, None, 2, 6, _plan(L), 3 * far, 3 * far, 2, None) == L.KITTY_E_OVERLAP
     st = L.i64_array((2 * 6 * 128, 6 * 128, 128) * 3)
     for name in ("key", "value", "query"):
         at = {"key": far, "value": 2 * far, "query": 3 * far}
