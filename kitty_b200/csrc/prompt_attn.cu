@@ -906,7 +906,9 @@ int64_t prompt_pairs(bool packed, int64_t B, int64_t Lq, int64_t G, bool rest) {
 }
 
 // In how many parts the keys are cut.  Unit: the time of one key tile against a pair of query tiles; a block of threads
-// costs FIXED of them besides its tiles, and joining parts costs a launch and the parts' way through memory.
+// costs FIXED of them besides its tiles, and joining parts costs a launch and the parts' way through memory.  With it
+// 1, 16 and 128 rows over 131072 keys (32 query heads, 8 key heads) take 212, 214 and 226 us, launch and join included, from a
+// cold L2, which is 2.6 times the keys' and values' way through memory: a tile takes its time whatever rows it has.
 int prompt_splits(bool packed, int64_t B, int64_t Lq, int64_t Lk, int64_t h_kv, int64_t G, bool causal) {
   constexpr double FIXED = 2.5, JOIN = 3.0;
   if (Lq == 0 || Lk == 0 || B == 0) return 1;
