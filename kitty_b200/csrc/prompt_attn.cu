@@ -50,6 +50,10 @@ constexpr float LAG = 8.0f;                    // log2 of how far a maximum may 
 template <typename T>
 constexpr float SHIFT = __is_same(T, __half) ? 7.0f : 0.0f;      // log2 of the weight of a maximum
 
+// A wait for something that comes once an item lasts as long as its key tiles do (1.5 us each): their number is added to the
+// limit.
+__device__ __forceinline__ unsigned long long item_limit(int tiles) { return WAIT_LIMIT_NS + 20000ull * tiles; }
+
 struct PromptArgs {
   const void *q, *k, *v;
   void *out;
@@ -633,7 +637,7 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
         __syncwarp();
         for (int j = w.clean; j < w.n; ++j, ++cleaned) {
           const uint32_t at = pos + 2 * j + 1, st = at % KV_STAGES;
-          ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_turn[cleaned & 1]), (cleaned >> 1) & 1) &&
+          ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_turn[cleaned & 1]), (cleaned >> 1) & 1, item_limit(w.n)) &&
                                            mbar_wait_asleep(smem_u32(&bar_full[st]), at / KV_STAGES & 1));
           if (!ok) break;
           clear_odd_values<T>(kv_addr + st * TILE_BYTES + (warp - 10) * (TILE_BYTES / 2), rows + 4 * (j - w.clean));
@@ -756,7 +760,8 @@ __global__ void __launch_bounds__(PROMPT_THREADS, 1)
       step += nb;
       outs += nb > 0;
       tc_fence_after();
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_odd[count & 1]), (count >> 1) & 1));
+      // a tile that sees fewer keys than its neighbour, or none, waits here for the item's end
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait_asleep(smem_u32(&bar_odd[count & 1]), (count >> 1) & 1, item_limit(w_.n)));
       if (ok) {
         const Odd &o = odd[count & 1];
         const bool some = lane < 4 * CLEAN_TILES && (o.rows[0][lane] | o.rows[1][lane]) != 0;

@@ -17,7 +17,7 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
       : "memory");
 }
 // Bounded wait that sleeps in hardware (up to the hint, in ns, per try) instead of spending issue slots of the warps that
-// share the scheduler; false when the phase did not complete within WAIT_LIMIT_NS.
+// share the scheduler; false when the phase did not complete within `limit` ns.
 __device__ __forceinline__ bool mbar_try_asleep(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -29,14 +29,14 @@ __device__ __forceinline__ bool mbar_try_asleep(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_wait_asleep(uint32_t bar, uint32_t parity, unsigned long long limit = WAIT_LIMIT_NS) {
   if (mbar_try_asleep(bar, parity)) return true;
   const unsigned long long t0 = global_ns();
   for (;;) {
 #pragma unroll 1
     for (int i = 0; i < 64; ++i)
       if (mbar_try_asleep(bar, parity)) return true;
-    if (global_ns() - t0 > WAIT_LIMIT_NS) return false;
+    if (global_ns() - t0 > limit) return false;
   }
 }
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {

@@ -474,3 +474,30 @@ def test_many_small_weights_behind_a_large_one(kb, dtype, margin):
     # 2^-24, and the largest weight 2^7); logits and exponentials are off by 2^-16 of the weight at most; the output's half step
     part = max(HALF[dtype], 2.0 ** -32 / w if dtype == torch.float16 else 0.0) + 2.0 ** -16
     assert (got.double() - want).abs().max().item() <= want * (part + HALF[dtype] * (1.0 + part))
+
+
+@pytest.mark.parametrize("hq", [1, 2])
+def test_an_item_that_takes_longer_than_a_wait_may(kb, hq):
+    """One row over 2^28 keys (rows of a small buffer, 16 bytes apart) that are not cut in parts: some two million key tiles in
+    a row, over two seconds, during which those who wait for the item's end wait on."""
+    from kitty_b200 import _lib
+
+    n = (1 << 28) - 5
+    buf = torch.zeros(8 * n + 120, dtype=torch.bfloat16, device=DEV)
+    buf[-928:] = 1.0                                                    # the last 101 rows are all ones, their logits 45
+    k = buf.as_strided((1, 1, n, 128), (8 * n, 8 * n, 8, 1))
+    q = torch.full((1, hq, 1, 128), 4.0, dtype=torch.bfloat16, device=DEV)
+    out = torch.zeros(1, 1, hq, 128, dtype=torch.bfloat16, device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    st = [_lib.head_rows(x, repeated=False) for x in (q, k, k)]
+    assert all(a is b for (a, _), b in zip(st, (q, k, k)))
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    _lib.call_on(q.device, _lib.lib().kitty_prompt_attn, "kitty_prompt_attn", q.data_ptr(), k.data_ptr(), k.data_ptr(), _lib.KITTY_BF16,
+                 _lib.i64_array(st[0][1] + st[1][1] + st[2][1]), 1, 1, n, hq, 1, SC, 1, None, None, None, None, out.data_ptr(), 1,
+                 status.data_ptr(), None, 0)
+    b.record()
+    b.synchronize()
+    # the rows before those, whose first channels are zero, have a 17th of the weight and less: 1 - 0.0006 and up
+    assert int(status.item()) == 0 and (out == 1.0).all()
+    assert a.elapsed_time(b) > 2000.0, a.elapsed_time(b)                # the case in the name
