@@ -88,7 +88,10 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     that shares memory with an input is refused.
 
     causal: the last query of a sequence sees its last key, so with more keys than queries the queries are a further
-    piece of a prompt.  A row that sees no key is zero.  What a row does not see does not reach it, whatever it holds."""
+    piece of a prompt.  A row that sees no key is zero.  What a row does not see does not reach it, whatever it holds.
+
+    Weights are rounded to the inputs' type for the product with the values; over very many keys the tensor cores'
+    additions cost up to about 2^-26 of a result per key (0.1 % at 65536)."""
     packed = cu_seqlens is not None
     _lib.refuse_gradients("prompt_attention", query, key, value, out)
     q, q_st = _source(query, "query", query, packed)
